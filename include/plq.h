@@ -364,6 +364,71 @@ PLQ_API int plq_gemv_tc(const void* a_lo_codes, const void* a_lo_sf, const void*
                         int64_t m, int64_t n, int64_t k_lo, int64_t k_hi,
                         void* y_bf16, int64_t ldy, int32_t* dev_status, int flags, void* stream);
 
+/*
+ * E4M3 quantisers with one float32 scale per block of 128 columns (k % 16 == 0; the last block may be shorter; k <= 32768).
+ * plq_fp8_pack: rows of x (row stride ldx elements, ldx % 8 == 0).
+ *   with residual: h = bf16(residual + x) (row stride ldr), written to h_out [rows, k]; without: h = x
+ *   with gamma (required with a residual): y = gamma * (h * rsqrt(mean(h^2) + eps)) in float32; without: y = h
+ *   per row and block: a = max(max |y|, 2^-100), code = e4m3(y * (448 / a)), scale = a / 448
+ *   codes u8 [rows, k], scales float32 [rows, ceil(k / 128)]
+ * plq_fp8_pack_weight: w bf16 [n, k], a over blocks of 128 rows x 128 columns; scales [ceil(n / 128), ceil(k / 128)].
+ * plq_fp8_unpack: bf16(code * scale); block_rows 1 or 128 says which of the two forms it is.
+ * A block with a value that is not finite gets the scale NaN and codes of zero.
+ * The final norm of a decoder in front of an 8-bit LM head (inference/forward_pass.py:178-181; the head is 16 bits there).
+ */
+PLQ_API int plq_fp8_pack(const void* x_bf16, int64_t ldx, const void* residual_bf16, int64_t ldr, void* h_out_bf16,
+                         const void* gamma_bf16, float eps, int64_t rows, int64_t k, void* codes, void* scales_f32, void* stream);
+PLQ_API int plq_fp8_pack_weight(const void* w_bf16, int64_t n, int64_t k, void* codes, void* scales_f32, void* stream);
+PLQ_API int plq_fp8_unpack(const void* codes, const void* scales_f32, int64_t rows, int64_t k, int64_t block_rows, void* y_bf16,
+                           void* stream);
+
+/*
+ * y[m, n] = sum over K blocks b of sa[m, b] * sw[n / 128, b] * sum_{k in b} a[m, k] w[n, k], float32 sums, for operands as
+ * plq_fp8_pack and plq_fp8_pack_weight make them (k % 16 == 0, any m and n).  y: bf16 or (y_is_f32) float32, row stride ldy.
+ * `flags`: PLQ_FP8_STATIC_W promises that the weight was complete before the kernels that precede this call were launched
+ * (its first bytes are then fetched while they drain); PLQ_FP8_VARIANT(v) picks the kernel (tests and tuning).
+ * `dev_status` as for plq_mixed_gemm.
+ */
+#define PLQ_FP8_STATIC_W       1
+#define PLQ_FP8_AUTO           0
+#define PLQ_FP8_ROWS           1   /* m <= 64: streams the weights once */
+#define PLQ_FP8_128x128        2
+#define PLQ_FP8_PAIR_256x256   3
+#define PLQ_FP8_VARIANT(v)     ((v) << 4)
+PLQ_API int plq_fp8_gemm(const void* a_codes, const void* a_scales_f32, const void* w_codes, const void* w_scales_f32, int64_t m,
+                         int64_t n, int64_t k, void* y, int64_t ldy, int y_is_f32, int32_t* dev_status, int flags, void* stream);
+
+/*
+ * RoPE of a fused QKV projection's queries and keys (as plq_rope_kv_append: float32, one rounding to bf16) and append of keys
+ * and values to an E4M3 cache: codes u8 [batch, t_max, kv_heads, 128], scales float32 [batch, kv_heads, ceil(t_max / 64)], one
+ * per 64 positions and head, a power of two.  For each block that the new positions touch: a = max |new rows|, s = the
+ * smallest 2^e >= a / 448 with e >= -100, at least the block's scale if earlier positions of the sequence lie in the block,
+ * whose codes move to s where it grew; code = e4m3(x / s).  A value that is not finite makes its block's scale NaN and the
+ * codes of the call's rows in it zeros.  Positions behind the last new one are not written.
+ *   cos, sin       float32 [t, 128] (cs_batch_stride 0) or one [t, 128] per sequence, cs_batch_stride elements apart
+ *   pos_dev        device int64: the first new position, one value or (pos_per_sequence) one per sequence; NULL: `pos`
+ * A sequence with a negative position sits out.  One whose new rows do not fit t_max stores nothing and writes
+ * PLQ_DEV_RANGE to `dev_status` (its queries are rotated all the same).
+ */
+PLQ_API int plq_rope_kv_append_fp8(const void* qkv_bf16, int64_t ld, const void* cos_f32, const void* sin_f32, int64_t cs_batch_stride,
+                                   int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, void* q_out_bf16, void* k_codes,
+                                   void* k_scales_f32, void* v_codes, void* v_scales_f32, int64_t t_max, const int64_t* pos_dev,
+                                   int pos_per_sequence, int64_t pos, int32_t* dev_status, void* stream);
+
+/*
+ * Attention of queries [batch, t, heads, 128] (bf16) over such a cache: query i of a sequence sees the positions 0 .. pos + i,
+ * out = softmax(scale * q . k) v, head h reading key head h / (heads / kv_heads).  pos as above; a sequence with a negative
+ * position sees nothing, one with pos + t > t_max is reported (PLQ_DEV_RANGE); their outputs are zeros.
+ *   ctx            an upper bound of pos + t over the sequences (t_max where it is not known): how the work is split
+ *   workspace      plq_fp8_attention_workspace_bytes(...) bytes (0 for most calls), used by this call only
+ * Codes of visible positions have to be finite, as the append writes them; the others may hold anything.
+ */
+PLQ_API int64_t plq_fp8_attention_workspace_bytes(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t ctx);
+PLQ_API int plq_fp8_attention(const void* q_bf16, const void* k_codes, const void* k_scales_f32, const void* v_codes,
+                              const void* v_scales_f32, int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t t_max,
+                              const int64_t* pos_dev, int pos_per_sequence, int64_t pos, int64_t ctx, float scale, void* out_bf16,
+                              void* workspace, int64_t workspace_bytes, int32_t* dev_status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,6 +38,13 @@ SIGNATURES = {
     "plq_unpack_head_rows": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
     "plq_gptq_block_frozen": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
     "plq_gemv_tc": (_i32, [_vp] * 8 + [_i64] * 4 + [_vp, _i64, _vp, _i32, _vp]),
+    "plq_fp8_pack": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _f32, _i64, _i64, _vp, _vp, _vp]),
+    "plq_fp8_pack_weight": (_i32, [_vp, _i64, _i64, _vp, _vp, _vp]),
+    "plq_fp8_unpack": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "plq_fp8_gemm": (_i32, [_vp] * 4 + [_i64] * 3 + [_vp, _i64, _i32, _vp, _i32, _vp]),
+    "plq_rope_kv_append_fp8": (_i32, [_vp, _i64, _vp, _vp] + [_i64] * 5 + [_vp] * 5 + [_i64, _vp, _i32, _i64, _vp, _vp]),
+    "plq_fp8_attention_workspace_bytes": (_i64, [_i64] * 5),
+    "plq_fp8_attention": (_i32, [_vp] * 5 + [_i64] * 5 + [_vp, _i32, _i64, _i64, _f32, _vp, _vp, _i64, _vp, _vp]),
 }
 
 _lib = None

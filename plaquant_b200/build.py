@@ -14,13 +14,14 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libplq_b200.so")
-SOURCES = ["plq_api.cu", "plq_pack.cu", "plq_gemv.cu", "plq_gemv_tc.cu", "plq_gemm.cu", "plq_gptq.cu", "plq_rope.cu"]
-HEADERS = ["plq_common.cuh", "plq_quant.cuh", "plq_tc.cuh", os.path.join("..", "..", "include", "plq.h")]
+SOURCES = ["plq_api.cu", "plq_pack.cu", "plq_gemv.cu", "plq_gemv_tc.cu", "plq_gemm.cu", "plq_gptq.cu", "plq_rope.cu",
+           "plq_fp8_pack.cu", "plq_fp8_gemm.cu", "plq_fp8_cache.cu"]
+HEADERS = ["plq_common.cuh", "plq_quant.cuh", "plq_tc.cuh", "plq_fp8.cuh", os.path.join("..", "..", "include", "plq.h")]
 TORCH_LIB_PATH = os.path.join(HERE, "_plq_torch.so")
 TORCH_SOURCES = ["plq_torch.cpp", os.path.join("..", "..", "include", "plq.h")]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--shared",
+    "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--shared", "--threads", "0",
 ]
 
 

@@ -1,0 +1,590 @@
+// E4M3 product with a float32 scale per block of 128:
+//
+//   Y[m, n] = sum over K blocks b of  sa[m, b] * sw[n / 128, b] * sum_{k in b} A[m, k] W[n, k]
+//
+// A: codes [m, k], scales [m, ceil(k / 128)] (plq_fp8_pack);  W: codes [n, k], scales [ceil(n / 128), ceil(k / 128)].
+// The scales are arbitrary float32 numbers, so the tensor core cannot apply them: each K block of 128 is a product of its
+// own into a fresh tensor-memory accumulator (four tcgen05.mma kind::f8f6f4), and the epilogue warps add it, times its
+// scale, to float32 sums in registers while the next block's MMAs run into another accumulator.
+//
+// Two kernels:
+//   fp8_gemv_kernel<MR>     m <= 64: the weights are the 128-row side of the MMA and the activations the narrow one, so
+//                           that a few rows stream the weights once; bound by HBM (n k bytes).
+//   fp8_gemm_kernel<BN, CG> more rows: 128 x 128 tiles of one CTA or 256 x 256 tiles of a CTA pair; bound by the tensor
+//                           pipe (2 m n k) or, for few tiles, by the chain of one tile.
+//
+// Every wait is bounded; on expiry PLQ_DEV_TIMEOUT goes to the caller's status word and all roles leave their loops.
+#include <cstring>
+
+#include "plq_fp8.cuh"
+#include "plq_quant.cuh"
+
+namespace plq {
+
+struct Fp8GemmArgs {
+  const float* sa;             // [m, kb]
+  const float* sw;             // [ceil(n / 128), kb]
+  void* y;
+  long long ldy;
+  int32_t* status;
+  int m, n, kb;                // kb: K blocks of 128
+  int tiles_m, tiles_n;
+  int vec;                     // rows of y allow stores of 32 (2), 16 (1) bytes or of single elements (0)
+  int static_w;                // weights may be read before the programmatic dependency wait
+  int band;                    // row tiles per band of the tile order
+};
+struct Fp8GemmMaps { CUtensorMap a, w; };
+
+template <typename T> __device__ __forceinline__ T round_out(float v);
+template <> __device__ __forceinline__ float round_out<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 round_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// ---- a few rows ------------------------------------------------------------------------------------------------------
+// MR: activation rows (accumulator columns), 16, 32 or 64.  Tiles of 128 weight rows.  Where there are fewer tiles than
+// CTA slots a cluster of S CTAs shares a tile along K; CTAs 1 .. S-1 hand their sums to CTA 0 through its (by then idle)
+// ring of stages, and CTA 0 adds them in order: results do not depend on timing and no scratch in HBM is needed.
+//   warp 0 producer, warp 1 MMA issuer, warps 2 - 5 epilogue (one weight row per thread)
+template <int MR>
+struct GvCfg {
+  static constexpr int kStages = MR == 64 ? 4 : MR == 32 ? 5 : 6;
+  static constexpr int kXBytes = MR * kStageKBytes;
+  static constexpr int kStageBytes = kABytes + kXBytes;
+  static constexpr int kAcc = MR == 64 ? 4 : 8;                       // accumulators in flight
+  static constexpr int kTmemCols = MR == 16 ? 128 : 256;              // two CTAs share an SM
+  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + 512;
+  static constexpr int kSlotBytes = MR * 128 * 4;                     // one CTA's partial sums
+  static constexpr int kMaxSlices = kStages * kStageBytes / kSlotBytes + 1 < 8 ? kStages * kStageBytes / kSlotBytes + 1 : 8;
+  static constexpr int kThreads = 192;
+  static_assert(kAcc * MR <= kTmemCols, "tensor memory budget");
+  static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
+};
+
+template <int MR, typename OUT>
+__global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant__ Fp8GemmMaps maps, const Fp8GemmArgs g) {
+  using C = GvCfg<MR>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes);
+  uint64_t* empty_bar = full_bar + C::kStages;
+  uint64_t* acc_full = empty_bar + C::kStages;
+  uint64_t* acc_empty = acc_full + C::kAcc;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + C::kAcc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  uint32_t nslice_u;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nslice_u));
+  const int nslice = static_cast<int>(nslice_u), slice = static_cast<int>(cluster_ctarank());
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int s = 0; s < C::kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 4); }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && elect_one()) { prefetch_tmap(&maps.a); prefetch_tmap(&maps.w); }
+  if (warp == 1) {
+    tmem_alloc<1>(tmem_holder, C::kTmemCols);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  pdl_launch_dependents();
+
+  const int kb0 = g.kb * slice / nslice, kb1 = g.kb * (slice + 1) / nslice;
+  const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(nclusters_x());
+  const uint32_t smem_base = smem_u32(smem);
+
+  float acc[MR];                                 // epilogue: this weight row's sums
+#pragma unroll
+  for (int j = 0; j < MR; ++j) acc[j] = 0.0f;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      auto load_w = [&](uint32_t slot, int tile, int kb) {
+        mbar_arrive_expect_tx(&full_bar[slot], C::kStageBytes);
+        tma_load_2d_cg<1>(smem_base + slot * C::kStageBytes, &maps.w, kb * kStageKBytes, tile * kBM, smem_u32(&full_bar[slot]));
+      };
+      auto load_x = [&](uint32_t slot, int kb) {
+        tma_load_2d_cg<1>(smem_base + slot * C::kStageBytes + kABytes, &maps.a, kb * kStageKBytes, 0, smem_u32(&full_bar[slot]));
+      };
+      // Static weights: the first ring fill of weight bytes is requested while the previous kernel drains.
+      uint32_t early = 0;
+      if (g.static_w)
+        for (int tile = first_tile; tile < g.tiles_n && early < C::kStages; tile += tile_step)
+          for (int kb = kb0; kb < kb1 && early < C::kStages; ++kb, ++early) load_w(early, tile, kb);
+      pdl_wait();
+      uint32_t gs = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < g.tiles_n; tile += tile_step)
+        for (int kb = kb0; kb < kb1; ++kb, ++gs) {
+          const uint32_t slot = gs % C::kStages;
+          if (gs >= early) {
+            ok = mbar_wait_bounded(&empty_bar[slot], ((gs / C::kStages) & 1u) ^ 1u, abort_flag);
+            if (!ok) break;
+            load_w(slot, tile, kb);
+          }
+          load_x(slot, kb);
+        }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = make_idesc_e4m3(128, MR);
+      uint32_t gs = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < g.tiles_n; tile += tile_step)
+        for (int kb = kb0; kb < kb1; ++kb, ++gs) {
+          const uint32_t slot = gs % C::kStages, as = gs % C::kAcc;
+          ok = mbar_wait_bounded(&acc_empty[as], ((gs / C::kAcc) & 1u) ^ 1u, abort_flag) &&
+               mbar_wait_bounded(&full_bar[slot], (gs / C::kStages) & 1u, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t w_lo = desc_lo_sw128(smem_base + slot * C::kStageBytes), x_lo = desc_lo_sw128(smem_base + slot * C::kStageBytes + kABytes);
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            tc_mma_e4m3<1>(tmem_base + as * MR, w_lo + 2 * h, kDescHiSw128, x_lo + 2 * h, kDescHiSw128, idesc, h != 0);
+          tc_commit<1>(smem_u32(&empty_bar[slot]));
+          tc_commit<1>(smem_u32(&acc_full[as]));
+        }
+    }
+  } else {
+    // ---- epilogue: thread = weight row; lane l of a warp carries the scales of activation rows l (and l + 32) ----
+    constexpr int kPer = MR > 32 ? 2 : 1;
+    const int trow = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    pdl_wait();
+    uint32_t gs = 0;
+    bool ok = true;
+    for (int tile = first_tile; ok && tile < g.tiles_n; tile += tile_step) {
+#pragma unroll
+      for (int j = 0; j < MR; ++j) acc[j] = 0.0f;
+      const float* sw = g.sw + static_cast<long long>(tile) * g.kb;
+      auto scale = [&](int kb, int p) {
+        const int row = lane + 32 * p;
+        return kb < kb1 && row < g.m && row < MR ? g.sa[static_cast<long long>(row) * g.kb + kb] * sw[kb] : 0.0f;
+      };
+      float next[4][kPer];                       // scales of the next four K blocks, on their way
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int p = 0; p < kPer; ++p) next[i][p] = scale(kb0 + i, p);
+      for (int kb = kb0; ok && kb < kb1; kb += 4) {
+        float f[4][kPer];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int p = 0; p < kPer; ++p) { f[i][p] = next[i][p]; next[i][p] = scale(kb + 4 + i, p); }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!ok || kb + i >= kb1) break;
+          const uint32_t as = gs % C::kAcc;
+          ok = mbar_wait_bounded_warp(&acc_full[as], (gs / C::kAcc) & 1u, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t r[MR / 16][16];
+#pragma unroll
+          for (int c = 0; c < MR / 16; ++c) tc_ld_32x32b_x16(tmem_base + lane_base + as * MR + c * 16, r[c]);
+          tc_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[as]);
+#pragma unroll
+          for (int j = 0; j < MR; ++j)
+            acc[j] = fmaf(__uint_as_float(r[j / 16][j & 15]), __shfl_sync(0xFFFFFFFFu, f[i][j / 32], j & 31), acc[j]);
+          ++gs;
+        }
+      }
+      if (nslice == 1 && ok) {
+        const long long row = static_cast<long long>(tile) * kBM + trow;
+        OUT* y = static_cast<OUT*>(g.y) + row;
+        if (row < g.n) {
+#pragma unroll
+          for (int j = 0; j < MR; ++j)
+            if (j < g.m) y[j * g.ldy] = round_out<OUT>(acc[j]);
+        }
+      }
+    }
+  }
+  if (nslice > 1) {
+    // One tile per cluster.  First barrier: CTA 0's MMAs have read its ring and nothing is on its way into it.
+    const bool sender = slice > 0 && warp >= 2, receiver = slice == 0 && warp >= 2;
+    const int trow = (warp & 3) * 32 + lane;
+    __syncwarp();
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    if (sender) {
+      const uint32_t dst = map_to_cta(smem_base, 0u) + static_cast<uint32_t>((slice - 1) * C::kSlotBytes + trow * 4);
+#pragma unroll
+      for (int j = 0; j < MR; ++j) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + j * 512), "f"(acc[j]) : "memory");
+    }
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    if (receiver && !*abort_flag) {
+      const float* slots = reinterpret_cast<const float*>(smem);
+      for (int s = 0; s < nslice - 1; ++s) {
+#pragma unroll
+        for (int j = 0; j < MR; ++j) acc[j] += slots[s * (C::kSlotBytes / 4) + j * 128 + trow];
+      }
+      const long long row = static_cast<long long>(first_tile) * kBM + trow;
+      OUT* y = static_cast<OUT*>(g.y) + row;
+      if (row < g.n) {
+#pragma unroll
+        for (int j = 0; j < MR; ++j)
+          if (j < g.m) y[j * g.ldy] = round_out<OUT>(acc[j]);
+      }
+    }
+  }
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) atomicExch(g.status, PLQ_DEV_TIMEOUT);
+    const long long t0 = clock64();                    // copies still in flight get time to land
+    while (clock64() - t0 < 400000ll) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem_base, C::kTmemCols);
+  }
+}
+
+// ---- many rows -------------------------------------------------------------------------------------------------------
+// Persistent; warp 0 producer, warp 1 MMA issuer (leader CTA of a pair), then four epilogue warps per 128 columns, each
+// thread one row x 128 columns of float32 sums.  Per K block an epilogue warp reads 128 columns from tensor memory and
+// does 64 packed multiply-adds (128 cycles of the FMA pipe) beside the 256 (128 x 128) or 512 cycles of the block's MMAs.
+template <int BN, int CG>
+struct GmCfg {
+  static constexpr int kBRows = BN / CG;
+  static constexpr int kStageBytes = kABytes + kBRows * kStageKBytes;      // 32 KiB
+  static constexpr int kStages = 6;
+  static constexpr int kAcc = 512 / BN;
+  static constexpr int kEpiWarps = BN / 32;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + 512;
+  static_assert(kStageBytes == 32768 && kSmemBytes <= 232448, "shared memory budget");
+};
+
+// Tile order: bands of `band` row tiles, M fastest inside a band, so that the CTAs running together share operands in L2.
+__device__ __forceinline__ void fp8_tile(int tile, const Fp8GemmArgs& g, int& tm, int& tn) {
+  const int per = g.band * g.tiles_n, b = tile / per, r = tile - b * per, rows = min(g.band, g.tiles_m - b * g.band);
+  tn = r / rows;
+  tm = b * g.band + (r - tn * rows);
+}
+
+template <int BN, int CG, typename OUT>
+__global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(const __grid_constant__ Fp8GemmMaps maps, const Fp8GemmArgs g) {
+  using C = GmCfg<BN, CG>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes);
+  uint64_t* empty_bar = full_bar + C::kStages;
+  uint64_t* acc_full = empty_bar + C::kStages;
+  uint64_t* acc_empty = acc_full + C::kAcc;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + C::kAcc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int s = 0; s < C::kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], C::kEpiWarps * CG); }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && elect_one()) { prefetch_tmap(&maps.a); prefetch_tmap(&maps.w); }
+  if (warp == 1) {
+    tmem_alloc<CG>(tmem_holder, 512);
+    tmem_relinquish<CG>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) {
+    cluster_arrive_release();
+    cluster_wait_acquire();
+  }
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  pdl_launch_dependents();
+
+  const int num_tiles = g.tiles_m * g.tiles_n;
+  const int first = CG == 2 ? static_cast<int>(cluster_id_x()) : static_cast<int>(blockIdx.x);
+  const int step = CG == 2 ? static_cast<int>(nclusters_x()) : static_cast<int>(gridDim.x);
+  const uint32_t smem_base = smem_u32(smem);
+
+  if (warp == 0) {
+    if (elect_one()) {
+      pdl_wait();
+      uint32_t gs = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < num_tiles; tile += step) {
+        int tm, tn;
+        fp8_tile(tile, g, tm, tn);
+        const int row_a = (tm * CG + static_cast<int>(rank)) * kBM, row_b = tn * BN + static_cast<int>(rank) * C::kBRows;
+        for (int kb = 0; kb < g.kb; ++kb, ++gs) {
+          const uint32_t slot = gs % C::kStages;
+          ok = mbar_wait_bounded(&empty_bar[slot], ((gs / C::kStages) & 1u) ^ 1u, abort_flag);
+          if (!ok) break;
+          const uint32_t st = smem_base + slot * C::kStageBytes;
+          // in a pair every load of both CTAs is counted on the leader's barrier
+          const uint32_t bar = smem_u32(&full_bar[slot]) & (CG == 2 ? 0xFEFFFFFFu : 0xFFFFFFFFu);
+          if (leader) mbar_arrive_expect_tx(&full_bar[slot], CG * C::kStageBytes);
+          tma_load_2d_cg<CG>(st, &maps.a, kb * kStageKBytes, row_a, bar);
+          tma_load_2d_cg<CG>(st + kABytes, &maps.w, kb * kStageKBytes, row_b, bar);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one() && leader) {
+      constexpr uint32_t idesc = make_idesc_e4m3(128 * CG, BN);
+      const uint32_t peer_off = CG == 2 ? map_to_cta(smem_u32(full_bar), 1u) - smem_u32(full_bar) : 0u;
+      auto commit_all = [&](uint64_t* bar) {
+        tc_commit<CG>(smem_u32(bar));
+        if constexpr (CG == 2) tc_commit<CG>(smem_u32(bar) + peer_off);
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return CG == 2 ? mbar_wait_bounded_cluster(bar, parity, abort_flag) : mbar_wait_bounded(bar, parity, abort_flag);
+      };
+      const uint32_t a_lo0 = desc_lo_sw128(smem_base), b_lo0 = desc_lo_sw128(smem_base + kABytes);
+      uint32_t gs = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < num_tiles; tile += step)
+        for (int kb = 0; kb < g.kb; ++kb, ++gs) {
+          const uint32_t slot = gs % C::kStages, as = gs % C::kAcc;
+          ok = wait(&acc_empty[as], ((gs / C::kAcc) & 1u) ^ 1u) && wait(&full_bar[slot], (gs / C::kStages) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t off = slot * (C::kStageBytes >> 4);
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            tc_mma_e4m3<CG>(tmem_base + as * BN, a_lo0 + off + 2 * h, kDescHiSw128, b_lo0 + off + 2 * h, kDescHiSw128, idesc, h != 0);
+          commit_all(&empty_bar[slot]);
+          commit_all(&acc_full[as]);
+        }
+    }
+  } else {
+    const int quad = warp & 3, cgp = (warp - 2) >> 2;
+    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t empty_addr = CG == 2 ? map_to_cta(smem_u32(acc_empty), 0u) : smem_u32(acc_empty);
+    pdl_wait();
+    uint32_t gs = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < num_tiles; tile += step) {
+      int tm, tn;
+      fp8_tile(tile, g, tm, tn);
+      const int row = (tm * CG + static_cast<int>(rank)) * kBM + quad * 32 + lane;
+      const int col0 = tn * BN + cgp * 128;
+      // rows and columns behind the end: their operands are zeros, their scales not read
+      const float* sa = g.sa + static_cast<long long>(min(row, g.m - 1)) * g.kb;
+      const float* sw = g.sw + static_cast<long long>(min(col0, g.n - 1) / kFp8Block) * g.kb;
+      float2 acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
+      float na = sa[0], nw = sw[0];
+      for (int kb = 0; kb < g.kb; ++kb, ++gs) {
+        const uint32_t as = gs % C::kAcc;
+        const float f = na * nw;
+        if (kb + 1 < g.kb) { na = sa[kb + 1]; nw = sw[kb + 1]; }
+        ok = mbar_wait_bounded_warp(&acc_full[as], (gs / C::kAcc) & 1u, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + lane_base + as * BN + cgp * 128;
+        const float2 f2 = make_float2(f, f);
+        uint32_t r[2][16];
+        tc_ld_32x32b_x16(taddr, r[0]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          tc_wait_ld();
+          if (c < 7) tc_ld_32x32b_x16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
+          else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(empty_addr + 8u * as);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            acc[c * 8 + j] = __ffma2_rn(make_float2(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1])), f2, acc[c * 8 + j]);
+        }
+      }
+      if (!ok) break;
+      if (row < g.m) {
+        OUT* y = static_cast<OUT*>(g.y) + row * g.ldy;
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {                       // 16 columns at a time
+          const int col = col0 + v * 16;
+          const float2* s = acc + v * 8;
+          if (g.vec && col + 16 <= g.n) {
+            if constexpr (sizeof(OUT) == 4) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                __stcs(reinterpret_cast<float4*>(y + col) + i, make_float4(s[2 * i].x, s[2 * i].y, s[2 * i + 1].x, s[2 * i + 1].y));
+            } else {
+              uint32_t d[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) d[i] = f32x2_to_bf16x2(s[i].x, s[i].y);
+              if (g.vec == 2)
+                asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(y + col), "r"(d[0]), "r"(d[1]), "r"(d[2]),
+                             "r"(d[3]), "r"(d[4]), "r"(d[5]), "r"(d[6]), "r"(d[7]) : "memory");
+              else {
+                __stcs(reinterpret_cast<uint4*>(y + col), make_uint4(d[0], d[1], d[2], d[3]));
+                __stcs(reinterpret_cast<uint4*>(y + col + 8), make_uint4(d[4], d[5], d[6], d[7]));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (col + 2 * i < g.n) y[col + 2 * i] = round_out<OUT>(s[i].x);
+              if (col + 2 * i + 1 < g.n) y[col + 2 * i + 1] = round_out<OUT>(s[i].y);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) atomicExch(g.status, PLQ_DEV_TIMEOUT);
+    const long long t0 = clock64();                    // copies still in flight get time to land
+    while (clock64() - t0 < 400000ll) __nanosleep(1000);
+    __syncthreads();
+  }
+  if constexpr (CG == 2) {          // the leader's MMAs read the peer's shared memory: leave together
+    tc_fence_before();
+    cluster_arrive_release();
+    cluster_wait_acquire();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<CG>(tmem_base, 512);
+  }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+// Raises the kernel's shared-memory limit once per thread and device.
+template <typename K>
+static int allow_smem(K kernel, size_t bytes, int* done_dev) {
+  int dev = 0;
+  PLQ_CUDA_TRY(cudaGetDevice(&dev));
+  if (*done_dev != dev) {
+    PLQ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    *done_dev = dev;
+  }
+  return PLQ_OK;
+}
+
+template <typename K>
+static int launch_clusters(K kernel, unsigned grid, unsigned cluster, unsigned threads, size_t smem, void* stream, const Fp8GemmMaps& tm,
+                           const Fp8GemmArgs& g) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tm, g));
+  return PLQ_OK;
+}
+
+struct Fp8Ptrs { const void *a, *w; int64_t k; };
+
+template <int MR, typename OUT>
+static int launch_gemv(const Fp8Ptrs& p, Fp8GemmArgs& g, void* stream) {
+  using C = GvCfg<MR>;
+  auto kernel = fp8_gemv_kernel<MR, OUT>;
+  static thread_local int done_dev = -1;
+  int st = allow_smem(kernel, C::kSmemBytes, &done_dev);
+  if (st != PLQ_OK) return st;
+  Fp8GemmMaps tm;
+  memset(&tm, 0, sizeof(tm));
+  if ((st = make_tmap(&tm.w, p.w, g.n, p.k, kBM)) != PLQ_OK) return st;
+  if ((st = make_tmap(&tm.a, p.a, g.m, p.k, MR)) != PLQ_OK) return st;
+  g.tiles_n = (g.n + kBM - 1) / kBM;
+  const int slots = 2 * sm_count();
+  int slices = slots / g.tiles_n;
+  if (slices > C::kMaxSlices) slices = C::kMaxSlices;
+  if (slices > g.kb) slices = g.kb;
+  if (slices < 1) slices = 1;
+  const int grid = slices > 1 ? g.tiles_n * slices : (g.tiles_n < slots ? g.tiles_n : slots);
+  return launch_clusters(kernel, static_cast<unsigned>(grid), static_cast<unsigned>(slices), C::kThreads, C::kSmemBytes, stream, tm, g);
+}
+
+template <int BN, int CG, typename OUT>
+static int launch_gemm_fp8(const Fp8Ptrs& p, Fp8GemmArgs& g, void* stream) {
+  using C = GmCfg<BN, CG>;
+  auto kernel = fp8_gemm_kernel<BN, CG, OUT>;
+  static thread_local int done_dev = -1;
+  int st = allow_smem(kernel, C::kSmemBytes, &done_dev);
+  if (st != PLQ_OK) return st;
+  Fp8GemmMaps tm;
+  memset(&tm, 0, sizeof(tm));
+  if ((st = make_tmap(&tm.a, p.a, g.m, p.k, kBM)) != PLQ_OK) return st;
+  if ((st = make_tmap(&tm.w, p.w, g.n, p.k, C::kBRows)) != PLQ_OK) return st;
+  g.tiles_m = (g.m + kBM * CG - 1) / (kBM * CG);
+  g.tiles_n = (g.n + BN - 1) / BN;
+  // The operand walked in the inner direction should stay in L2: narrow bands when A is the larger one and too big for that.
+  const int64_t a_bytes = static_cast<int64_t>(g.m) * p.k, w_bytes = static_cast<int64_t>(g.n) * p.k;
+  g.band = a_bytes > w_bytes && a_bytes > (32ll << 20) ? 4 : g.tiles_m;
+  if (g.band > g.tiles_m) g.band = g.tiles_m;
+  const int slots = sm_count() / CG, tiles = g.tiles_m * g.tiles_n;
+  return launch_clusters(kernel, static_cast<unsigned>((tiles < slots ? tiles : slots) * CG), CG, C::kThreads, C::kSmemBytes, stream, tm, g);
+}
+
+template <typename OUT>
+static int launch_fp8(const Fp8Ptrs& p, Fp8GemmArgs& g, int variant, void* stream) {
+  if (variant == PLQ_FP8_AUTO) {
+    const int64_t sms = sm_count(), pairs = sms / 2 > 0 ? sms / 2 : 1;
+    const int64_t wide = (g.m + 255ll) / 256 * ((g.n + 255ll) / 256), small = (g.m + 127ll) / 128 * ((g.n + 127ll) / 128);
+    if (g.m <= 64) variant = PLQ_FP8_ROWS;
+    else variant = (wide + pairs - 1) / pairs * 2 <= (small + sms - 1) / sms ? PLQ_FP8_PAIR_256x256 : PLQ_FP8_128x128;
+  }
+  if (variant == PLQ_FP8_ROWS) {
+    if (g.m > 64) return PLQ_ERR_SHAPE;
+    if (g.m <= 16) return launch_gemv<16, OUT>(p, g, stream);
+    return g.m <= 32 ? launch_gemv<32, OUT>(p, g, stream) : launch_gemv<64, OUT>(p, g, stream);
+  }
+  if (variant == PLQ_FP8_128x128) return launch_gemm_fp8<128, 1, OUT>(p, g, stream);
+  if (variant == PLQ_FP8_PAIR_256x256) return launch_gemm_fp8<256, 2, OUT>(p, g, stream);
+  return PLQ_ERR_SHAPE;
+}
+
+}  // namespace plq
+
+extern "C" int plq_fp8_gemm(const void* a_codes, const void* a_scales_f32, const void* w_codes, const void* w_scales_f32, int64_t m, int64_t n,
+                            int64_t k, void* y, int64_t ldy, int y_is_f32, int32_t* dev_status, int flags, void* stream) {
+  using namespace plq;
+  const int variant = flags >> 4;
+  if (m < 1 || n < 1 || k < 16 || k % 16 != 0 || ldy < n || variant < 0 || variant > PLQ_FP8_PAIR_256x256) return PLQ_ERR_SHAPE;
+  if (m > (1 << 30) || n > (1 << 30) || k > (1 << 24) || (m + 127) / 128 * ((n + 127) / 128) > 0x7FFFFFFF) return PLQ_ERR_LIMIT;
+  if (!a_codes || !a_scales_f32 || !w_codes || !w_scales_f32 || !y || !dev_status) return PLQ_ERR_NULL;
+  const uintptr_t es = y_is_f32 ? 4 : 2;
+  if (!aligned16(a_codes) || !aligned16(w_codes) || (reinterpret_cast<uintptr_t>(a_scales_f32) & 3u) || (reinterpret_cast<uintptr_t>(w_scales_f32) & 3u) ||
+      reinterpret_cast<uintptr_t>(y) % es != 0)
+    return PLQ_ERR_ALIGN;
+  const int st = device_check();
+  if (st != PLQ_OK) return st;
+  Fp8GemmArgs g;
+  memset(&g, 0, sizeof(g));
+  g.sa = static_cast<const float*>(a_scales_f32);
+  g.sw = static_cast<const float*>(w_scales_f32);
+  g.y = y;
+  g.ldy = ldy;
+  g.status = dev_status;
+  g.m = static_cast<int>(m);
+  g.n = static_cast<int>(n);
+  g.kb = static_cast<int>((k + kFp8Block - 1) / kFp8Block);
+  g.static_w = flags & PLQ_FP8_STATIC_W;
+  const auto fits = [&](uintptr_t bytes) { return reinterpret_cast<uintptr_t>(y) % bytes == 0 && static_cast<uintptr_t>(ldy) * es % bytes == 0; };
+  g.vec = fits(32) ? 2 : fits(16) ? 1 : 0;
+  const Fp8Ptrs p = {a_codes, w_codes, k};
+  return y_is_f32 ? launch_fp8<float>(p, g, variant, stream) : launch_fp8<__nv_bfloat16>(p, g, variant, stream);
+}

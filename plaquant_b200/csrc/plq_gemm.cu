@@ -451,6 +451,20 @@ int make_tmap(CUtensorMap* tm, const void* base, int64_t rows, int64_t row_bytes
   return r == CUDA_SUCCESS ? PLQ_OK : PLQ_ERR_TENSORMAP;
 }
 
+// u8 [depth, rows, row_bytes], box = 1 x box_rows x box_bytes, 128-byte swizzle, zero fill out of bounds.
+int make_tmap_3d(CUtensorMap* tm, const void* base, int64_t row_bytes, int64_t rows, int64_t depth, int box_bytes, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return PLQ_ERR_TENSORMAP;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(depth)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(row_bytes) * static_cast<cuuint64_t>(rows)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_bytes), static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? PLQ_OK : PLQ_ERR_TENSORMAP;
+}
+
 // Tiled scale buffer as int32 [128 words, chunks per group, groups]; box = 4 chunks of `box_groups` groups.
 int make_sf_tmap(CUtensorMap* tm, const void* base, int64_t chunks, int64_t groups, int box_groups) {
   EncodeTiledFn fn = encode_fn();

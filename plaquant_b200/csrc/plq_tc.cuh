@@ -41,6 +41,8 @@ __host__ __device__ constexpr uint32_t make_idesc(uint32_t fmt, uint32_t m, uint
 // Host side (defined in plq_gemm.cu).
 // u8 matrix [rows, row_bytes], box = 128 bytes x box_rows, 128-byte swizzle, zero fill out of bounds.
 int make_tmap(CUtensorMap* tm, const void* base, int64_t rows, int64_t row_bytes, int box_rows);
+// u8 [depth, rows, row_bytes], box = 1 x box_rows x box_bytes, 128-byte swizzle, zero fill out of bounds.
+int make_tmap_3d(CUtensorMap* tm, const void* base, int64_t row_bytes, int64_t rows, int64_t depth, int box_bytes, int box_rows);
 // Tiled scale buffer as int32 [128 words, chunks per group, groups]; box = 4 chunks of `box_groups` groups.
 int make_sf_tmap(CUtensorMap* tm, const void* base, int64_t chunks, int64_t groups, int box_groups);
 

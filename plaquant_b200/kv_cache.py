@@ -11,6 +11,8 @@ Hadamard (`rotate_heads`), which leaves q . k unchanged up to quantisation error
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from . import ops
@@ -75,3 +77,63 @@ def unpack_head_rows(rows: torch.Tensor) -> torch.Tensor:
     p = ops.PackedMatrix(n, HEAD_DIM, 0, flat[:, : HEAD_DIM // 2].contiguous(), flat[:, HEAD_DIM // 2:].contiguous(),
                          empty, empty, ops.SF_ROWMAJOR)
     return ops.unpack(p).view(*rows.shape[:-1], HEAD_DIM)
+
+
+CACHE_BLOCK = 64        # positions that share a scale of an Fp8Cache
+
+
+@dataclass
+class Fp8Cache:
+    """Keys and values of one layer in E4M3, `room` positions for each sequence of a batch, heads of 128.  One scale per
+    64 positions and head, a power of two: value = code * scale.  Positions nobody has written may hold anything.
+    ops.rope_kv_append_fp8 fills it in place, ops.fp8_cache_attention reads it; 1.03 bytes per 2 of a bf16 cache."""
+    k: torch.Tensor           # u8 [B, room, kv_heads, 128]
+    k_scale: torch.Tensor     # float32 [B, kv_heads, ceil(room / 64)]
+    v: torch.Tensor
+    v_scale: torch.Tensor
+
+    @classmethod
+    def empty(cls, batch: int, room: int, kv_heads: int, device) -> "Fp8Cache":
+        def side():
+            return (torch.empty(batch, room, kv_heads, HEAD_DIM, dtype=torch.uint8, device=device),
+                    torch.empty(batch, kv_heads, -(-room // CACHE_BLOCK), dtype=torch.float32, device=device))
+        return cls(*side(), *side())
+
+    @property
+    def batch(self) -> int:
+        return self.k.shape[0]
+
+    @property
+    def room(self) -> int:
+        return self.k.shape[1]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.k.shape[2]
+
+    def check(self, batch: int, kv_heads: int, device) -> None:
+        """Raises unless this is a well-formed cache of `batch` sequences on `device`."""
+        room = self.room
+        for name, c, s in (("k", self.k, self.k_scale), ("v", self.v, self.v_scale)):
+            if c.dtype != torch.uint8 or tuple(c.shape) != (batch, room, kv_heads, HEAD_DIM) or not c.is_contiguous():
+                raise TypeError(f"cache.{name} must be contiguous uint8 {[batch, room, kv_heads, HEAD_DIM]}, it is {c.dtype} {list(c.shape)}")
+            if s.dtype != torch.float32 or tuple(s.shape) != (batch, kv_heads, -(-room // CACHE_BLOCK)) or not s.is_contiguous():
+                raise TypeError(f"cache.{name}_scale must be contiguous float32 {[batch, kv_heads, -(-room // CACHE_BLOCK)]}")
+            if c.device != device or s.device != device:
+                raise RuntimeError(f"cache.{name} is on {c.device}, the call on {device}")
+
+    def grown(self, room: int) -> "Fp8Cache":
+        """A cache with room for `room` positions that holds what this one does."""
+        new = Fp8Cache.empty(self.batch, room, self.kv_heads, self.k.device)
+        for old, dst in ((self.k, new.k), (self.v, new.v)):
+            dst[:, : self.room].copy_(old)
+        for old, dst in ((self.k_scale, new.k_scale), (self.v_scale, new.v_scale)):
+            dst[..., : old.shape[-1]].copy_(old)
+        return new
+
+    def values(self, t: int):
+        """bf16 keys and values [B, t, kv_heads, 128] of the first `t` positions."""
+        def side(codes, scale):
+            s = scale[..., : -(-t // CACHE_BLOCK)].repeat_interleave(CACHE_BLOCK, -1)[..., :t]
+            return (codes[:, :t].view(torch.float8_e4m3fn).float() * s.transpose(1, 2)[..., None]).to(torch.bfloat16)
+        return side(self.k, self.k_scale), side(self.v, self.v_scale)

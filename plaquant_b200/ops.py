@@ -411,3 +411,232 @@ def gemv_tc(a: PackedMatrix, b: PackedMatrix, out: Optional[torch.Tensor] = None
                                     _stream(a.device))
     _lib.check(st)
     return y
+
+
+# ---- E4M3 with a scale per block of 128 ------------------------------------------------------------------------------
+FP8_BLOCK = 128
+
+
+@dataclass
+class Fp8Matrix:
+    """E4M3 matrix with one float32 scale per 128 columns of a row (block_rows = 1: activations) or per 128 x 128 block
+    (block_rows = 128: weights); the last block of either direction may be shorter.  Value = code * scale."""
+    codes: torch.Tensor      # u8 [rows, k], k a multiple of 16
+    scales: torch.Tensor     # float32 [ceil(rows / block_rows), ceil(k / 128)]
+    block_rows: int
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def k(self) -> int:
+        return self.codes.shape[1]
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + 4 * self.scales.numel()
+
+
+def _fp8_buffers(rows: int, k: int, block_rows: int, device) -> Fp8Matrix:
+    return Fp8Matrix(torch.empty(rows, k, dtype=torch.uint8, device=device),
+                     torch.empty(-(-rows // block_rows), -(-k // FP8_BLOCK), dtype=torch.float32, device=device), block_rows)
+
+
+def _check_fp8(p: Fp8Matrix, name: str, block_rows: Optional[int] = None) -> None:
+    """Only addresses reach a kernel: whatever does not have the layout it reads is refused here."""
+    _require_cuda(p.codes, name)
+    if p.block_rows not in (1, FP8_BLOCK) or (block_rows is not None and p.block_rows != block_rows):
+        raise ValueError(f"{name} has a scale per {p.block_rows} rows" + (f", {block_rows} are needed here" if block_rows else ""))
+    if p.codes.dtype != torch.uint8 or p.codes.dim() != 2 or not p.codes.is_contiguous():
+        raise TypeError(f"{name}.codes must be contiguous uint8 [rows, k]")
+    want = (-(-p.rows // p.block_rows), -(-p.k // FP8_BLOCK))
+    if p.scales.dtype != torch.float32 or tuple(p.scales.shape) != want or not p.scales.is_contiguous() or p.scales.device != p.codes.device:
+        raise TypeError(f"{name}.scales must be contiguous float32 {list(want)} on {p.codes.device}")
+
+
+def _rows_of(x: torch.Tensor, name: str):
+    """bf16 [..., k] as rows with a common stride (copied only where there is none): (tensor [rows, k], stride)."""
+    _require_cuda(x, name)
+    if x.dtype != torch.bfloat16 or x.dim() < 1:
+        raise TypeError(f"{name} must be bfloat16 [..., K]")
+    k = x.shape[-1]
+    x2 = x.reshape(x.numel() // k if k else 0, k)
+    if x2.shape[0] == 1 and x2.stride(1) == 1:
+        return x2 if x2.data_ptr() % 16 == 0 else x2.clone(), k
+    if x2.stride(1) != 1 or x2.stride(0) < k or x2.stride(0) % 8 or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2, x2.stride(0)
+
+
+def _check_gamma(gamma: torch.Tensor, k: int, device) -> torch.Tensor:
+    if gamma.dtype != torch.bfloat16 or gamma.numel() != k:
+        raise TypeError("gamma must be bfloat16 [K]")
+    if gamma.device != device:
+        raise RuntimeError(f"gamma is on {gamma.device}, x on {device}")
+    gamma = gamma.contiguous()
+    return gamma if gamma.data_ptr() % 16 == 0 else gamma.clone()
+
+
+def fp8_pack(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Fp8Matrix:
+    """[RMSNorm(gamma, eps)] -> E4M3 with a scale per row and 128 columns, of bf16 x[..., K] (K a multiple of 16, at most
+    32768).  The normalised values are quantised from float32.  A block with a value that is not finite is NaN as a whole."""
+    x2, ld = _rows_of(x, "x")
+    rows, k = x2.shape
+    p = _fp8_buffers(rows, k, 1, x.device)
+    if gamma is not None:
+        gamma = _check_gamma(gamma, k, x.device)
+    with torch.cuda.device(x.device):
+        st = _lib.lib().plq_fp8_pack(_ptr(x2), ld, None, 0, None, _ptr(gamma), float(eps), rows, k, _ptr(p.codes), _ptr(p.scales),
+                                     _stream(x.device))
+    _lib.check(st)
+    return p
+
+
+def add_rmsnorm_fp8_pack(x: torch.Tensor, residual: torch.Tensor, gamma: torch.Tensor, eps: float):
+    """h = residual + x (bf16) -> RMSNorm(gamma, eps) -> E4M3 as fp8_pack.  Returns (h, packed): the residual add, the norm
+    and the quantiser of an 8-bit product in one pass."""
+    if x.shape != residual.shape or x.device != residual.device:
+        raise TypeError("x and residual must be bfloat16 tensors of one shape on one device")
+    x2, ld = _rows_of(x, "x")
+    r2, ldr = _rows_of(residual, "residual")
+    rows, k = x2.shape
+    gamma = _check_gamma(gamma, k, x.device)
+    h = torch.empty(rows, k, dtype=torch.bfloat16, device=x.device)
+    p = _fp8_buffers(rows, k, 1, x.device)
+    with torch.cuda.device(x.device):
+        st = _lib.lib().plq_fp8_pack(_ptr(x2), ld, _ptr(r2), ldr, _ptr(h), _ptr(gamma), float(eps), rows, k, _ptr(p.codes),
+                                     _ptr(p.scales), _stream(x.device))
+    _lib.check(st)
+    return h.view(x.shape), p
+
+
+def fp8_pack_weight(w: torch.Tensor) -> Fp8Matrix:
+    """E4M3 with a scale per 128 x 128 block, of a bf16 weight [N, K] (K a multiple of 16, at most 32768)."""
+    _require_cuda(w, "w")
+    if w.dtype != torch.bfloat16 or w.dim() != 2:
+        raise TypeError("w must be bfloat16 [N, K]")
+    w = w.contiguous()
+    if w.data_ptr() % 16:
+        w = w.clone()
+    p = _fp8_buffers(*w.shape, FP8_BLOCK, w.device)
+    with torch.cuda.device(w.device):
+        st = _lib.lib().plq_fp8_pack_weight(_ptr(w), *w.shape, _ptr(p.codes), _ptr(p.scales), _stream(w.device))
+    _lib.check(st)
+    return p
+
+
+def fp8_unpack(p: Fp8Matrix) -> torch.Tensor:
+    """Dequantise to bf16 [rows, K]."""
+    _check_fp8(p, "p")
+    y = torch.empty(p.rows, p.k, dtype=torch.bfloat16, device=p.device)
+    with torch.cuda.device(p.device):
+        st = _lib.lib().plq_fp8_unpack(_ptr(p.codes), _ptr(p.scales), p.rows, p.k, p.block_rows, _ptr(y), _stream(p.device))
+    _lib.check(st)
+    return y
+
+
+FP8_GEMM_VARIANTS = {None: 0, "auto": 0, "rows": 1, "128x128": 2, "pair256x256": 3}
+
+
+def fp8_gemm(a: Fp8Matrix, w: Fp8Matrix, out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16,
+             static_weights: bool = False, variant: Optional[str] = None) -> torch.Tensor:
+    """y[m, n] = deq(a) @ deq(w).T, float32 sums, bf16 or float32 (`out_dtype`, or that of `out`).  `static_weights`: w was
+    complete long before this call, so that its first bytes may be fetched while the previous kernel of the stream drains.
+    `variant` picks the kernel ("rows" for up to 64 rows, "128x128", "pair256x256"); default: by the sizes."""
+    _check_fp8(a, "a", 1)
+    _check_fp8(w, "w", FP8_BLOCK)
+    if a.k != w.k:
+        raise ValueError(f"K mismatch: activations {a.k}, weights {w.k}")
+    if a.device != w.device:
+        raise RuntimeError(f"a is on {a.device}, w on {w.device}")
+    dtype = out_dtype if out is None else out.dtype
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("out must be bfloat16 or float32")
+    if out is None:
+        y = torch.empty(a.rows, w.rows, dtype=dtype, device=a.device)
+    else:
+        y = out
+        if y.device != a.device:
+            raise RuntimeError(f"out is on {y.device}, the product on {a.device}")
+        if tuple(y.shape) != (a.rows, w.rows) or (y.numel() and y.stride(1) != 1 and w.rows > 1) or (a.rows > 1 and y.stride(0) < w.rows):
+            raise RuntimeError(f"out {tuple(y.shape)} with strides {tuple(y.stride())} does not hold [{a.rows}, {w.rows}] with contiguous rows")
+    if a.rows == 0 or w.rows == 0:
+        return y
+    if a.k == 0:
+        raise ValueError("K must be at least 16")
+    ld = max(y.stride(0), w.rows) if a.rows > 1 else w.rows
+    with torch.cuda.device(a.device):
+        st = _lib.lib().plq_fp8_gemm(_ptr(a.codes), _ptr(a.scales), _ptr(w.codes), _ptr(w.scales), a.rows, w.rows, a.k, y.data_ptr(), ld,
+                                     int(dtype == torch.float32), _ptr(status_word(a.device)),
+                                     int(static_weights) | FP8_GEMM_VARIANTS[variant] << 4, _stream(a.device))
+    _lib.check(st)
+    return y
+
+
+def _positions(pos, batch: int, device):
+    """`pos` as (device pointer or None, one per sequence?, host value)."""
+    if not isinstance(pos, torch.Tensor):
+        return None, 0, int(pos)
+    if pos.dtype != torch.int64 or pos.numel() not in (1, batch) or pos.device != device or not pos.is_contiguous():
+        raise TypeError("pos must be an int or a contiguous int64 tensor with one element, or one per sequence, on the device of the call")
+    return pos.data_ptr(), int(pos.numel() == batch and batch != 1), 0
+
+
+def rope_kv_append_fp8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, heads: int, kv_heads: int, cache, pos) -> torch.Tensor:
+    """RoPE on the query and key heads of `qkv` (bf16 [B, T, (heads + 2 kv_heads) * 128]) and append of the rotated keys and
+    the values to `cache` (a kv_cache.Fp8Cache of B sequences) at positions pos .. pos + T - 1, one kernel.  `cos` / `sin`:
+    float32 with T * 128 elements (one row per new position) or B * T * 128 (sequences at different positions).  `pos`: an
+    int, or a device int64 tensor with one element or one per sequence; a sequence with a negative position sits out.
+    Returns the rotated queries, bf16 [B, T, heads, 128]."""
+    _require_cuda(qkv, "qkv")
+    b, t, n = qkv.shape
+    if qkv.dtype != torch.bfloat16 or not qkv.is_contiguous() or n != (heads + 2 * kv_heads) * 128:
+        raise TypeError("qkv must be contiguous bfloat16 [B, T, (heads + 2 kv_heads) * 128]")
+    for name, c in (("cos", cos), ("sin", sin)):
+        if c.dtype != torch.float32 or c.numel() not in (t * 128, b * t * 128) or not c.is_contiguous() or c.device != qkv.device:
+            raise TypeError(f"{name} must be contiguous float32 with T * 128 or B * T * 128 elements")
+    if cos.numel() != sin.numel():
+        raise TypeError("cos and sin must have the same number of elements")
+    cache.check(b, kv_heads, qkv.device)
+    ptr, each, host = _positions(pos, b, qkv.device)
+    q = torch.empty(b, t, heads, 128, dtype=torch.bfloat16, device=qkv.device)
+    with torch.cuda.device(qkv.device):
+        st = _lib.lib().plq_rope_kv_append_fp8(
+            _ptr(qkv), n, _ptr(cos), _ptr(sin), t * 128 if cos.numel() != t * 128 else 0, b, t, heads, kv_heads, _ptr(q), _ptr(cache.k),
+            _ptr(cache.k_scale), _ptr(cache.v), _ptr(cache.v_scale), cache.room, ptr, each, host, _ptr(status_word(qkv.device)),
+            _stream(qkv.device))
+    _lib.check(st)
+    return q
+
+
+def fp8_cache_attention(q: torch.Tensor, cache, pos, scale: Optional[float] = None, ctx: Optional[int] = None) -> torch.Tensor:
+    """Attention of bf16 queries [B, T, heads, 128] over a kv_cache.Fp8Cache: query i of a sequence sees the positions
+    0 .. pos + i (the T queries are the last ones appended).  heads is a multiple of the cache's key heads.  `pos` as in
+    rope_kv_append_fp8; the output of a sequence with a negative position is zero.  `scale`: default 128 ** -0.5.  `ctx`:
+    an upper bound of pos + T for positions in device memory (default: the cache's room); it only decides how the work is
+    split.  Returns bf16 [B, T, heads, 128]."""
+    _require_cuda(q, "q")
+    if q.dtype != torch.bfloat16 or q.dim() != 4 or q.shape[-1] != 128 or not q.is_contiguous():
+        raise TypeError("q must be contiguous bfloat16 [B, T, heads, 128]")
+    b, t, heads, _ = q.shape
+    kv_heads = cache.kv_heads
+    cache.check(b, kv_heads, q.device)
+    ptr, each, host = _positions(pos, b, q.device)
+    if ptr is None and host >= 0:
+        ctx = min(host + t, cache.room)
+    elif ctx is None:
+        ctx = cache.room
+    L = _lib.lib()
+    out = torch.empty_like(q)
+    need = L.plq_fp8_attention_workspace_bytes(b, t, heads, kv_heads, ctx)
+    with torch.cuda.device(q.device):
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        st = L.plq_fp8_attention(_ptr(q), _ptr(cache.k), _ptr(cache.k_scale), _ptr(cache.v), _ptr(cache.v_scale), b, t, heads, kv_heads,
+                                 cache.room, ptr, each, host, ctx, 128 ** -0.5 if scale is None else float(scale), _ptr(out), _ptr(ws), need,
+                                 _ptr(status_word(q.device)), _stream(q.device))
+    _lib.check(st)
+    return out
