@@ -1,0 +1,388 @@
+"""The E4M3 key / value cache: append (RoPE, block scales, growth of a block's scale) to the last bit against a restatement of
+its definition, attention against float64."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BLOCK = 64
+
+
+@pytest.fixture(scope="module")
+def plq():
+    import plaquant_b200
+    from plaquant_b200 import kv_cache  # noqa: F401
+    return plaquant_b200
+
+
+def _cache(plq, batch, room, kv_heads, seed=0):
+    """A cache whose unwritten positions hold anything: random bytes (NaN codes among them) and scales."""
+    g = torch.Generator().manual_seed(seed)
+    c = plq.kv_cache.Fp8Cache.empty(batch, room, kv_heads, "cuda")
+    for codes, scale in ((c.k, c.k_scale), (c.v, c.v_scale)):
+        codes.copy_(torch.randint(0, 256, codes.shape, generator=g, dtype=torch.uint8))
+        scale.copy_(torch.randn(scale.shape, generator=g))
+        scale.view(-1)[::3] = float("nan")
+    return c
+
+
+def _clone(plq, c):
+    return plq.kv_cache.Fp8Cache(c.k.clone(), c.k_scale.clone(), c.v.clone(), c.v_scale.clone())
+
+
+def _same(a, b):
+    return all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip((a.k, a.k_scale, a.v, a.v_scale), (b.k, b.k_scale, b.v, b.v_scale)))
+
+
+def _angles(positions):
+    inv = 1.0 / (500000.0 ** (torch.arange(0, 128, 2, dtype=torch.float64) / 128))
+    ang = positions.double().cpu()[..., None] * inv
+    ang = torch.cat([ang, ang], -1)
+    return ang.cos().float().cuda().contiguous(), ang.sin().float().cuda().contiguous()
+
+
+def _rope(x, cos, sin):
+    """x * cos + rotate_half(x) * sin, every float32 operation rounded on its own, one rounding to bf16."""
+    f = x.float()
+    return (f * cos + torch.cat([-f[..., 64:], f[..., :64]], -1) * sin).to(torch.bfloat16)
+
+
+def _scale_of(amax):
+    """The smallest 2^e >= amax / 448 with e >= -100."""
+    m, e = math.frexp(amax)
+    return 2.0 ** max(e - (9 if m <= 0.875 else 8), -100) if amax > 0 else 2.0 ** -100
+
+
+def _append_side(codes, scales, new, pos):
+    """One sequence: new [t, kv_heads, 128] bf16 into codes [room, kv_heads, 128], scales [kv_heads, blocks], on the CPU."""
+    t = new.shape[0]
+    for block in range(pos // BLOCK, (pos + t - 1) // BLOCK + 1):
+        lo, hi = block * BLOCK, min(block * BLOCK + BLOCK, pos + t)
+        start = max(lo, pos)
+        for h in range(new.shape[1]):
+            x = new[start - pos:hi - pos, h].float()
+            old = float(scales[h, block]) if start > lo else 0.0
+            if not (torch.isfinite(x).all() and old == old):
+                scales[h, block] = float("nan")
+                codes[start:hi, h] = 0
+                continue
+            s = max(_scale_of(float(x.abs().max())), old)
+            if start > lo and s != old:
+                was = codes[lo:start, h].contiguous().view(torch.float8_e4m3fn).float()
+                codes[lo:start, h] = (was * (old / s)).to(torch.float8_e4m3fn).view(torch.uint8)
+            codes[start:hi, h] = (x / torch.tensor(s)).to(torch.float8_e4m3fn).view(torch.uint8)
+            scales[h, block] = s
+
+
+def _append(plq, cache, qkv, cos, sin, heads, kv_heads, pos):
+    """The definition, in place on a CPU copy; returns (rotated queries, cache on the GPU)."""
+    b, t, _ = qkv.shape
+    x = qkv.view(b, t, -1, 128)
+    cos, sin = cos.view(-1, t, 1, 128), sin.view(-1, t, 1, 128)
+    k, v = _rope(x[:, :, heads:heads + kv_heads], cos, sin).cpu(), x[:, :, heads + kv_heads:].cpu()
+    side = [[c.cpu(), s.cpu()] for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale))]
+    for i in range(b):
+        if pos[i] < 0:
+            continue
+        for (codes, scales), new in zip(side, (k, v)):
+            _append_side(codes[i], scales[i], new[i], pos[i])
+    return _rope(x[:, :, :heads], cos, sin), plq.kv_cache.Fp8Cache(*(x.cuda() for s in side for x in s))
+
+
+def _qkv(b, t, heads, kv_heads, seed, gain=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(b, t, (heads + 2 * kv_heads), 128, generator=g) * gain
+    x[..., ::29] *= 6.0
+    x *= torch.exp2(torch.randint(-3, 4, (b, t, 1, 1), generator=g).float())          # rows of different size: scales that grow
+    return x.flatten(2).to(torch.bfloat16).cuda()
+
+
+@pytest.mark.parametrize("b,t,heads,kv_heads,pos", [
+    (1, 1, 1, 1, [0]), (1, 1, 4, 1, [63]), (2, 1, 8, 2, [64, 64]), (3, 5, 2, 2, [60, 60, 60]), (1, 64, 4, 4, [0]), (1, 65, 4, 2, [0]),
+    (2, 200, 8, 4, [37, 37]), (1, 700, 4, 1, [130]),
+    (3, 1, 8, 8, [0, 5, 127]), (4, 3, 4, 2, [61, 0, 126, 199]), (3, 130, 6, 3, [1, 63, 64]), (3, 2, 4, 2, [-1, 7, -5])])
+@pytest.mark.parametrize("where", ["host", "device"])
+def test_append_bit_exact(plq, b, t, heads, kv_heads, pos, where):
+    same = len(set(pos)) == 1
+    if where == "host" and not same:
+        pytest.skip("sequences at different positions are given in device memory")
+    room = max(max(pos), 0) + t + 3
+    cache = _cache(plq, b, room, kv_heads, 1)
+    for step in range(3):                              # from an empty cache, and behind what the calls before left
+        start = [p if p < 0 else (0 if step == 0 else p) for p in pos]
+        n = t if step else max(max(pos), 1)             # the first call fills up to the largest position
+        qkv = _qkv(b, n, heads, kv_heads, 10 + step, gain=(1.0, 2.0, 0.5)[step])
+        at = torch.tensor(start)[:, None] + torch.arange(n)
+        cos, sin = _angles(at if not same else at[0])
+        want_q, want = _append(plq, cache, qkv, cos, sin, heads, kv_heads, start)
+        p = start[0] if where == "host" else torch.tensor(start if not same or b == 1 else start[:1], dtype=torch.int64, device="cuda")
+        q = plq.ops.rope_kv_append_fp8(qkv, cos, sin, heads, kv_heads, cache, p)
+        assert torch.equal(q, want_q)
+        assert _same(cache, want)
+    plq.check_device_status()
+
+
+def test_append_token_by_token_with_growing_values(plq):
+    """Every token larger than the one before: the block's scale moves with almost every call."""
+    heads, kv_heads = 2, 2
+    cache = _cache(plq, 1, 130, kv_heads, 2)
+    for i in range(130):
+        qkv = _qkv(1, 1, heads, kv_heads, 100 + i, gain=2.0 ** (i % 64 - 20))
+        cos, sin = _angles(torch.tensor([i]))
+        _, want = _append(plq, cache, qkv, cos, sin, heads, kv_heads, [i])
+        plq.ops.rope_kv_append_fp8(qkv, cos, sin, heads, kv_heads, cache, i)
+        assert _same(cache, want)
+
+
+def test_append_values_at_the_border_of_a_scale(plq):
+    """448, 2^-100 * 448, zeros, the largest and the smallest bf16, not finite ones."""
+    for i, v in enumerate([448.0, 450.0, 447.0, 0.0, 3.38e38, 1e-38, 2.0 ** -100 * 448, 2.0 ** -91, -448.0, float("inf"), float("-inf"), float("nan")]):
+        cache = _cache(plq, 1, 70, 1, 3)
+        qkv = torch.zeros(1, 66, 3 * 128, dtype=torch.bfloat16, device="cuda")
+        qkv[0, 3, 128 + 17] = v
+        qkv[0, 5, 256 + 100] = v
+        qkv[0, 7, 256:] = 1.0
+        cos, sin = torch.ones(66, 128, device="cuda"), torch.zeros(66, 128, device="cuda")
+        _, want = _append(plq, cache, qkv, cos, sin, 1, 1, [0])
+        plq.ops.rope_kv_append_fp8(qkv, cos, sin, 1, 1, cache, 0)
+        if v == v and abs(v) < 1e39:
+            assert _same(cache, want), v
+        else:
+            assert cache.v_scale[0, 0, 0].isnan() and not cache.v_scale[0, 0, 1].isnan()
+            assert torch.all(cache.v[0, :64] == 0)
+
+
+def test_append_refuses_what_does_not_fit(plq):
+    heads, kv_heads = 4, 2
+    cache = _cache(plq, 2, 100, kv_heads, 4)
+    qkv = _qkv(2, 3, heads, kv_heads, 5)
+    cos, sin = _angles(torch.arange(3))
+    before = _clone(plq, cache)
+    with pytest.raises(plq.PlqError):
+        plq.ops.rope_kv_append_fp8(qkv, cos, sin, heads, kv_heads, cache, 98)
+    plq.ops.rope_kv_append_fp8(qkv, cos, sin, heads, kv_heads, cache, torch.tensor([98, -1], device="cuda"))
+    assert _same(cache, before)
+    with pytest.raises(plq.PlqError):
+        plq.check_device_status()
+    plq.check_device_status()
+
+
+# ---- attention -------------------------------------------------------------------------------------------------------
+def _filled(plq, batch, room, kv_heads, lengths, seed, gain=1.0):
+    """A cache filled by the append itself, `lengths` positions of every sequence, anything behind them."""
+    cache = _cache(plq, batch, room, kv_heads, seed)
+    n = max(lengths)
+    if n > 0:
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x = torch.randn(batch, n, 3 * kv_heads, 128, generator=g, device="cuda") * gain
+        x[..., ::37] *= 4.0
+        full = plq.kv_cache.Fp8Cache.empty(batch, n, kv_heads, "cuda")
+        ones = torch.ones(n, 128, device="cuda")
+        plq.ops.rope_kv_append_fp8(x.flatten(2).to(torch.bfloat16), ones, torch.zeros_like(ones), kv_heads, kv_heads, full, 0)
+        for i, m in enumerate(lengths):
+            cache.k[i, :m], cache.v[i, :m] = full.k[i, :m], full.v[i, :m]
+            blocks = -(-m // BLOCK)
+            cache.k_scale[i, :, :blocks], cache.v_scale[i, :, :blocks] = full.k_scale[i, :, :blocks], full.v_scale[i, :, :blocks]
+    return cache
+
+
+def _check_attention(out, q, cache, pos, scale=128 ** -0.5):
+    """Against float64.  Allowed: the rounding of the result (2^-8) and, relative to the largest value that a row sees: 2^-12
+    for weights of 12 bits, 2^-11 for their fixed step of 2^-18 of the tile's largest weight over 128 tokens, and twice the
+    error of a score, which is 2^-22 of max |q| sum |k| (query in 8 + 14 bits) and 2^-21 of its own size (float32, exp2)."""
+    b, t, heads, _ = q.shape
+    group = heads // cache.kv_heads
+    for i in range(b):
+        n = pos[i] + t
+        if pos[i] < 0:
+            assert torch.all(out[i] == 0)
+            continue
+        s = lambda x: x[i].double().repeat_interleave(BLOCK, -1)[:, :n, None]        # noqa: E731
+        k = cache.k[i, :n].contiguous().view(torch.float8_e4m3fn).double().transpose(0, 1) * s(cache.k_scale)
+        v = cache.v[i, :n].contiguous().view(torch.float8_e4m3fn).double().transpose(0, 1) * s(cache.v_scale)
+        qq = q[i].double().view(t, cache.kv_heads, group, 128).permute(1, 2, 0, 3)                   # [kv, group, t, 128]
+        score = qq @ k[:, None].transpose(-1, -2) * scale
+        seen = torch.arange(n, device=q.device)[None, :] <= pos[i] + torch.arange(t, device=q.device)[:, None]
+        score = score.masked_fill(~seen, -math.inf)
+        want = (torch.softmax(score, -1) @ v[:, None]).permute(2, 0, 1, 3).reshape(t, heads, 128)
+        off = 2.0 ** -22 * scale * float(qq.abs().max()) * float(k.abs().sum(-1).max()) + 2.0 ** -21 * float(score[seen.expand_as(score)].abs().max())
+        bound = want.abs() * 2.0 ** -8 + (2.0 ** -12 + 2.0 ** -11 + 2 * off) * float(v.abs().max()) * (1 + 2.0 ** -8)
+        err = (out[i].double() - want).abs()
+        assert torch.all(err <= bound), (i, float((err / bound).max()))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (4, 1), (8, 8), (12, 4), (16, 1), (40, 2), (33, 1)])
+@pytest.mark.parametrize("t,pos", [(1, 0), (1, 1), (1, 62), (1, 63), (1, 64), (1, 127), (1, 128), (1, 300), (2, 0), (3, 126), (5, 1000), (40, 0), (33, 95)])
+def test_attention(plq, heads, kv_heads, t, pos):
+    b = 2
+    cache = _filled(plq, b, pos + t + 5, kv_heads, [pos + t] * b, heads * 1000 + t + pos)
+    q = (_rand_q((b, t, heads, 128), t + pos)).cuda()
+    out = plq.ops.fp8_cache_attention(q, cache, pos)
+    _check_attention(out, q, cache, [pos] * b)
+    at = torch.tensor([pos], device="cuda")
+    assert torch.equal(plq.ops.fp8_cache_attention(q, cache, at, ctx=pos + t), out)          # the same split, the same bits
+    _check_attention(plq.ops.fp8_cache_attention(q, cache, at), q, cache, [pos] * b)
+    plq.check_device_status()
+
+
+def _rand_q(shape, seed, gain=1.5):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * gain).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("t", [1, 4, 70])
+@pytest.mark.parametrize("lengths", [[1, 500, 64], [0, 129, 2000], [0, 0, 0], [65, 64, 63], [5000, 1, 0]])
+def test_attention_of_ragged_batches(plq, t, lengths):
+    """Sequences of different lengths, one that sits out."""
+    pos = [n if n > 0 else -1 for n in lengths]
+    room = max(lengths) + t + 60
+    cache = _filled(plq, 3, room, 2, [p + t if p >= 0 else 0 for p in pos], 7)
+    q = _rand_q((3, t, 8, 128), 8).cuda()
+    out = plq.ops.fp8_cache_attention(q, cache, torch.tensor(pos, device="cuda"))
+    _check_attention(out, q, cache, pos)
+    plq.check_device_status()
+
+
+@pytest.mark.parametrize("b,t,heads,kv_heads,pos", [(1, 1, 64, 8, 40000), (1, 2, 8, 1, 70001), (16, 1, 32, 8, 4095), (2, 600, 8, 2, 0), (1, 300, 16, 2, 3000)])
+def test_attention_of_ordinary_sizes(plq, b, t, heads, kv_heads, pos):
+    cache = _filled(plq, b, pos + t, kv_heads, [pos + t] * b, 9)
+    q = _rand_q((b, t, heads, 128), 10).cuda()
+    out = plq.ops.fp8_cache_attention(q, cache, pos)
+    _check_attention(out, q, cache, [pos] * b)
+    assert torch.equal(out, plq.ops.fp8_cache_attention(q, cache, pos))
+    plq.check_device_status()
+
+
+@pytest.mark.parametrize("gain,q_gain,scale", [(1.0, 30.0, None), (1e-3, 1.0, None), (1e4, 1e-4, None), (1.0, 1.0, 0.0), (1.0, 0.0, None), (1.0, 1.0, -0.3), (1e-30, 1e30, None)])
+def test_attention_of_sharp_flat_large_and_small_scores(plq, gain, q_gain, scale):
+    cache = _filled(plq, 1, 900, 2, [900], 11, gain)
+    q = _rand_q((1, 3, 8, 128), 12, q_gain).cuda()
+    out = plq.ops.fp8_cache_attention(q, cache, 897, scale=scale)
+    _check_attention(out, q, cache, [897], 128 ** -0.5 if scale is None else scale)
+
+
+def test_attention_where_one_position_outweighs_the_others(plq):
+    """A first token with a score far above the rest and next to no value, and a block of large values with low scores."""
+    cache = _filled(plq, 1, 1500, 1, [1500], 13)
+    q = _rand_q((1, 1, 4, 128), 14).cuda()
+    first = plq.kv_cache.Fp8Cache.empty(1, 1500, 1, "cuda")
+    row = torch.zeros(1, 1, 3 * 128, dtype=torch.bfloat16, device="cuda")
+    row[..., 128:256] = q.float().mean(2).to(torch.bfloat16) * 3
+    row[..., 256:] = 1e-3
+    one = torch.ones(1, 128, device="cuda")
+    plq.ops.rope_kv_append_fp8(row, one, one * 0, 1, 1, first, 0)
+    for dst, src in ((cache.k, first.k), (cache.v, first.v)):
+        dst[:, 1:64] = 0
+        dst[:, 0] = src[:, 0]
+    cache.k_scale[..., 0], cache.v_scale[..., 0] = first.k_scale[..., 0], first.v_scale[..., 0]
+    cache.v_scale[..., 5] *= 2.0 ** 12
+    _check_attention(plq.ops.fp8_cache_attention(q, cache, 1499), q, cache, [1499])
+
+
+def test_attention_of_equal_values_returns_them(plq):
+    """Weights and their sum belong together: a cache of one value gives that value."""
+    cache = _filled(plq, 1, 777, 1, [777], 15)
+    cache.v.fill_(0x38)                                # 1.0
+    cache.v_scale.fill_(0.25)
+    q = _rand_q((1, 7, 4, 128), 16).cuda()
+    out = plq.ops.fp8_cache_attention(q, cache, 770)
+    assert torch.all((out.float() - 0.25).abs() <= 0.25 * (2.0 ** -8 + 2.0 ** -11))
+
+
+def test_attention_keeps_what_is_not_finite_where_it_is_seen(plq):
+    """A block of NaN reaches the rows that see it and no others; a query of NaN or infinity its own row alone."""
+    b, t, pos = 1, 100, 150
+    for side in ("k_scale", "v_scale"):
+        cache = _filled(plq, b, 256, 2, [250], 17)
+        q = _rand_q((b, t, 8, 128), 18).cuda()
+        want = plq.ops.fp8_cache_attention(q, cache, pos)
+        getattr(cache, side)[0, 1, 3] = float("nan")              # positions 192 .. 255 of the second key head
+        got = plq.ops.fp8_cache_attention(q, cache, pos)
+        hit = torch.zeros(b, t, 8, dtype=torch.bool, device="cuda")
+        hit[:, 192 - pos:, 4:] = True
+        assert torch.all(got[hit].isnan()) and torch.equal(got[~hit], want[~hit])
+    q[0, 7, 3, 5], q[0, 9, 6, 0] = float("nan"), float("inf")
+    cache = _filled(plq, b, 256, 2, [250], 17)
+    got = plq.ops.fp8_cache_attention(q, cache, pos)
+    hit = torch.zeros(b, t, 8, dtype=torch.bool, device="cuda")
+    hit[0, 7, 3] = hit[0, 9, 6] = True
+    assert torch.all(got[hit].isnan()) and not got[~hit].isnan().any()
+    # positions behind the last one may hold NaN codes and scales (every cache here does)
+    plq.check_device_status()
+
+
+def test_attention_reports_positions_outside_the_cache(plq):
+    cache = _filled(plq, 2, 100, 1, [100, 100], 19)
+    q = _rand_q((2, 2, 4, 128), 20).cuda()
+    with pytest.raises(plq.PlqError):
+        plq.ops.fp8_cache_attention(q, cache, 99)
+    out = plq.ops.fp8_cache_attention(q, cache, torch.tensor([99, 98], device="cuda"))
+    assert torch.all(out[0] == 0)
+    _check_attention(out[1:], q[1:], plq.kv_cache.Fp8Cache(cache.k[1:], cache.k_scale[1:], cache.v[1:], cache.v_scale[1:]), [98])
+    with pytest.raises(plq.PlqError):
+        plq.check_device_status()
+
+
+def test_step_in_a_graph_at_moving_positions(plq):
+    """Append and attention captured once, replayed while the position in device memory moves; two graphs of different shapes
+    and an eager stream beside them."""
+    heads, kv_heads, b, room = 8, 2, 3, 700
+    eager, caught = _filled(plq, b, room, kv_heads, [600] * b, 21), None
+    caught = _clone(plq, eager)
+    pos = torch.tensor([500, 70, -1], device="cuda")
+    qkv = _qkv(b, 1, heads, kv_heads, 22)
+    cos, sin = torch.ones(1, 128, device="cuda"), torch.zeros(1, 128, device="cuda")
+
+    def step(cache):
+        q = plq.ops.rope_kv_append_fp8(qkv, cos, sin, heads, kv_heads, cache, pos)
+        return plq.ops.fp8_cache_attention(q, cache, pos)
+    step(_clone(plq, eager))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(side):
+        step(_clone(plq, eager))
+        side.synchronize()
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                y = step(caught)
+            graphs.append((g, y))
+    torch.cuda.synchronize()
+    for i in range(6):
+        qkv.copy_(_qkv(b, 1, heads, kv_heads, 30 + i))
+        g, y = graphs[i % 2]
+        g.replay()
+        want = step(eager)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and _same(eager, caught)
+        pos.add_((pos >= 0).long())
+    plq.check_device_status()
+
+
+def test_long_cache_behind_the_32_bit_border(plq):
+    """More than 2^32 bytes of codes: the last sequence's rows and scales are found."""
+    b, kv_heads, room = 5, 8, (1 << 32) // (4 * 8 * 128) + 64
+    cache = plq.kv_cache.Fp8Cache.empty(b, room, kv_heads, "cuda")
+    for x in (cache.k, cache.v):
+        x.zero_()
+    for x in (cache.k_scale, cache.v_scale):
+        x.fill_(2.0 ** -8)
+    pos = torch.tensor([3, -1, room - 700, -1, room - 300], device="cuda")
+    qkv = _qkv(b, 300, 16, kv_heads, 40)
+    at = pos[:, None].cpu() + torch.arange(300)
+    cos, sin = _angles(at)
+    q = plq.ops.rope_kv_append_fp8(qkv, cos, sin, 16, kv_heads, cache, pos)
+    k, v = _rope(qkv.view(b, 300, -1, 128)[:, :, 16:24], cos[:, :, None], sin[:, :, None]), qkv.view(b, 300, -1, 128)[:, :, 24:]
+    for i in (0, 2, 4):
+        p = int(pos[i])
+        for codes, scale, new in ((cache.k, cache.k_scale, k), (cache.v, cache.v_scale, v)):
+            s = scale[i].repeat_interleave(BLOCK, -1)[:, p:p + 300].t()[..., None]
+            got = codes[i, p:p + 300].view(torch.float8_e4m3fn).float() * s
+            assert torch.all((got - new[i].float()).abs() <= torch.maximum(new[i].float().abs() * 2.0 ** -4, s * 2.0 ** -10))
+    only = plq.kv_cache.Fp8Cache(*(x[4:] for x in (cache.k, cache.k_scale, cache.v, cache.v_scale)))
+    out = plq.ops.fp8_cache_attention(q[:, -1:].contiguous(), cache, pos + 299 * (pos >= 0))
+    _check_attention(out[4:], q[4:, -1:].contiguous(), only, [room - 1])
+    plq.check_device_status()
