@@ -122,6 +122,11 @@ __device__ __forceinline__ bool mbar_wait_bounded_warp(uint64_t* bar, uint32_t p
   return ok != 0;
 }
 
+// Every lane waits by itself (the instruction is one for the warp); the answer is the same for all of them.
+__device__ __forceinline__ bool mbar_wait_bounded_lanes(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar, parity, abort)) != 0;
+}
+
 // Tiled TMA loads for kernels that may run as a CTA pair.  CG = 2 uses the pair form of the
 // instruction, whose completion bytes may be counted on an mbarrier of the other CTA of the
 // pair: `bar_addr` is a shared::cluster address (clear bit 24 of a local address to name the

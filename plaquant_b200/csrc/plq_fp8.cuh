@@ -26,6 +26,18 @@ __device__ __forceinline__ float2 e4m3x2_to_f32x2(uint32_t c) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(c)));
   return __half22float2(*reinterpret_cast<__half2*>(&h));
 }
+// Two float32 in [0, 448] -> their nearest E4M3 codes (low half) and those of what is left (high half), by way of f16, whose
+// rounding (2^-11) is far below that of the second code.
+__device__ __forceinline__ uint32_t e4m3_split(float a, float b) {
+  uint32_t x, back;
+  uint16_t hi, lo;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(hi) : "r"(x));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(hi));
+  const __half2 rest = __hsub2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&back));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(lo) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
+  return hi | static_cast<uint32_t>(lo) << 16;
+}
 __device__ __forceinline__ uint2 e4m3x8(const float (&y)[8]) {
   return make_uint2(e4m3x2(y[0], y[1]) | e4m3x2(y[2], y[3]) << 16, e4m3x2(y[4], y[5]) | e4m3x2(y[6], y[7]) << 16);
 }
@@ -61,6 +73,22 @@ __device__ __forceinline__ void tc_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[1
       : "r"(taddr)
       : "memory");
 }
+
+// four bytes global -> shared, and an arrival on the mbarrier when all earlier ones of this thread have landed
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// An arrival that orders nothing but the tensor-memory reads that a tcgen05 fence in front of it covers: the release of
+// mbar_arrive_cluster costs a memory barrier.
+__device__ __forceinline__ void mbar_arrive_relaxed_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The warps of a warpgroup hand registers back, or take more.
+template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int32_t x, int32_t y, int32_t z, uint32_t bar) {
   tma_load_3d_cg<1>(dst, tmap, x, y, z, bar);

@@ -149,14 +149,16 @@ __global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8Append
 // out[row] = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale * q_row . k_t),  over the positions t <= pos + i of a query i.
 //
 // One pass over the cache with the 8-bit codes fed to the tensor core as they are (tcgen05 kind::f8f6f4): no thread
-// converts or scales a key or a value.  For that the other operand has to be 8-bit too, without losing its precision:
-//   q      as the sum of two E4M3 numbers, hi + lo / 16 (4 + 4 significant bits: exact for bf16 within 2^-22 of the largest
-//          query of the tile; tile-wide power-of-two scale), two column sets of one product
-//   p      as the sum of three E4M3 numbers (12 bits), 256 * p <= 256 within a tile of 128 tokens
-// With S^T = K Q^T the 128 tokens of a tile are the lanes of tensor memory and the query rows its columns (R = 16 or 32 of
-// them: heads of a group x queries), so a thread owns one token, whose key scale is one multiplication; O^T = V^T P^T has
-// the 128 elements of the head as its lanes.  Each 64-token block of V gets an accumulator of its own, to which the block's
-// scale is applied in float32 on the way into the running sums in registers.
+// converts or scales a key or a value.  For that the other operand has to be 8-bit too, without losing its precision, and
+// is the sum of two E4M3 numbers, which are two sets of columns of one product:
+//   q      hi + lo / 16 (4 + 4 significant bits: exact for bf16 within 2^-22 of the largest query of the tile; one
+//          power-of-two scale per tile of queries)
+//   256 p  hi + lo, 256 p <= 256 within a tile of 128 tokens: off by at most 2^-9 of itself (a bf16 would be by 2^-8) or by
+//          half a step of 2^-9, which is 2^-18 of the tile's largest weight
+// With S^T = K Q^T the 128 tokens of a tile are the lanes of tensor memory and the query rows its columns (R = 8, 16 or 32 of
+// them: heads of a group x queries), so a thread owns one token, and the scale of its key is a factor of the whole warp;
+// O^T = V^T P^T has the 128 elements of the head as its lanes.  Each 64-token block of V gets an accumulator of its own, to
+// which the block's scale is applied in float32 on the way into the running sums in registers.
 //   warp 0 producer (TMA: 128 tokens x 128 bytes of keys, of values), warp 1 MMA issuer, warps 2 - 5 softmax and sums
 // The cache's tiles can be split over several CTAs whose partial sums fp8_attention_join_kernel adds in a fixed order.
 struct Fp8AttnArgs {
@@ -174,17 +176,15 @@ struct Fp8AttnArgs {
 
 template <int R>
 struct AtCfg {
-  static constexpr int kPieces = 3;
-  static constexpr int kPBytes = kPieces * R * 128;
-  static constexpr int kQBytes = 2 * R * 128;
-  static constexpr int kKStages = 3, kVStages = R == 16 ? 3 : 2;
+  static constexpr int kN = 2 * R;                     // columns of either product: hi | lo
+  static constexpr int kPBytes = kN * 128;
+  static constexpr int kQBytes = kN * 128;
+  static constexpr int kKStages = 3, kVStages = R == 32 ? 2 : 3;
   static constexpr int kTile = 128 * kHeadDim;         // 16 KiB
-  static constexpr int kSCols = 2 * R;                 // hi | lo
-  static constexpr int kDCol0 = 2 * kSCols;
-  static constexpr int kTmemCols = R == 16 ? 128 : 256;
+  static constexpr int kDCol0 = 2 * kN;                // two S accumulators, then one D per 64-token block
+  static constexpr int kTmemCols = 8 * R;
   static constexpr int kStatFloats = 2 * 4 * R /* warp maxima */ + 4 * 2 * 2 * R /* per warp: factors */ + 4 * R /* per warp: maxima */ + 4 * R;
   static constexpr size_t kSmemBytes = 1024 + kQBytes + kPBytes + static_cast<size_t>(kKStages + kVStages) * kTile + kStatFloats * 4 + R * 4 + 256;
-  static_assert(kDCol0 + 2 * R <= kTmemCols, "tensor memory budget");
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
 
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     }
   } else if (warp == 1) {
     if (elect_one() && n > 0) {
-      constexpr uint32_t idesc_s = make_idesc_e4m3(128, 2 * R), idesc_d = make_idesc_e4m3(128, R, true, true);
+      constexpr uint32_t idesc_s = make_idesc_e4m3(128, C::kN), idesc_d = make_idesc_e4m3(128, C::kN, true, true);
       const uint32_t q_lo = desc_lo_sw128(smem_u32(q_s)), p_lo = desc_lo_p(smem_u32(p_s));
       bool ok = mbar_wait_bounded(q_full, 0, abort_flag);
       for (int j = 0; ok && j <= n; ++j) {
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
           const uint32_t k_lo = desc_lo_sw128(k_base + ks * C::kTile);
 #pragma unroll
           for (int h = 0; h < 4; ++h)
-            tc_mma_e4m3<1>(tmem_base + (j & 1) * C::kSCols, k_lo + 2 * h, kDescHiSw128, q_lo + 2 * h, kDescHiSw128, idesc_s, h != 0);
+            tc_mma_e4m3<1>(tmem_base + (j & 1) * C::kN, k_lo + 2 * h, kDescHiSw128, q_lo + 2 * h, kDescHiSw128, idesc_s, h != 0);
           tc_commit<1>(smem_u32(&s_full[j & 1]));
           tc_commit<1>(smem_u32(&k_empty[ks]));
         }
@@ -312,11 +312,9 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
           tc_fence_after();
           const uint32_t v_lo = desc_lo_sw128(v_base + vs * C::kTile);
 #pragma unroll
-          for (int piece = 0; piece < C::kPieces; ++piece)
-#pragma unroll
-            for (int h = 0; h < 4; ++h)               // 32 tokens each; two 64-token blocks, two accumulators
-              tc_mma_e4m3<1>(tmem_base + C::kDCol0 + (h >> 1) * R, v_lo + h * (4096 >> 4), kDescHiSw128, p_lo + ((piece * R * 128 + h * 512) >> 4),
-                             kDescHiP, idesc_d, !(piece == 0 && (h & 1) == 0));
+          for (int h = 0; h < 4; ++h)                 // 32 tokens each; two 64-token blocks, two accumulators
+            tc_mma_e4m3<1>(tmem_base + C::kDCol0 + (h >> 1) * C::kN, v_lo + h * (4096 >> 4), kDescHiSw128, p_lo + h * (512 >> 4), kDescHiP,
+                           idesc_d, h & 1);
           tc_commit<1>(smem_u32(d_full));
           tc_commit<1>(smem_u32(&v_empty[vs]));
         }
@@ -329,7 +327,9 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     float* my_max = mloc + sw * R;
 
     // ---- the queries: tile-wide power-of-two scale, hi and lo codes ----
-    constexpr int kPer = R / 16;                      // 16-element chunks per thread
+    constexpr int kPer = R > 16 ? R / 16 : 1;         // 16-element chunks per thread
+    const bool has_q = R >= 16 || tid < 8 * R;
+    const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu;      // a negative or no scale
     const __nv_bfloat16* q_base = a.q + ((b * a.t) * a.heads + static_cast<long long>(kh) * a.group) * kHeadDim;
     uint4 qv[kPer][2];
     uint32_t top = 0;
@@ -343,9 +343,10 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
         qv[c][0] = src[0];
         qv[c][1] = src[1];
       }
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(qv[c]);
+      uint32_t* w = reinterpret_cast<uint32_t*>(qv[c]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
+        w[e] = (w[e] & keep) ^ flip;
         const uint32_t lo = (w[e] << 16) & 0x7FFF0000u, hi = w[e] & 0x7FFF0000u;
         if (lo < 0x7F800000u) top = max(top, lo);
         if (hi < 0x7F800000u) top = max(top, hi);
@@ -386,8 +387,10 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
         lo[d] = l2[0] | l2[1] << 16;
       }
       auto at = [&](int rr) { return reinterpret_cast<uint4*>(q_s + (rr >> 3) * 1024 + (rr & 7) * 128 + ((chunk ^ (rr & 7)) << 4)); };
-      *at(r) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *at(R + r) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      if (has_q) {
+        *at(r) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *at(R + r) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -404,30 +407,41 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
 
     // adds the product of the tile before: o = o * alpha + (D0 * vs0 + D1 * vs1) * beta / 256
     auto promote = [&](int j, float vs0, float vs1) {
-      const bool odd = vs1 != vs1;                    // a second block of NaN: not for the rows that end in the first
-      const int second = (tile0 + j) * 128 + kCacheBlock;
-      ok = mbar_wait_bounded_warp(d_full, j & 1u, abort_flag);
+      ok = mbar_wait_bounded_lanes(d_full, j & 1u, abort_flag);
       if (!ok) return;
       tc_fence_after();
       const float* f = my_fac + (j & 1) * 2 * R;
-#pragma unroll
-      for (int c = 0; c < R / 16; ++c) {
+      const bool finite = fabsf(vs0) < 3e38f && fabsf(vs1) < 3e38f;
+      auto add = [&](int r, float d0, float d1, float al, float be) {
+        if (!finite) {                                // a block of NaN: not for the rows that end before it
+          d0 = lim_s[r] >= (tile0 + j) * 128 ? d0 * vs0 : 0.0f;
+          d1 = lim_s[r] >= (tile0 + j) * 128 + kCacheBlock ? d1 * vs1 : 0.0f;
+          o[r] = fmaf(o[r], al, (d0 + d1) * be);
+        } else {
+          o[r] = fmaf(o[r], al, fmaf(d0, vs0, d1 * vs1) * be);
+        }
+      };
+      if constexpr (R == 8) {
         uint32_t d0[16], d1[16];
-        tc_ld_32x32b_x16(tmem_base + lane_base + C::kDCol0 + c * 16, d0);
-        tc_ld_32x32b_x16(tmem_base + lane_base + C::kDCol0 + R + c * 16, d1);
+        tc_ld_32x32b_x16(tmem_base + lane_base + C::kDCol0, d0);
+        tc_ld_32x32b_x16(tmem_base + lane_base + C::kDCol0 + C::kN, d1);
         tc_wait_ld();
 #pragma unroll
-        for (int x = 0; x < 16; x += 4) {
-          const float4 al = *reinterpret_cast<const float4*>(f + c * 16 + x), be = *reinterpret_cast<const float4*>(f + R + c * 16 + x);
-          const float av[4] = {al.x, al.y, al.z, al.w}, bv[4] = {be.x, be.y, be.z, be.w};
+        for (int r = 0; r < 8; ++r)
+          add(r, __uint_as_float(d0[r]) + __uint_as_float(d0[8 + r]), __uint_as_float(d1[r]) + __uint_as_float(d1[8 + r]), f[r], f[R + r]);
+      } else {
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            float e1 = __uint_as_float(d1[x + y]) * vs1;
-            if (odd && lim_s[c * 16 + x + y] < second) e1 = 0.0f;
-            const float d = fmaf(__uint_as_float(d0[x + y]), vs0, e1);
-            // a row that sees nothing of the tile keeps its sum, whatever the block's scale is
-            o[c * 16 + x + y] = fmaf(o[c * 16 + x + y], av[y], bv[y] == 0.0f ? 0.0f : d * bv[y]);
-          }
+        for (int c = 0; c < R / 8; ++c) {
+          uint32_t h0[8], l0[8], h1[8], l1[8];
+          const uint32_t at = tmem_base + lane_base + C::kDCol0 + c * 8;
+          tc_ld_32x32b_x8(at, h0);
+          tc_ld_32x32b_x8(at + R, l0);
+          tc_ld_32x32b_x8(at + C::kN, h1);
+          tc_ld_32x32b_x8(at + C::kN + R, l1);
+          tc_wait_ld();
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            add(c * 8 + x, __uint_as_float(h0[x]) + __uint_as_float(l0[x]), __uint_as_float(h1[x]) + __uint_as_float(l1[x]), f[c * 8 + x], f[R + c * 8 + x]);
         }
       }
       tc_fence_before();
@@ -436,8 +450,9 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     const float* k_scale = a.k_scale + head_scales;
     const float* v_scale = a.v_scale + head_scales;
     const int last_block = static_cast<int>((written - 1) / kCacheBlock);       // the last one that holds a position
-    auto scale_of = [&](const float* side, int block) { return block <= last_block ? side[block] : 0.0f; };
-    float next_k = 0.0f, next_v0 = 0.0f, next_v1 = 0.0f;
+    auto scale_of = [&](const float* side, int block) { return block <= last_block ? side[block] : 1.0f; };
+    float next_k = 1.0f, next_v0 = 1.0f, next_v1 = 1.0f;
+    const float per_k = down * (a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2));
     if (n > 0) {
       next_k = scale_of(k_scale, tile0 * 2 + (quad >> 1));
       next_v0 = scale_of(v_scale, tile0 * 2);
@@ -445,28 +460,39 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     }
     for (int j = 0; j < n; ++j) {                     // `ok` is looked at by all warps together, at the barrier
       const int tile = tile0 + j;
-      const float ksc = next_k * (down * a.scale_log2), nv0 = next_v0 * (1.0f / 256.0f), nv1 = next_v1 * (1.0f / 256.0f);
+      const float nv0 = next_v0, nv1 = next_v1;
+      float ksc = next_k * per_k;                     // of the warp's tokens
+      if (ksc < 1.2e-38f) ksc = 1.2e-38f;             // a score of zero, and minus infinity stays what it is
       if (j + 1 < n) {                                // a tile ahead: they come from L2
         next_k = scale_of(k_scale, tile * 2 + 2 + (quad >> 1));
         next_v0 = scale_of(v_scale, tile * 2 + 2);
         next_v1 = scale_of(v_scale, tile * 2 + 3);
       }
-      if (ok) ok = mbar_wait_bounded_warp(&s_full[j & 1], (j >> 1) & 1u, abort_flag);
+      if (ok) ok = mbar_wait_bounded_lanes(&s_full[j & 1], (j >> 1) & 1u, abort_flag);
       tc_fence_after();
-      float s[R];
+      float s[R];                                      // scores without the scale of the keys
       {
-        uint32_t hi[R / 16][16], lo[R / 16][16];
+        const uint32_t at = tmem_base + lane_base + (j & 1) * C::kN;
+        if constexpr (R == 8) {
+          uint32_t x[16];
+          tc_ld_32x32b_x16(at, x);
+          tc_wait_ld();
 #pragma unroll
-        for (int c = 0; c < R / 16; ++c) {
-          tc_ld_32x32b_x16(tmem_base + lane_base + (j & 1) * C::kSCols + c * 16, hi[c]);
-          tc_ld_32x32b_x16(tmem_base + lane_base + (j & 1) * C::kSCols + R + c * 16, lo[c]);
+          for (int r = 0; r < 8; ++r) s[r] = fmaf(__uint_as_float(x[8 + r]), 0.0625f, __uint_as_float(x[r]));
+        } else {
+#pragma unroll
+          for (int c = 0; c < R / 16; ++c) {
+            uint32_t x[16], y[16];
+            tc_ld_32x32b_x16(at + c * 16, x);
+            tc_ld_32x32b_x16(at + R + c * 16, y);
+            tc_wait_ld();
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[c * 16 + r] = fmaf(__uint_as_float(y[r]), 0.0625f, __uint_as_float(x[r]));
+          }
         }
-        tc_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_empty[j & 1]);
-#pragma unroll
-        for (int r = 0; r < R; ++r) s[r] = fmaf(__uint_as_float(lo[r / 16][r & 15]), 0.0625f, __uint_as_float(hi[r / 16][r & 15])) * ksc;
       }
       const int token = tile * 128 + tok;
       const bool masked = tile * 128 + 127 > lim_min;            // the same for the whole CTA
@@ -482,39 +508,37 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
         if (lane == r) mine = m;
       }
       float* wm = wmax + (j & 1) * 4 * R;
-      if (lane < R) wm[sw * R + lane] = mine;
+      if (lane < R) wm[sw * R + lane] = mine * ksc;
       ok = softmax_barrier(ok);
       if (!ok) break;
       if (lane < R) {
         const float m = fmaxf(fmaxf(wm[lane], wm[R + lane]), fmaxf(wm[2 * R + lane], wm[3 * R + lane]));
         const float m_new = fmaxf(m_run, m);
-        my_fac[(j & 1) * 2 * R + lane] = m_run == kNegInf ? 0.0f : ex2_approx(m_run - m_new);
-        my_fac[(j & 1) * 2 * R + R + lane] = m == kNegInf ? 0.0f : ex2_approx(m - m_new);
-        my_max[lane] = m == kNegInf ? 0.0f : m;
+        my_fac[(j & 1) * 2 * R + lane] = m_run > kNegInf ? ex2_approx(m_run - m_new) : 0.0f;
+        my_fac[(j & 1) * 2 * R + R + lane] = m > kNegInf ? ex2_approx(m - m_new - 8.0f) : 0.0f;
+        my_max[lane] = m > kNegInf ? 8.0f - m : 0.0f;
         m_run = m_new;
       }
       __syncwarp();
       const float* f = my_fac + (j & 1) * 2 * R;
-      uint32_t piece[C::kPieces][R / 4];
+      uint32_t hi[R / 4], lo[R / 4];
 #pragma unroll
       for (int r = 0; r < R; r += 4) {
         const float4 mx = *reinterpret_cast<const float4*>(my_max + r), al = *reinterpret_cast<const float4*>(f + r), be = *reinterpret_cast<const float4*>(f + R + r);
-        float p[4] = {ex2_approx(s[r] - mx.x), ex2_approx(s[r + 1] - mx.y), ex2_approx(s[r + 2] - mx.z), ex2_approx(s[r + 3] - mx.w)};
+        float p[4] = {ex2_approx(fmaf(s[r], ksc, mx.x)), ex2_approx(fmaf(s[r + 1], ksc, mx.y)), ex2_approx(fmaf(s[r + 2], ksc, mx.z)),
+                      ex2_approx(fmaf(s[r + 3], ksc, mx.w))};      // 256 p
+        if (masked) {                                  // whatever the scale of their block is
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (token > lim_s[r + x]) p[x] = 0.0f;
+        }
         l[r] = fmaf(l[r], al.x, p[0] * be.x);
         l[r + 1] = fmaf(l[r + 1], al.y, p[1] * be.y);
         l[r + 2] = fmaf(l[r + 2], al.z, p[2] * be.z);
         l[r + 3] = fmaf(l[r + 3], al.w, p[3] * be.w);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) p[x] *= 256.0f;
-#pragma unroll
-        for (int pc = 0; pc < C::kPieces; ++pc) {
-          const uint32_t c0 = e4m3x2(p[0], p[1]), c1 = e4m3x2(p[2], p[3]);
-          piece[pc][r / 4] = c0 | c1 << 16;
-          if (pc + 1 < C::kPieces) {
-            const float2 b0 = e4m3x2_to_f32x2(c0), b1 = e4m3x2_to_f32x2(c1);
-            p[0] -= b0.x; p[1] -= b0.y; p[2] -= b1.x; p[3] -= b1.y;
-          }
-        }
+        const uint32_t c0 = e4m3_split(p[0], p[1]), c1 = e4m3_split(p[2], p[3]);
+        hi[r / 4] = __byte_perm(c0, c1, 0x5410);
+        lo[r / 4] = __byte_perm(c0, c1, 0x7632);
       }
       if (j > 0) {                                     // the product of tile j - 1 is done: its P may be overwritten
         promote(j - 1, vs0, vs1);
@@ -522,15 +546,18 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
       }
       vs0 = nv0;
       vs1 = nv1;
+      if constexpr (R == 8) {
+        *reinterpret_cast<uint4*>(p_s + tok * 16) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+      } else {
 #pragma unroll
-      for (int pc = 0; pc < C::kPieces; ++pc)
-#pragma unroll
-        for (int c = 0; c < R / 16; ++c)
-          *reinterpret_cast<uint4*>(p_s + pc * R * 128 + c * 2048 + tok * 16) =
-              make_uint4(piece[pc][4 * c], piece[pc][4 * c + 1], piece[pc][4 * c + 2], piece[pc][4 * c + 3]);
+        for (int c = 0; c < R / 16; ++c) {
+          *reinterpret_cast<uint4*>(p_s + c * 2048 + tok * 16) = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
+          *reinterpret_cast<uint4*>(p_s + (R / 16 + c) * 2048 + tok * 16) = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+        }
+      }
       if (static_cast<long long>(tile) * 128 + 128 > written) {  // rows that nobody has written: 0 x NaN would be NaN
         const int vs = j % C::kVStages;
-        ok = mbar_wait_bounded_warp(&v_full[vs], (j / C::kVStages) & 1u, abort_flag);
+        ok = mbar_wait_bounded_lanes(&v_full[vs], (j / C::kVStages) & 1u, abort_flag);
         if (!ok) continue;
         if (static_cast<long long>(tile) * 128 + tok >= written) {
           uint4* row = reinterpret_cast<uint4*>(v_s + vs * C::kTile + tok * 128);
@@ -657,7 +684,7 @@ struct AttnPlan { int rows, row_tiles, splits; };
 static AttnPlan attn_plan(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t ctx) {
   AttnPlan p;
   const int64_t rows = t * (heads / kv_heads);
-  p.rows = rows <= 16 ? 16 : 32;
+  p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
   p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
   // Two CTAs fit an SM.  As many splits as fill the device once, none shorter than four tiles of 128 tokens: a CTA's
   // set-up and its share of the join cost about what two tiles do.
@@ -779,5 +806,6 @@ extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const 
   memset(&mv, 0, sizeof(mv));
   if ((st = make_cache_tmap(&mk, k_codes, batch, t_max, kv_heads)) != PLQ_OK) return st;
   if ((st = make_cache_tmap(&mv, v_codes, batch, t_max, kv_heads)) != PLQ_OK) return st;
+  if (p.rows == 8) return launch_attention<8>(mk, mv, a, stream);
   return p.rows == 16 ? launch_attention<16>(mk, mv, a, stream) : launch_attention<32>(mk, mv, a, stream);
 }

@@ -250,19 +250,26 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------
-// Persistent; warp 0 producer, warp 1 MMA issuer (leader CTA of a pair), then four epilogue warps per 128 columns, each
-// thread one row x 128 columns of float32 sums.  Per K block an epilogue warp reads 128 columns from tensor memory and
-// does 64 packed multiply-adds (128 cycles of the FMA pipe) beside the 256 (128 x 128) or 512 cycles of the block's MMAs.
+// Persistent; warp 0 producer, warp 1 MMA issuer (leader CTA of a pair), warp 2 fetches scales, warps 4 - 11 epilogue: four
+// warps (the quadrants of tensor memory) for either half of the tile's columns, each thread one row x 64 or 128 float32 sums.
+// Per K block an epilogue warp reads its columns from tensor memory and does one packed multiply-add per two of them,
+// beside the 256 (128 x 128) or 512 cycles of the block's MMAs.  The scales travel ahead of the epilogue through a ring of
+// their own (cp.async, 16 K blocks deep): loaded by the epilogue itself their latency was longer than a K block.
 template <int BN, int CG>
 struct GmCfg {
   static constexpr int kBRows = BN / CG;
   static constexpr int kStageBytes = kABytes + kBRows * kStageKBytes;      // 32 KiB
   static constexpr int kStages = 6;
   static constexpr int kAcc = 512 / BN;
-  static constexpr int kEpiWarps = BN / 32;
-  static constexpr int kThreads = 64 + 32 * kEpiWarps;
-  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + 512;
+  static constexpr int kCols = BN / 2;                                      // per epilogue warp
+  static constexpr int kSfSlots = 16;
+  static constexpr int kSfBytes = 512 + 16;                                 // 128 row scales, the scales of the tile's weight blocks
+  static constexpr int kThreads = 384;
+  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kSfSlots * kSfBytes + 512;
   static_assert(kStageBytes == 32768 && kSmemBytes <= 232448, "shared memory budget");
+  // Registers: 168 a thread at launch (384 x 168); the epilogue of 128 columns needs more, the other warpgroup less.
+  static constexpr int kRegsMain = 72, kRegsEpi = 216;
+  static_assert(128 * kRegsMain + 256 * kRegsEpi <= 384 * 168, "register split");
 };
 
 // Tile order: bands of `band` row tiles, M fastest inside a band, so that the CTAs running together share operands in L2.
@@ -277,11 +284,14 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
   using C = GmCfg<BN, CG>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes);
+  uint8_t* sf_ring = smem + static_cast<size_t>(C::kStages) * C::kStageBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sf_ring + C::kSfSlots * C::kSfBytes);
   uint64_t* empty_bar = full_bar + C::kStages;
   uint64_t* acc_full = empty_bar + C::kStages;
   uint64_t* acc_empty = acc_full + C::kAcc;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_empty + C::kAcc);
+  uint64_t* sf_full = acc_empty + C::kAcc;
+  uint64_t* sf_empty = sf_full + C::kSfSlots;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sf_empty + C::kSfSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
@@ -289,7 +299,8 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
   const bool leader = rank == 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int s = 0; s < C::kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], C::kEpiWarps * CG); }
+    for (int s = 0; s < C::kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8 * CG); }
+    for (int s = 0; s < C::kSfSlots; ++s) { mbar_init(&sf_full[s], 32); mbar_init(&sf_empty[s], 8); }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -313,6 +324,8 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
   const int step = CG == 2 ? static_cast<int>(nclusters_x()) : static_cast<int>(gridDim.x);
   const uint32_t smem_base = smem_u32(smem);
 
+  if constexpr (BN == 256)
+    if (warp < 4) registers_down<C::kRegsMain>();
   if (warp == 0) {
     if (elect_one()) {
       pdl_wait();
@@ -363,8 +376,33 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
           commit_all(&acc_full[as]);
         }
     }
-  } else {
-    const int quad = warp & 3, cgp = (warp - 2) >> 2;
+  } else if (warp == 2) {
+    pdl_wait();
+    uint32_t gs = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < num_tiles; tile += step) {
+      int tm, tn;
+      fp8_tile(tile, g, tm, tn);
+      // rows and columns behind the end: their operands are zeros, any scale will do that can be read
+      const float* src[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        src[i] = g.sa + static_cast<long long>(min((tm * CG + static_cast<int>(rank)) * kBM + lane + 32 * i, g.m - 1)) * g.kb;
+      const float* sw = g.sw + static_cast<long long>(min(tn * BN + (lane & 1) * 128, g.n - 1) / kFp8Block) * g.kb;
+      for (int kb = 0; kb < g.kb; ++kb, ++gs) {
+        const uint32_t slot = gs % C::kSfSlots;
+        ok = mbar_wait_bounded_lanes(&sf_empty[slot], ((gs / C::kSfSlots) & 1u) ^ 1u, abort_flag);
+        if (!ok) break;
+        const uint32_t dst = smem_u32(sf_ring) + slot * C::kSfBytes;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cp_async4(dst + (lane + 32 * i) * 4, src[i] + kb);
+        if (lane < BN / 128) cp_async4(dst + 512 + lane * 4, sw + kb);
+        cp_async_arrive(&sf_full[slot]);
+      }
+    }
+  } else if (warp >= 4) {
+    if constexpr (BN == 256) registers_up<C::kRegsEpi>();
+    const int quad = warp & 3, cgp = (warp - 4) >> 2;
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t empty_addr = CG == 2 ? map_to_cta(smem_u32(acc_empty), 0u) : smem_u32(acc_empty);
     pdl_wait();
@@ -374,44 +412,47 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
       int tm, tn;
       fp8_tile(tile, g, tm, tn);
       const int row = (tm * CG + static_cast<int>(rank)) * kBM + quad * 32 + lane;
-      const int col0 = tn * BN + cgp * 128;
-      // rows and columns behind the end: their operands are zeros, their scales not read
-      const float* sa = g.sa + static_cast<long long>(min(row, g.m - 1)) * g.kb;
-      const float* sw = g.sw + static_cast<long long>(min(col0, g.n - 1) / kFp8Block) * g.kb;
-      float2 acc[64];
+      const int col0 = tn * BN + cgp * C::kCols;
+      float2 acc[C::kCols / 2];
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
-      float na = sa[0], nw = sw[0];
+      for (int j = 0; j < C::kCols / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
       for (int kb = 0; kb < g.kb; ++kb, ++gs) {
-        const uint32_t as = gs % C::kAcc;
-        const float f = na * nw;
-        if (kb + 1 < g.kb) { na = sa[kb + 1]; nw = sw[kb + 1]; }
-        ok = mbar_wait_bounded_warp(&acc_full[as], (gs / C::kAcc) & 1u, abort_flag);
+        const uint32_t as = gs % C::kAcc, slot = gs % C::kSfSlots;
+        ok = mbar_wait_bounded_lanes(&sf_full[slot], (gs / C::kSfSlots) & 1u, abort_flag);
+        if (!ok) break;
+        const float* sf = reinterpret_cast<const float*>(sf_ring + slot * C::kSfBytes);
+        const float f = sf[quad * 32 + lane] * sf[128 + (BN == 256 ? cgp : 0)];
+        const float2 f2 = make_float2(f, f);
+        ok = mbar_wait_bounded_lanes(&acc_full[as], (gs / C::kAcc) & 1u, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t taddr = tmem_base + lane_base + as * BN + cgp * 128;
-        const float2 f2 = make_float2(f, f);
-        uint32_t r[2][16];
-        tc_ld_32x32b_x16(taddr, r[0]);
+        const uint32_t taddr = tmem_base + lane_base + as * BN + cgp * C::kCols;
+        uint32_t r[2][32];
+        tc_ld_32x32b_x32(taddr, r[0]);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < C::kCols / 32; ++c) {
           tc_wait_ld();
-          if (c < 7) tc_ld_32x32b_x16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
-          else {
+          if (c + 1 < C::kCols / 32) {
+            tc_ld_32x32b_x32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
+          } else {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(empty_addr + 8u * as);
+            if (lane == 0) {
+              mbar_arrive(&sf_empty[slot]);
+              if constexpr (CG == 2) mbar_arrive_relaxed_cluster(empty_addr + 8u * as);
+              else mbar_arrive(&acc_empty[as]);
+            }
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            acc[c * 8 + j] = __ffma2_rn(make_float2(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1])), f2, acc[c * 8 + j]);
+          for (int j = 0; j < 16; ++j)
+            acc[c * 16 + j] = __ffma2_rn(make_float2(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1])), f2, acc[c * 16 + j]);
         }
       }
       if (!ok) break;
       if (row < g.m) {
         OUT* y = static_cast<OUT*>(g.y) + row * g.ldy;
 #pragma unroll
-        for (int v = 0; v < 8; ++v) {                       // 16 columns at a time
+        for (int v = 0; v < C::kCols / 16; ++v) {            // 16 columns at a time
           const int col = col0 + v * 16;
           const float2* s = acc + v * 8;
           if (g.vec && col + 16 <= g.n) {

@@ -1,5 +1,5 @@
 // PyTorch front end of the calls that a forward pass makes most often: the pack, a whole quantised linear, a whole decoder
-// layer.
+// layer, the E4M3 operators.
 // The kernels are those of libplq_b200.so, launched one after the other on the current stream; this file only allocates
 // and forwards.  Called operator by operator from Python a linear is two foreign calls and nine allocations (~40 us of
 // host time against 8 - 15 us on the device for up to a few hundred rows), a layer nine foreign calls and ~30.
@@ -9,6 +9,7 @@
 
 #include <dlfcn.h>
 
+#include <array>
 #include <optional>
 #include <tuple>
 
@@ -30,6 +31,11 @@ struct Api {
   decltype(&::plq_rope_kv_append) rope_kv_append;
   decltype(&::plq_rope_kv_append_nvfp4_values) rope_kv_append_nvfp4_values;
   decltype(&::plq_sf_tiled_bytes) sf_tiled_bytes;
+  decltype(&::plq_fp8_pack) fp8_pack;
+  decltype(&::plq_fp8_gemm) fp8_gemm;
+  decltype(&::plq_rope_kv_append_fp8) rope_kv_append_fp8;
+  decltype(&::plq_fp8_attention_workspace_bytes) fp8_attention_workspace_bytes;
+  decltype(&::plq_fp8_attention) fp8_attention;
 } api;
 
 void init(const std::string& path) {
@@ -50,6 +56,11 @@ void init(const std::string& path) {
   find(api.rope_kv_append, "plq_rope_kv_append");
   find(api.rope_kv_append_nvfp4_values, "plq_rope_kv_append_nvfp4_values");
   find(api.sf_tiled_bytes, "plq_sf_tiled_bytes");
+  find(api.fp8_pack, "plq_fp8_pack");
+  find(api.fp8_gemm, "plq_fp8_gemm");
+  find(api.rope_kv_append_fp8, "plq_rope_kv_append_fp8");
+  find(api.fp8_attention_workspace_bytes, "plq_fp8_attention_workspace_bytes");
+  find(api.fp8_attention, "plq_fp8_attention");
 }
 
 // Raises the package's PlqError for a non-zero status.
@@ -268,6 +279,103 @@ bool alone(const Tensor& a, const Tensor& b) {
   return one(a) && one(b);
 }
 
+// ---- the E4M3 operators ----------------------------------------------------------------------------------------------
+// From Python each was 10 - 15 us of checks, allocations and a foreign call with up to twenty arguments, as long as the
+// kernels of a decode step take.  Each of these handles what needs no further look - contiguous, aligned tensors of the right
+// types on one device - and returns nullopt for anything else: the Python path then copies or raises.
+bool plain(const Tensor& t, at::ScalarType type, c10::Device device) {
+  return t.scalar_type() == type && t.device() == device && t.is_contiguous() && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+}
+
+// [h = residual + x] -> [RMSNorm] -> E4M3: (h or nothing, codes, scales)
+std::optional<std::tuple<std::optional<Tensor>, Tensor, Tensor>> fp8_pack(const Tensor& x, const std::optional<Tensor>& residual,
+                                                                          const std::optional<Tensor>& gamma, double eps) {
+  if (!x.is_cuda() || x.dim() < 1 || x.numel() == 0 || !plain(x, at::kBFloat16, x.device())) return std::nullopt;
+  const int64_t k = x.size(-1), rows = x.numel() / k;
+  if (residual && (residual->sizes() != x.sizes() || !plain(*residual, at::kBFloat16, x.device()))) return std::nullopt;
+  if (gamma && (gamma->numel() != k || !plain(*gamma, at::kBFloat16, x.device()))) return std::nullopt;
+  if (residual && !gamma) return std::nullopt;
+  pybind11::gil_scoped_release nogil;
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor codes = at::empty({rows, k}, x.options().dtype(at::kByte)), scales = at::empty({rows, (k + 127) / 128}, x.options().dtype(at::kFloat));
+  std::optional<Tensor> h;
+  if (residual) h = at::empty_like(x);
+  check(api.fp8_pack(x.const_data_ptr(), k, residual ? residual->const_data_ptr() : nullptr, k, h ? h->data_ptr() : nullptr,
+                     gamma ? gamma->const_data_ptr() : nullptr, static_cast<float>(eps), rows, k, codes.data_ptr(), scales.data_ptr(),
+                     c10::cuda::getCurrentCUDAStream().stream()));
+  return std::make_tuple(h, codes, scales);
+}
+
+std::optional<Tensor> fp8_gemm(const Tensor& a, const Tensor& sa, int64_t a_rows, const Tensor& w, const Tensor& sw, int64_t w_rows,
+                               const Tensor& status, bool f32, int64_t flags) {
+  const auto dev = a.device();
+  if (!a.is_cuda() || a.dim() != 2 || w.dim() != 2 || a_rows != 1 || w_rows != 128 || a.numel() == 0 || w.numel() == 0 ||
+      !plain(a, at::kByte, dev) || !plain(w, at::kByte, dev) || !plain(sa, at::kFloat, dev) || !plain(sw, at::kFloat, dev))
+    return std::nullopt;
+  const int64_t m = a.size(0), n = w.size(0), k = a.size(1), kb = (k + 127) / 128;
+  if (w.size(1) != k || sa.dim() != 2 || sa.size(0) != m || sa.size(1) != kb || sw.dim() != 2 || sw.size(0) != (n + 127) / 128 || sw.size(1) != kb)
+    return std::nullopt;
+  pybind11::gil_scoped_release nogil;
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor y = at::empty({m, n}, a.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  check(api.fp8_gemm(a.const_data_ptr(), sa.const_data_ptr(), w.const_data_ptr(), sw.const_data_ptr(), m, n, k, y.data_ptr(), n, f32,
+                     status.data_ptr<int32_t>(), static_cast<int>(flags), c10::cuda::getCurrentCUDAStream().stream()));
+  return y;
+}
+
+// A cache's sides are what kv_cache.Fp8Cache.check asks for.
+bool plain_cache(const Tensor& k, const Tensor& ks, const Tensor& v, const Tensor& vs, int64_t b, int64_t kv_heads, c10::Device dev) {
+  if (k.dim() != 4 || k.size(0) != b || k.size(1) < 1 || k.size(2) != kv_heads || k.size(3) != 128 || v.sizes() != k.sizes()) return false;
+  const std::array<int64_t, 3> scales = {b, kv_heads, (k.size(1) + 63) / 64};
+  return ks.sizes() == c10::IntArrayRef(scales) && vs.sizes() == c10::IntArrayRef(scales) && plain(k, at::kByte, dev) && plain(v, at::kByte, dev) &&
+         plain(ks, at::kFloat, dev) && plain(vs, at::kFloat, dev);
+}
+bool plain_positions(const std::optional<Tensor>& at, int64_t b, c10::Device dev) {
+  return !at || (at->scalar_type() == at::kLong && (at->numel() == 1 || at->numel() == b) && at->device() == dev && at->is_contiguous());
+}
+
+std::optional<Tensor> rope_kv_append_fp8(const Tensor& qkv, const Tensor& cos, const Tensor& sin, int64_t heads, int64_t kv_heads, const Tensor& k,
+                                         const Tensor& ks, const Tensor& v, const Tensor& vs, const std::optional<Tensor>& pos_dev, int64_t pos,
+                                         const Tensor& status) {
+  const auto dev = qkv.device();
+  if (!qkv.is_cuda() || qkv.dim() != 3 || heads < 1 || kv_heads < 1 || qkv.numel() == 0 || qkv.size(2) != (heads + 2 * kv_heads) * 128 ||
+      !plain(qkv, at::kBFloat16, dev) || !plain(cos, at::kFloat, dev) || !plain(sin, at::kFloat, dev))
+    return std::nullopt;
+  const int64_t b = qkv.size(0), t = qkv.size(1), n = cos.numel();
+  if (sin.numel() != n || (n != t * 128 && n != b * t * 128) || !plain_cache(k, ks, v, vs, b, kv_heads, dev) || !plain_positions(pos_dev, b, dev))
+    return std::nullopt;
+  pybind11::gil_scoped_release nogil;
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor q = at::empty({b, t, heads, 128}, qkv.options());
+  check(api.rope_kv_append_fp8(qkv.const_data_ptr(), qkv.size(2), cos.const_data_ptr(), sin.const_data_ptr(), n == t * 128 ? 0 : t * 128, b, t, heads,
+                               kv_heads, q.data_ptr(), k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), k.size(1),
+                               pos_dev ? pos_dev->const_data_ptr<int64_t>() : nullptr, pos_dev && b > 1 && pos_dev->numel() == b, pos,
+                               status.data_ptr<int32_t>(), c10::cuda::getCurrentCUDAStream().stream()));
+  return q;
+}
+
+std::optional<Tensor> fp8_attention(const Tensor& q, const Tensor& k, const Tensor& ks, const Tensor& v, const Tensor& vs,
+                                    const std::optional<Tensor>& pos_dev, int64_t pos, int64_t ctx, double scale, const Tensor& status) {
+  const auto dev = q.device();
+  if (!q.is_cuda() || q.dim() != 4 || q.numel() == 0 || q.size(3) != 128 || !plain(q, at::kBFloat16, dev) || k.dim() != 4 ||
+      !plain_cache(k, ks, v, vs, q.size(0), k.size(2), dev) || !plain_positions(pos_dev, q.size(0), dev))
+    return std::nullopt;
+  const int64_t b = q.size(0), t = q.size(1), heads = q.size(2), kv_heads = k.size(2), room = k.size(1);
+  if (kv_heads < 1 || heads % kv_heads != 0) return std::nullopt;
+  pybind11::gil_scoped_release nogil;
+  const c10::cuda::CUDAGuard guard(dev);
+  if (!pos_dev && pos >= 0) ctx = std::min(pos + t, room);
+  else if (ctx <= 0) ctx = room;
+  Tensor out = at::empty_like(q), ws;
+  const int64_t need = api.fp8_attention_workspace_bytes(b, t, heads, kv_heads, ctx);
+  if (need) ws = at::empty({need}, q.options().dtype(at::kByte));
+  check(api.fp8_attention(q.const_data_ptr(), k.const_data_ptr(), ks.const_data_ptr(), v.const_data_ptr(), vs.const_data_ptr(), b, t, heads, kv_heads,
+                          room, pos_dev ? pos_dev->const_data_ptr<int64_t>() : nullptr, pos_dev && b > 1 && pos_dev->numel() == b, pos, ctx,
+                          static_cast<float>(scale), out.data_ptr(), need ? ws.data_ptr() : nullptr, need, status.data_ptr<int32_t>(),
+                          c10::cuda::getCurrentCUDAStream().stream()));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_plq_torch, m) {
@@ -280,4 +388,8 @@ PYBIND11_MODULE(_plq_torch, m) {
   m.def("pack", &pack);
   m.def("alone", &alone);
   m.def("decoder_layer", &decoder_layer);
+  m.def("fp8_pack", &fp8_pack);
+  m.def("fp8_gemm", &fp8_gemm);
+  m.def("rope_kv_append_fp8", &rope_kv_append_fp8);
+  m.def("fp8_attention", &fp8_attention);
 }

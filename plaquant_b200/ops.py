@@ -484,6 +484,9 @@ def _check_gamma(gamma: torch.Tensor, k: int, device) -> torch.Tensor:
 def fp8_pack(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Fp8Matrix:
     """[RMSNorm(gamma, eps)] -> E4M3 with a scale per row and 128 columns, of bf16 x[..., K] (K a multiple of 16, at most
     32768).  The normalised values are quantised from float32.  A block with a value that is not finite is NaN as a whole."""
+    done = _lib.torch_lib().fp8_pack(x, None, gamma, eps)
+    if done is not None:
+        return Fp8Matrix(done[1], done[2], 1)
     x2, ld = _rows_of(x, "x")
     rows, k = x2.shape
     p = _fp8_buffers(rows, k, 1, x.device)
@@ -499,6 +502,9 @@ def fp8_pack(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, eps: float =
 def add_rmsnorm_fp8_pack(x: torch.Tensor, residual: torch.Tensor, gamma: torch.Tensor, eps: float):
     """h = residual + x (bf16) -> RMSNorm(gamma, eps) -> E4M3 as fp8_pack.  Returns (h, packed): the residual add, the norm
     and the quantiser of an 8-bit product in one pass."""
+    done = _lib.torch_lib().fp8_pack(x, residual, gamma, eps)
+    if done is not None:
+        return done[0], Fp8Matrix(done[1], done[2], 1)
     if x.shape != residual.shape or x.device != residual.device:
         raise TypeError("x and residual must be bfloat16 tensors of one shape on one device")
     x2, ld = _rows_of(x, "x")
@@ -547,6 +553,13 @@ def fp8_gemm(a: Fp8Matrix, w: Fp8Matrix, out: Optional[torch.Tensor] = None, out
     """y[m, n] = deq(a) @ deq(w).T, float32 sums, bf16 or float32 (`out_dtype`, or that of `out`).  `static_weights`: w was
     complete long before this call, so that its first bytes may be fetched while the previous kernel of the stream drains.
     `variant` picks the kernel ("rows" for up to 64 rows, "128x128", "pair256x256"); default: by the sizes."""
+    flags = int(static_weights) | FP8_GEMM_VARIANTS[variant] << 4
+    if out is None and (out_dtype is torch.bfloat16 or out_dtype is torch.float32):
+        word = _status_words.get(a.codes.get_device())
+        y = None if word is None else _lib.torch_lib().fp8_gemm(a.codes, a.scales, a.block_rows, w.codes, w.scales, w.block_rows, word,
+                                                                out_dtype is torch.float32, flags)
+        if y is not None:
+            return y
     _check_fp8(a, "a", 1)
     _check_fp8(w, "w", FP8_BLOCK)
     if a.k != w.k:
@@ -571,8 +584,7 @@ def fp8_gemm(a: Fp8Matrix, w: Fp8Matrix, out: Optional[torch.Tensor] = None, out
     ld = max(y.stride(0), w.rows) if a.rows > 1 else w.rows
     with torch.cuda.device(a.device):
         st = _lib.lib().plq_fp8_gemm(_ptr(a.codes), _ptr(a.scales), _ptr(w.codes), _ptr(w.scales), a.rows, w.rows, a.k, y.data_ptr(), ld,
-                                     int(dtype == torch.float32), _ptr(status_word(a.device)),
-                                     int(static_weights) | FP8_GEMM_VARIANTS[variant] << 4, _stream(a.device))
+                                     int(dtype == torch.float32), _ptr(status_word(a.device)), flags, _stream(a.device))
     _lib.check(st)
     return y
 
@@ -592,6 +604,11 @@ def rope_kv_append_fp8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
     float32 with T * 128 elements (one row per new position) or B * T * 128 (sequences at different positions).  `pos`: an
     int, or a device int64 tensor with one element or one per sequence; a sequence with a negative position sits out.
     Returns the rotated queries, bf16 [B, T, heads, 128]."""
+    word, at = _status_words.get(qkv.get_device()), pos if isinstance(pos, torch.Tensor) else None
+    q = None if word is None else _lib.torch_lib().rope_kv_append_fp8(qkv, cos, sin, heads, kv_heads, cache.k, cache.k_scale, cache.v,
+                                                                      cache.v_scale, at, pos if at is None else 0, word)
+    if q is not None:
+        return q
     _require_cuda(qkv, "qkv")
     b, t, n = qkv.shape
     if qkv.dtype != torch.bfloat16 or not qkv.is_contiguous() or n != (heads + 2 * kv_heads) * 128:
@@ -619,6 +636,12 @@ def fp8_cache_attention(q: torch.Tensor, cache, pos, scale: Optional[float] = No
     rope_kv_append_fp8; the output of a sequence with a negative position is zero.  `scale`: default 128 ** -0.5.  `ctx`:
     an upper bound of pos + T for positions in device memory (default: the cache's room); it only decides how the work is
     split.  Returns bf16 [B, T, heads, 128]."""
+    scale = 128 ** -0.5 if scale is None else scale
+    word, at = _status_words.get(q.get_device()), pos if isinstance(pos, torch.Tensor) else None
+    out = None if word is None else _lib.torch_lib().fp8_attention(q, cache.k, cache.k_scale, cache.v, cache.v_scale, at, pos if at is None else 0,
+                                                                   ctx or 0, scale, word)
+    if out is not None:
+        return out
     _require_cuda(q, "q")
     if q.dtype != torch.bfloat16 or q.dim() != 4 or q.shape[-1] != 128 or not q.is_contiguous():
         raise TypeError("q must be contiguous bfloat16 [B, T, heads, 128]")
@@ -636,7 +659,7 @@ def fp8_cache_attention(q: torch.Tensor, cache, pos, scale: Optional[float] = No
     with torch.cuda.device(q.device):
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         st = L.plq_fp8_attention(_ptr(q), _ptr(cache.k), _ptr(cache.k_scale), _ptr(cache.v), _ptr(cache.v_scale), b, t, heads, kv_heads,
-                                 cache.room, ptr, each, host, ctx, 128 ** -0.5 if scale is None else float(scale), _ptr(out), _ptr(ws), need,
+                                 cache.room, ptr, each, host, ctx, float(scale), _ptr(out), _ptr(ws), need,
                                  _ptr(status_word(q.device)), _stream(q.device))
     _lib.check(st)
     return out
