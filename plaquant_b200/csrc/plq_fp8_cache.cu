@@ -160,19 +160,34 @@ __global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8Append
 // O^T = V^T P^T has the 128 elements of the head as its lanes.  Each 64-token block of V gets an accumulator of its own, to
 // which the block's scale is applied in float32 on the way into the running sums in registers.
 //   warp 0 producer (TMA: 128 tokens x 128 bytes of keys, of values), warp 1 MMA issuer, warps 2 - 5 softmax and sums
-// The cache's tiles can be split over several CTAs whose partial sums fp8_attention_join_kernel adds in a fixed order.
+// Work: the tiles of all sequences in one row, cut into as many equal runs as CTAs fit the device, so that sequences of
+// different lengths load it evenly and no length has to be known on the host.  A run is one or several segments (tiles of one
+// sequence); a sequence that lies in several runs leaves partial sums, at most two per run (its first and its last segment),
+// which fp8_attention_join_kernel adds in a fixed order.
+constexpr int kMaxFlat = 256;                          // sequences whose tiles are cut as one row
+
 struct Fp8AttnArgs {
   const __nv_bfloat16* q;      // [batch, t, heads, 128]
   const float* k_scale;        // [batch, kv_heads, scale_blocks]
   const float* v_scale;
   __nv_bfloat16* out;          // [batch, t, heads, 128]
-  float* part;                 // [splits][batch * t * heads][128] sums, then [splits][batch * t * heads][2] (maximum, weight)
+  float* part;                 // [units][runs][2][R][128] sums, then [units][runs][2][R][2] (maximum, weight)
   const long long* pos_dev;
-  long long pos, t_max, rows_all;      // rows_all = batch * t * heads
+  long long pos, t_max;
   int* status;
   float scale_log2;            // scale * log2(e)
-  int batch, t, heads, kv_heads, group, pos_batch, scale_blocks, splits, row_tiles;
+  int batch, t, heads, kv_heads, group, pos_batch, scale_blocks, row_tiles;
+  int runs;                    // runs of the row of tiles, or 0: one CTA per sequence
 };
+
+// Tiles of 128 positions that sequence b has (0: it sits out, or does not fit).
+__device__ __forceinline__ int sequence_tiles(const Fp8AttnArgs& a, long long b, long long* pos_out = nullptr) {
+  const long long pos = a.pos_dev != nullptr ? a.pos_dev[b * a.pos_batch] : a.pos;
+  if (pos_out != nullptr) *pos_out = pos;
+  return pos < 0 || pos > a.t_max - a.t ? 0 : static_cast<int>((pos + a.t - 1) / 128) + 1;
+}
+// Run r holds the tiles [r * run_length, (r + 1) * run_length) of the row of tiles; the last runs may be empty.
+__device__ __forceinline__ int run_length(int total, int runs) { return max(1, (total + runs - 1) / runs); }
 
 template <int R>
 struct AtCfg {
@@ -184,7 +199,7 @@ struct AtCfg {
   static constexpr int kDCol0 = 2 * kN;                // two S accumulators, then one D per 64-token block
   static constexpr int kTmemCols = 8 * R;
   static constexpr int kStatFloats = 2 * 4 * R /* warp maxima */ + 4 * 2 * 2 * R /* per warp: factors */ + 4 * R /* per warp: maxima */ + 4 * R;
-  static constexpr size_t kSmemBytes = 1024 + kQBytes + kPBytes + static_cast<size_t>(kKStages + kVStages) * kTile + kStatFloats * 4 + R * 4 + 256;
+  static constexpr size_t kSmemBytes = 1024 + kQBytes + kPBytes + static_cast<size_t>(kKStages + kVStages) * kTile + kStatFloats * 4 + R * 4 + (kMaxFlat + 1) * 4 + 256;
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
 
@@ -224,7 +239,8 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   float* mloc = fac + 4 * 2 * 2 * R;                              // [4 warps][R]: the tile's maxima
   float* red = mloc + 4 * R;                                      // [4 warps][R]
   int* lim_s = reinterpret_cast<int*>(red + 4 * R);               // [R] last position a row sees, relative to the tile loop's base
-  uint64_t* bars = reinterpret_cast<uint64_t*>(lim_s + R);
+  int* first_s = lim_s + R;                                       // [batch + 1] first tile of each sequence in the row of tiles
+  uint64_t* bars = reinterpret_cast<uint64_t*>(first_s + kMaxFlat + 2);
   uint64_t* k_full = bars, *k_empty = k_full + C::kKStages, *v_full = k_empty + C::kKStages, *v_empty = v_full + C::kVStages;
   uint64_t* s_full = v_empty + C::kVStages, *s_empty = s_full + 2, *p_full = s_empty + 2, *d_full = p_full + 1, *q_full = d_full + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_full + 1);
@@ -253,71 +269,126 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   pdl_launch_dependents();
   pdl_wait();
 
-  // ---- this CTA's work: rows [row0, row0 + nrows) of (sequence b, key head kh), tiles [tile0, tile1) of the cache ----
-  const int split = static_cast<int>(blockIdx.x);
-  const int rt = a.row_tiles - 1 - static_cast<int>(blockIdx.y);       // the rows that see most first
-  const int kh = static_cast<int>(blockIdx.z) % a.kv_heads;
-  const long long b = blockIdx.z / static_cast<unsigned>(a.kv_heads);
+  // ---- this CTA's work: rows [row0, row0 + nrows) of key head kh, tiles [run0, run1) of the row of tiles ----
+  const int unit = static_cast<int>(blockIdx.x), run = static_cast<int>(blockIdx.y);
+  const int rt = a.row_tiles - 1 - unit / a.kv_heads, kh = unit % a.kv_heads;       // the rows that see most first
   const int row0 = rt * R, nrows = min(R, a.t * a.group - row0);
-  const long long pos = a.pos_dev != nullptr ? a.pos_dev[b * a.pos_batch] : a.pos;
-  const bool fits = pos <= a.t_max - a.t;
-  if (!fits && threadIdx.x == 0 && a.status != nullptr) atomicExch(a.status, PLQ_DEV_RANGE);
-  int tiles = 0;
   const int i_min = row0 / a.group, i_max = (row0 + nrows - 1) / a.group;
-  if (pos >= 0 && fits) tiles = static_cast<int>((pos + i_max) / 128) + 1;
-  const int tile0 = static_cast<int>(static_cast<long long>(tiles) * split / a.splits);
-  const int tile1 = static_cast<int>(static_cast<long long>(tiles) * (split + 1) / a.splits);
-  const int n = tile1 - tile0;
+  int run0 = 0, run1 = 0;
+  if (a.runs) {
+    if (warp == 0) {                                   // prefix sums of the sequences' tiles
+      int sum = 0;
+      for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const int own = b0 + lane < a.batch ? sequence_tiles(a, b0 + lane) : 0;
+        int x = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int y = __shfl_up_sync(0xFFFFFFFFu, x, d);
+          if (lane >= d) x += y;
+        }
+        if (b0 + lane < a.batch) first_s[b0 + lane] = sum + x - own;
+        sum += __shfl_sync(0xFFFFFFFFu, x, 31);
+      }
+      if (lane == 0) first_s[a.batch] = sum;
+    }
+    __syncthreads();
+    const int length = run_length(first_s[a.batch], a.runs);
+    run0 = min(run * length, first_s[a.batch]);
+    run1 = min(run0 + length, first_s[a.batch]);
+  }
+  // the segments of the run, in order; false behind the last one
+  struct Segment { int b, tile0, n; long long pos; bool whole; };
+  int next_b = a.runs ? 0 : run;
+  if (a.runs)
+    for (int step = kMaxFlat / 2; step >= 1; step >>= 1)          // the last sequence that starts at or before run0
+      if (next_b + step < a.batch && first_s[next_b + step] <= run0) next_b += step;
+  auto next_segment = [&](Segment& g) {
+    if (!a.runs) {
+      if (next_b != run) return false;
+      ++next_b;
+      g.b = run;
+      g.tile0 = 0;
+      g.n = sequence_tiles(a, run, &g.pos);
+      g.whole = true;
+    } else {
+      while (next_b < a.batch && first_s[next_b] < run1 && first_s[next_b + 1] <= max(run0, first_s[next_b])) ++next_b;     // empty ones
+      if (next_b >= a.batch || first_s[next_b] >= run1) return false;
+      g.b = next_b++;
+      const int f = first_s[g.b], all = sequence_tiles(a, g.b, &g.pos);
+      g.tile0 = max(run0 - f, 0);
+      const int end = min(run1 - f, all);
+      g.whole = g.tile0 == 0 && end == all;
+      g.n = end - g.tile0;
+    }
+    if (g.n > 0) g.n = max(0, min(g.n, static_cast<int>((g.pos + i_max) / 128) + 1 - g.tile0));      // what these rows see of it
+    return true;
+  };
+  if (unit == 0 && (run == 0 || !a.runs) && a.status != nullptr) {
+    const int first = a.runs ? static_cast<int>(threadIdx.x) : run;
+    for (int b = first; b < (a.runs ? a.batch : run + 1); b += 192) {
+      const long long pos = a.pos_dev != nullptr ? a.pos_dev[b * a.pos_batch] : a.pos;
+      if (pos > a.t_max - a.t && (a.runs || threadIdx.x == 0)) atomicExch(a.status, PLQ_DEV_RANGE);
+    }
+  }
   const uint32_t k_base = smem_u32(k_s), v_base = smem_u32(v_s);
 
   if (warp == 0) {
     if (elect_one()) {
       bool ok = true;
-      for (int j = 0; ok && j < n; ++j) {
-        const int ks = j % C::kKStages, vs = j % C::kVStages;
-        ok = mbar_wait_bounded(&k_empty[ks], ((j / C::kKStages) & 1u) ^ 1u, abort_flag);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&k_full[ks], C::kTile);
-        tma_load_3d(k_base + ks * C::kTile, &map_k, kh * kHeadDim, (tile0 + j) * 128, static_cast<int>(b), smem_u32(&k_full[ks]));
-        ok = mbar_wait_bounded(&v_empty[vs], ((j / C::kVStages) & 1u) ^ 1u, abort_flag);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&v_full[vs], C::kTile);
-        tma_load_3d(v_base + vs * C::kTile, &map_v, kh * kHeadDim, (tile0 + j) * 128, static_cast<int>(b), smem_u32(&v_full[vs]));
-      }
+      uint32_t gs = 0;
+      Segment g;
+      while (ok && next_segment(g))
+        for (int j = 0; j < g.n; ++j, ++gs) {
+          const uint32_t ks = gs % C::kKStages, vs = gs % C::kVStages;
+          ok = mbar_wait_bounded(&k_empty[ks], ((gs / C::kKStages) & 1u) ^ 1u, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&k_full[ks], C::kTile);
+          tma_load_3d(k_base + ks * C::kTile, &map_k, kh * kHeadDim, (g.tile0 + j) * 128, g.b, smem_u32(&k_full[ks]));
+          ok = mbar_wait_bounded(&v_empty[vs], ((gs / C::kVStages) & 1u) ^ 1u, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&v_full[vs], C::kTile);
+          tma_load_3d(v_base + vs * C::kTile, &map_v, kh * kHeadDim, (g.tile0 + j) * 128, g.b, smem_u32(&v_full[vs]));
+        }
     }
   } else if (warp == 1) {
-    if (elect_one() && n > 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc_s = make_idesc_e4m3(128, C::kN), idesc_d = make_idesc_e4m3(128, C::kN, true, true);
       const uint32_t q_lo = desc_lo_sw128(smem_u32(q_s)), p_lo = desc_lo_p(smem_u32(p_s));
-      bool ok = mbar_wait_bounded(q_full, 0, abort_flag);
-      for (int j = 0; ok && j <= n; ++j) {
-        if (j < n) {                                  // S of tile j
-          const int ks = j % C::kKStages;
-          ok = mbar_wait_bounded(&s_empty[j & 1], ((j >> 1) & 1u) ^ 1u, abort_flag) &&
-               mbar_wait_bounded(&k_full[ks], (j / C::kKStages) & 1u, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t k_lo = desc_lo_sw128(k_base + ks * C::kTile);
+      bool ok = true;
+      uint32_t gs = 0, seg = 0;
+      Segment g;
+      while (ok && next_segment(g)) {
+        if (g.n == 0) continue;
+        ok = mbar_wait_bounded(q_full, seg++ & 1u, abort_flag);
+        for (int j = 0; ok && j <= g.n; ++j) {
+          if (j < g.n) {                              // S of tile j
+            const uint32_t x = gs + j, ks = x % C::kKStages;
+            ok = mbar_wait_bounded(&s_empty[x & 1], ((x >> 1) & 1u) ^ 1u, abort_flag) &&
+                 mbar_wait_bounded(&k_full[ks], (x / C::kKStages) & 1u, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t k_lo = desc_lo_sw128(k_base + ks * C::kTile);
 #pragma unroll
-          for (int h = 0; h < 4; ++h)
-            tc_mma_e4m3<1>(tmem_base + (j & 1) * C::kN, k_lo + 2 * h, kDescHiSw128, q_lo + 2 * h, kDescHiSw128, idesc_s, h != 0);
-          tc_commit<1>(smem_u32(&s_full[j & 1]));
-          tc_commit<1>(smem_u32(&k_empty[ks]));
-        }
-        if (j > 0) {                                  // P V of tile j - 1
-          const int vs = (j - 1) % C::kVStages;
-          ok = mbar_wait_bounded(&v_full[vs], ((j - 1) / C::kVStages) & 1u, abort_flag) &&
-               mbar_wait_bounded(p_full, (j - 1) & 1u, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t v_lo = desc_lo_sw128(v_base + vs * C::kTile);
+            for (int h = 0; h < 4; ++h)
+              tc_mma_e4m3<1>(tmem_base + (x & 1) * C::kN, k_lo + 2 * h, kDescHiSw128, q_lo + 2 * h, kDescHiSw128, idesc_s, h != 0);
+            tc_commit<1>(smem_u32(&s_full[x & 1]));
+            tc_commit<1>(smem_u32(&k_empty[ks]));
+          }
+          if (j > 0) {                                // P V of tile j - 1
+            const uint32_t x = gs + j - 1, vs = x % C::kVStages;
+            ok = mbar_wait_bounded(&v_full[vs], (x / C::kVStages) & 1u, abort_flag) && mbar_wait_bounded(p_full, x & 1u, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t v_lo = desc_lo_sw128(v_base + vs * C::kTile);
 #pragma unroll
-          for (int h = 0; h < 4; ++h)                 // 32 tokens each; two 64-token blocks, two accumulators
-            tc_mma_e4m3<1>(tmem_base + C::kDCol0 + (h >> 1) * C::kN, v_lo + h * (4096 >> 4), kDescHiSw128, p_lo + h * (512 >> 4), kDescHiP,
-                           idesc_d, h & 1);
-          tc_commit<1>(smem_u32(d_full));
-          tc_commit<1>(smem_u32(&v_empty[vs]));
+            for (int h = 0; h < 4; ++h)               // 32 tokens each; two 64-token blocks, two accumulators
+              tc_mma_e4m3<1>(tmem_base + C::kDCol0 + (h >> 1) * C::kN, v_lo + h * (4096 >> 4), kDescHiSw128, p_lo + h * (512 >> 4), kDescHiP,
+                             idesc_d, h & 1);
+            tc_commit<1>(smem_u32(d_full));
+            tc_commit<1>(smem_u32(&v_empty[vs]));
+          }
         }
+        gs += g.n;
       }
     }
   } else {
@@ -326,6 +397,12 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     float* my_fac = fac + sw * 4 * R;
     float* my_max = mloc + sw * R;
 
+    bool ok = true;
+    uint32_t gs = 0;
+    Segment g;
+    while (ok && next_segment(g)) {
+    const long long b = g.b, pos = g.pos;
+    const int n = g.n, tile0 = g.tile0;
     // ---- the queries: tile-wide power-of-two scale, hi and lo codes ----
     constexpr int kPer = R > 16 ? R / 16 : 1;         // 16-element chunks per thread
     const bool has_q = R >= 16 || tid < 8 * R;
@@ -354,6 +431,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     }
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    softmax_barrier();                                // the segment before has been read out
     if (lane == 0) reinterpret_cast<uint32_t*>(red)[sw] = top;
     if (tid < R) {
       const int i = (row0 + tid) / a.group;
@@ -394,7 +472,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     }
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive(q_full);
+    if (lane == 0 && n > 0) mbar_arrive(q_full);
 
     // ---- the tiles ----
     float o[R], l[R], m_run = kNegInf;                // o: element `tok` of the head; m_run: row `lane`
@@ -403,11 +481,10 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     const long long head_scales = (b * a.kv_heads + kh) * a.scale_blocks;
     const int lim_min = static_cast<int>(min(pos + i_min, 0x7FFFFFFFll));
     const long long written = pos + a.t;              // rows behind the last sequence position may hold anything
-    bool ok = true;
 
     // adds the product of the tile before: o = o * alpha + (D0 * vs0 + D1 * vs1) * beta / 256
     auto promote = [&](int j, float vs0, float vs1) {
-      ok = mbar_wait_bounded_lanes(d_full, j & 1u, abort_flag);
+      ok = mbar_wait_bounded_lanes(d_full, (gs + j) & 1u, abort_flag);
       if (!ok) return;
       tc_fence_after();
       const float* f = my_fac + (j & 1) * 2 * R;
@@ -468,31 +545,32 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
         next_v0 = scale_of(v_scale, tile * 2 + 2);
         next_v1 = scale_of(v_scale, tile * 2 + 3);
       }
-      if (ok) ok = mbar_wait_bounded_lanes(&s_full[j & 1], (j >> 1) & 1u, abort_flag);
+      const uint32_t x = gs + j;                      // running index over the segments
+      if (ok) ok = mbar_wait_bounded_lanes(&s_full[x & 1], (x >> 1) & 1u, abort_flag);
       tc_fence_after();
       float s[R];                                      // scores without the scale of the keys
       {
-        const uint32_t at = tmem_base + lane_base + (j & 1) * C::kN;
+        const uint32_t at = tmem_base + lane_base + (x & 1) * C::kN;
         if constexpr (R == 8) {
-          uint32_t x[16];
-          tc_ld_32x32b_x16(at, x);
+          uint32_t v[16];
+          tc_ld_32x32b_x16(at, v);
           tc_wait_ld();
 #pragma unroll
-          for (int r = 0; r < 8; ++r) s[r] = fmaf(__uint_as_float(x[8 + r]), 0.0625f, __uint_as_float(x[r]));
+          for (int r = 0; r < 8; ++r) s[r] = fmaf(__uint_as_float(v[8 + r]), 0.0625f, __uint_as_float(v[r]));
         } else {
 #pragma unroll
           for (int c = 0; c < R / 16; ++c) {
-            uint32_t x[16], y[16];
-            tc_ld_32x32b_x16(at + c * 16, x);
+            uint32_t v[16], y[16];
+            tc_ld_32x32b_x16(at + c * 16, v);
             tc_ld_32x32b_x16(at + R + c * 16, y);
             tc_wait_ld();
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[c * 16 + r] = fmaf(__uint_as_float(y[r]), 0.0625f, __uint_as_float(x[r]));
+            for (int r = 0; r < 16; ++r) s[c * 16 + r] = fmaf(__uint_as_float(y[r]), 0.0625f, __uint_as_float(v[r]));
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[j & 1]);
+        if (lane == 0) mbar_arrive(&s_empty[x & 1]);
       }
       const int token = tile * 128 + tok;
       const bool masked = tile * 128 + 127 > lim_min;            // the same for the whole CTA
@@ -556,8 +634,8 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
         }
       }
       if (static_cast<long long>(tile) * 128 + 128 > written) {  // rows that nobody has written: 0 x NaN would be NaN
-        const int vs = j % C::kVStages;
-        ok = mbar_wait_bounded_lanes(&v_full[vs], (j / C::kVStages) & 1u, abort_flag);
+        const uint32_t vs = x % C::kVStages;
+        ok = mbar_wait_bounded_lanes(&v_full[vs], (x / C::kVStages) & 1u, abort_flag);
         if (!ok) continue;
         if (static_cast<long long>(tile) * 128 + tok >= written) {
           uint4* row = reinterpret_cast<uint4*>(v_s + vs * C::kTile + tok * 128);
@@ -572,32 +650,46 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     }
     if (ok && n > 0) promote(n - 1, vs0, vs1);
 
-    // ---- weights of the rows: over the lanes, then over the warps ----
+    // ---- weights of the rows: over the lanes (each exchange halves the rows a lane still carries), then over the warps ----
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
+    for (int d = 16, cnt = R / 2; cnt >= 1; d >>= 1, cnt >>= 1) {
+      const bool up = (lane & d) != 0;
 #pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], d);
-    }
-    float mine = 0.0f;
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (lane == r) mine = l[r];
-    if (lane < R) red[sw * R + lane] = mine;
-    softmax_barrier();
-    float total = 0.0f;
-    if (lane < R) total = (red[lane] + red[R + lane]) + (red[2 * R + lane] + red[3 * R + lane]);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float sum = __shfl_sync(0xFFFFFFFFu, total, r), m = __shfl_sync(0xFFFFFFFFu, m_run, r);
-      if (r >= nrows) continue;
-      const int row = row0 + r, i = row / a.group, h = row - i * a.group;
-      const long long at = (b * a.t + i) * a.heads + static_cast<long long>(kh) * a.group + h;
-      if (a.splits == 1) {
-        a.out[at * kHeadDim + tok] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : o[r] / sum);
-      } else {
-        if (n > 0) a.part[(split * a.rows_all + at) * kHeadDim + tok] = o[r];
-        if (tok == 0) *reinterpret_cast<float2*>(a.part + a.splits * a.rows_all * kHeadDim + (split * a.rows_all + at) * 2) = make_float2(m, sum);
+      for (int r = 0; r < cnt; ++r) {
+        const float give = up ? l[r] : l[r + cnt], keep_l = up ? l[r + cnt] : l[r];
+        l[r] = keep_l + __shfl_xor_sync(0xFFFFFFFFu, give, d);
       }
+    }
+#pragma unroll
+    for (int d = 16 / R; d >= 1; d >>= 1) l[0] += __shfl_xor_sync(0xFFFFFFFFu, l[0], d);
+    red[sw * R + lane / (32 / R)] = l[0];             // lane 32 / R * r and its neighbours have row r
+    ok = softmax_barrier(ok);
+    float total = 0.0f;
+    if (lane < R) {
+      total = (red[lane] + red[R + lane]) + (red[2 * R + lane] + red[3 * R + lane]);
+      my_max[lane] = total == 0.0f ? 0.0f : 1.0f / total;
+    }
+    __syncwarp();
+    const long long out_row = (b * a.t + i_min) * a.heads + static_cast<long long>(kh) * a.group;
+    if (g.whole) {
+      int h = row0 - i_min * a.group;
+      __nv_bfloat16* dst = a.out + (out_row + h) * kHeadDim + tok;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (r < nrows) *dst = __float2bfloat16_rn(o[r] * my_max[r]);
+        if (++h == a.group) { h = 0; dst += static_cast<long long>(a.heads - a.group) * kHeadDim; }
+        dst += kHeadDim;
+      }
+    } else {
+      const long long slot = (static_cast<long long>(unit) * a.runs + run) * 2 + (first_s[b] + tile0 == run0 ? 0 : 1);
+      float* dst = a.part + slot * R * kHeadDim + tok;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r < nrows) dst[r * kHeadDim] = o[r];
+      if (sw == 0 && lane < nrows)
+        *reinterpret_cast<float2*>(a.part + static_cast<long long>(gridDim.x) * a.runs * 2 * R * kHeadDim + (slot * R + lane) * 2) = make_float2(m_run, total);
+    }
+    gs += n;
     }
   }
 
@@ -614,39 +706,94 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   }
 }
 
-// Adds the splits' partial sums, in order: one CTA of 128 threads per row.
-__global__ void __launch_bounds__(128) fp8_attention_join_kernel(const float* part, __nv_bfloat16* out, long long rows, int splits) {
-  extern __shared__ float weight[];                    // [splits]
+// Adds the partial sums of the sequences that lie in several runs, in a fixed order, and clears the output of those that have
+// no tiles: one CTA of four warps per row, a warp taking every fourth run and a lane four elements.
+__global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnArgs a, int rows_per_tile) {
+  __shared__ int sum_s[4][2];
+  __shared__ float weight_s[4];
+  __shared__ float4 acc_s[4][32];
   pdl_launch_dependents();
   pdl_wait();
-  const long long row = blockIdx.x;
-  const float2* stat = reinterpret_cast<const float2*>(part + splits * rows * kHeadDim);
+  const int at = static_cast<int>(blockIdx.x), bi = at / a.heads, b = bi / a.t;
+  const int head = at - bi * a.heads, i = bi - b * a.t, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = sequence_tiles(a, b);
+  __nv_bfloat16* dst = a.out + static_cast<long long>(at) * kHeadDim;
+  if (tiles == 0) {
+    dst[threadIdx.x] = __float2bfloat16_rn(0.0f);
+    return;
+  }
+  int before = 0, all = 0;                             // tiles of the sequences in front, of all
+  if (a.pos_dev != nullptr && a.pos_batch) {
+    for (int x = threadIdx.x; x < a.batch; x += 128) {
+      const int n = sequence_tiles(a, x);
+      all += n;
+      if (x < b) before += n;
+    }
+    before = __reduce_add_sync(0xFFFFFFFFu, before);
+    all = __reduce_add_sync(0xFFFFFFFFu, all);
+    if (lane == 0) { sum_s[warp][0] = before; sum_s[warp][1] = all; }
+    __syncthreads();
+    before = sum_s[0][0] + sum_s[1][0] + sum_s[2][0] + sum_s[3][0];
+    all = sum_s[0][1] + sum_s[1][1] + sum_s[2][1] + sum_s[3][1];
+  } else {
+    before = tiles * b;
+    all = tiles * a.batch;
+  }
+  const int length = run_length(all, a.runs), r0 = before / length, n = (before + tiles - 1) / length - r0 + 1;
+  if (n == 1) return;                                  // written whole
+  const int kh = head / a.group, row = i * a.group + (head - kh * a.group), rt = row / rows_per_tile;
+  const long long unit = static_cast<long long>(a.row_tiles - 1 - rt) * a.kv_heads + kh;
+  const float2* stat = reinterpret_cast<const float2*>(a.part + static_cast<long long>(a.row_tiles) * a.kv_heads * a.runs * 2 * rows_per_tile * kHeadDim);
+  // the sequence is the first segment of every run but perhaps of the one it starts in
+  const long long base = (unit * a.runs + r0) * 2 * rows_per_tile + (row - rt * rows_per_tile);
+  const int late = r0 * length < before ? rows_per_tile : 0;
+  auto slot = [&](int x) { return base + (x == 0 ? late : static_cast<long long>(x) * 2 * rows_per_tile); };
   float top = kNegInf;
-  for (int s = 0; s < splits; ++s) {
-    const float2 st = stat[s * rows + row];
-    if (st.y != 0.0f) top = fmaxf(top, st.x);
+  for (int x = lane; x < n; x += 32) {
+    const float2 s = stat[slot(x)];
+    if (s.y != 0.0f) top = fmaxf(top, s.x);
   }
-  float total = 0.0f;
-  for (int s = 0; s < splits; ++s) {
-    const float2 st = stat[s * rows + row];
-    const float w = st.y == 0.0f ? 0.0f : ex2_approx(st.x - top);
-    if (threadIdx.x == 0) weight[s] = st.y == 0.0f ? -1.0f : w;
-    total = fmaf(st.y, w, total);
-  }
-  __syncthreads();
-  float sum = 0.0f;
+  top = warp_max(top);
+  float weight = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float w = weight[s];
-    if (w != -1.0f) sum = fmaf(part[(s * rows + row) * kHeadDim + threadIdx.x], w, sum);
+  for (int x = warp; x < n; x += 4) {                  // a run of which the row sees nothing left zeros
+    const long long sl = slot(x);
+    const float2 s = stat[sl];
+    const float4 v = *reinterpret_cast<const float4*>(a.part + sl * kHeadDim + 4 * lane);
+    const float w = s.y == 0.0f ? 0.0f : ex2_approx(s.x - top);
+    weight = fmaf(s.y, w, weight);
+    acc = make_float4(fmaf(v.x, w, acc.x), fmaf(v.y, w, acc.y), fmaf(v.z, w, acc.z), fmaf(v.w, w, acc.w));
   }
-  out[row * kHeadDim + threadIdx.x] = __float2bfloat16_rn(total == 0.0f ? 0.0f : sum / total);
+  acc_s[warp][lane] = acc;
+  if (lane == 0) weight_s[warp] = weight;
+  __syncthreads();
+  weight = (weight_s[0] + weight_s[1]) + (weight_s[2] + weight_s[3]);
+  const float* part = reinterpret_cast<const float*>(acc_s) + threadIdx.x;
+  const float sum = (part[0] + part[128]) + (part[256] + part[384]);
+  dst[threadIdx.x] = __float2bfloat16_rn(weight == 0.0f ? 0.0f : sum / weight);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
 // u8 cache [batch, t_max, kv_heads * 128]: boxes of 128 tokens x 128 bytes, 128-byte swizzle, zeros behind t_max.
 static int make_cache_tmap(CUtensorMap* tm, const void* base, int64_t batch, int64_t t_max, int64_t kv_heads) {
   return make_tmap_3d(tm, base, kv_heads * kHeadDim, t_max, batch, kHeadDim, 128);
+}
+
+// Rows of a CTA, their tiles, and runs of the row of tiles (0: one CTA per sequence) for a call that sees up to `ctx` positions.
+struct AttnPlan { int rows, row_tiles, runs; };
+static AttnPlan attn_plan(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t ctx) {
+  AttnPlan p;
+  const int64_t rows = t * (heads / kv_heads);
+  p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
+  // Two CTAs fit an SM: as many runs as fill the device once, none shorter than four tiles of 128 positions (a CTA's set-up
+  // and its share of the join cost about what two tiles do).
+  const int64_t tiles = (ctx + 127) / 128, units = kv_heads * p.row_tiles;
+  int64_t runs = 2 * static_cast<int64_t>(sm_count()) / units;
+  if (runs > batch * tiles / 4) runs = batch * tiles / 4;
+  p.runs = batch > kMaxFlat || batch * tiles > (1 << 30) || tiles <= 4 || runs < 2 ? 0 : static_cast<int>(runs);
+  return p;
 }
 
 template <int R>
@@ -660,7 +807,7 @@ static int launch_attention(const CUtensorMap& mk, const CUtensorMap& mv, const 
     done_dev = dev;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.splits), static_cast<unsigned>(a.row_tiles), static_cast<unsigned>(a.batch * a.kv_heads));
+  cfg.gridDim = dim3(static_cast<unsigned>(a.kv_heads * a.row_tiles), static_cast<unsigned>(a.runs ? a.runs : a.batch));
   cfg.blockDim = dim3(192, 1, 1);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = static_cast<cudaStream_t>(stream);
@@ -670,31 +817,13 @@ static int launch_attention(const CUtensorMap& mk, const CUtensorMap& mv, const 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp8_attention_kernel<R>, mk, mv, a));
-  if (a.splits > 1) {
-    cfg.gridDim = dim3(static_cast<unsigned>(a.rows_all));
+  if (a.runs) {
+    cfg.gridDim = dim3(static_cast<unsigned>(a.batch * a.t * a.heads));
     cfg.blockDim = dim3(128, 1, 1);
-    cfg.dynamicSmemBytes = a.splits * sizeof(float);
-    PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp8_attention_join_kernel, const_cast<const float*>(a.part), a.out, static_cast<long long>(a.rows_all), a.splits));
+    cfg.dynamicSmemBytes = 0;
+    PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp8_attention_join_kernel, a, R));
   }
   return PLQ_OK;
-}
-
-// Rows of a CTA and splits of the cache for a call that sees up to `ctx` positions.
-struct AttnPlan { int rows, row_tiles, splits; };
-static AttnPlan attn_plan(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t ctx) {
-  AttnPlan p;
-  const int64_t rows = t * (heads / kv_heads);
-  p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-  p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
-  // Two CTAs fit an SM.  As many splits as fill the device once, none shorter than four tiles of 128 tokens: a CTA's
-  // set-up and its share of the join cost about what two tiles do.
-  const int64_t ctas = batch * kv_heads * p.row_tiles, slots = 2 * static_cast<int64_t>(sm_count());
-  int64_t splits = slots / ctas;
-  const int64_t most = ((ctx + 127) / 128 + 3) / 4;
-  if (splits > most) splits = most;
-  if (splits < 1) splits = 1;
-  p.splits = static_cast<int>(splits);
-  return p;
 }
 
 }  // namespace plq
@@ -757,7 +886,7 @@ extern "C" int64_t plq_fp8_attention_workspace_bytes(int64_t batch, int64_t t, i
   using namespace plq;
   if (batch < 1 || t < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || ctx < 1) return 0;
   const AttnPlan p = attn_plan(batch, t, heads, kv_heads, ctx);
-  return p.splits == 1 ? 0 : p.splits * batch * t * heads * static_cast<int64_t>((kHeadDim + 2) * sizeof(float));
+  return kv_heads * p.row_tiles * static_cast<int64_t>(p.runs) * 2 * p.rows * static_cast<int64_t>((kHeadDim + 2) * sizeof(float));
 }
 
 extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const void* k_scales_f32, const void* v_codes, const void* v_scales_f32,
@@ -768,7 +897,7 @@ extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const 
   if (batch < 0 || t < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || t_max < 1 || ctx < 1 || ctx > t_max) return PLQ_ERR_SHAPE;
   if (pos_dev == nullptr && pos >= 0 && (t > t_max || pos > t_max - t)) return PLQ_ERR_SHAPE;
   if (pos_dev == nullptr && pos >= 0 && pos + t > ctx) return PLQ_ERR_SHAPE;
-  if (heads > 4096 || batch * kv_heads > 65535 || t > (1 << 24) || t_max > 0x7FFFFFFF - 128) return PLQ_ERR_LIMIT;
+  if (heads > 4096 || batch > 65535 || t > (1 << 24) || batch * t * heads > 0x7FFFFFFF || t_max > 0x7FFFFFFF - 128) return PLQ_ERR_LIMIT;
   if (batch == 0 || t == 0) return PLQ_OK;
   if (!q_bf16 || !k_codes || !k_scales_f32 || !v_codes || !v_scales_f32 || !out_bf16) return PLQ_ERR_NULL;
   if (!aligned16(q_bf16) || !aligned16(k_codes) || !aligned16(v_codes) || !aligned16(out_bf16) || !aligned16(workspace) ||
@@ -777,8 +906,8 @@ extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const 
   int st = device_check();
   if (st != PLQ_OK) return st;
   const AttnPlan p = attn_plan(batch, t, heads, kv_heads, ctx);
-  if (p.row_tiles > 65535) return PLQ_ERR_LIMIT;
-  if (p.splits > 1 && !workspace) return PLQ_ERR_NULL;
+  if (kv_heads * static_cast<int64_t>(p.row_tiles) > 0x7FFFFFFF) return PLQ_ERR_LIMIT;
+  if (p.runs && !workspace) return PLQ_ERR_NULL;
   if (workspace_bytes < plq_fp8_attention_workspace_bytes(batch, t, heads, kv_heads, ctx)) return PLQ_ERR_LIMIT;
   Fp8AttnArgs a;
   a.q = static_cast<const __nv_bfloat16*>(q_bf16);
@@ -789,7 +918,6 @@ extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const 
   a.pos_dev = reinterpret_cast<const long long*>(pos_dev);
   a.pos = pos;
   a.t_max = t_max;
-  a.rows_all = batch * t * heads;
   a.status = dev_status;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.batch = static_cast<int>(batch);
@@ -799,7 +927,7 @@ extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const 
   a.group = static_cast<int>(heads / kv_heads);
   a.pos_batch = pos_per_sequence ? 1 : 0;
   a.scale_blocks = static_cast<int>((t_max + kCacheBlock - 1) / kCacheBlock);
-  a.splits = p.splits;
+  a.runs = p.runs;
   a.row_tiles = p.row_tiles;
   CUtensorMap mk, mv;
   memset(&mk, 0, sizeof(mk));

@@ -40,20 +40,22 @@ template <> __device__ __forceinline__ float round_out<float>(float v) { return 
 template <> __device__ __forceinline__ __nv_bfloat16 round_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // ---- a few rows ------------------------------------------------------------------------------------------------------
-// MR: activation rows (accumulator columns), 16, 32 or 64.  Tiles of 128 weight rows.  Where there are fewer tiles than
-// CTA slots a cluster of S CTAs shares a tile along K; CTAs 1 .. S-1 hand their sums to CTA 0 through its (by then idle)
-// ring of stages, and CTA 0 adds them in order: results do not depend on timing and no scratch in HBM is needed.
+// MR: activation rows of a tile (accumulator columns), 16, 32 or 64; more rows are several groups of 64.  A tile is 128 weight
+// rows x one group.  Where there are fewer tiles than CTA slots a cluster of S CTAs shares a tile along K; each leaves its
+// sums in the shared memory of the CTA that owns the activation row (row j: CTA j mod S), which adds them in the order of the
+// slices: results do not depend on timing and no scratch in HBM is needed.
 //   warp 0 producer, warp 1 MMA issuer, warps 2 - 5 epilogue (one weight row per thread)
 template <int MR>
 struct GvCfg {
-  static constexpr int kStages = MR == 64 ? 4 : MR == 32 ? 5 : 6;
+  static constexpr int kStages = MR == 64 ? 3 : MR == 32 ? 4 : 5;
   static constexpr int kXBytes = MR * kStageKBytes;
   static constexpr int kStageBytes = kABytes + kXBytes;
   static constexpr int kAcc = MR == 64 ? 4 : 8;                       // accumulators in flight
   static constexpr int kTmemCols = MR == 16 ? 128 : 256;              // two CTAs share an SM
-  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + 512;
-  static constexpr int kSlotBytes = MR * 128 * 4;                     // one CTA's partial sums
-  static constexpr int kMaxSlices = kStages * kStageBytes / kSlotBytes + 1 < 8 ? kStages * kStageBytes / kSlotBytes + 1 : 8;
+  static constexpr int kMaxSlices = 8;
+  static constexpr int kSlotRows = MR + kMaxSlices;                   // S slices x ceil(MR / S) rows
+  static constexpr int kSlotBytes = kSlotRows * 128 * 4;
+  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kSlotBytes + 4 * MR * 4 + 512;
   static constexpr int kThreads = 192;
   static_assert(kAcc * MR <= kTmemCols, "tensor memory budget");
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
@@ -64,7 +66,9 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
   using C = GvCfg<MR>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes);
+  float* slots = reinterpret_cast<float*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes);       // [slice][owned row][128]
+  float* factors = slots + C::kSlotBytes / 4;                         // [4 warps][MR] scales of the K block at hand
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(factors + 4 * MR);
   uint64_t* empty_bar = full_bar + C::kStages;
   uint64_t* acc_full = empty_bar + C::kStages;
   uint64_t* acc_empty = acc_full + C::kAcc;
@@ -89,36 +93,36 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
   }
   tc_fence_before();
   __syncthreads();
+  if (nslice > 1) cluster_arrive_release();            // waited for in front of the first store to another CTA
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   pdl_launch_dependents();
 
   const int kb0 = g.kb * slice / nslice, kb1 = g.kb * (slice + 1) / nslice;
   const int first_tile = static_cast<int>(cluster_id_x()), tile_step = static_cast<int>(nclusters_x());
+  const int num_tiles = g.tiles_n * g.tiles_m;         // tiles_m: groups of activation rows, neighbours share a weight tile
   const uint32_t smem_base = smem_u32(smem);
 
-  float acc[MR];                                 // epilogue: this weight row's sums
-#pragma unroll
-  for (int j = 0; j < MR; ++j) acc[j] = 0.0f;
+  float acc[MR];                                       // epilogue: this weight row's sums
 
   if (warp == 0) {
     if (elect_one()) {
       auto load_w = [&](uint32_t slot, int tile, int kb) {
         mbar_arrive_expect_tx(&full_bar[slot], C::kStageBytes);
-        tma_load_2d_cg<1>(smem_base + slot * C::kStageBytes, &maps.w, kb * kStageKBytes, tile * kBM, smem_u32(&full_bar[slot]));
+        tma_load_2d_cg<1>(smem_base + slot * C::kStageBytes, &maps.w, kb * kStageKBytes, tile / g.tiles_m * kBM, smem_u32(&full_bar[slot]));
       };
-      auto load_x = [&](uint32_t slot, int kb) {
-        tma_load_2d_cg<1>(smem_base + slot * C::kStageBytes + kABytes, &maps.a, kb * kStageKBytes, 0, smem_u32(&full_bar[slot]));
+      auto load_x = [&](uint32_t slot, int tile, int kb) {
+        tma_load_2d_cg<1>(smem_base + slot * C::kStageBytes + kABytes, &maps.a, kb * kStageKBytes, tile % g.tiles_m * MR, smem_u32(&full_bar[slot]));
       };
       // Static weights: the first ring fill of weight bytes is requested while the previous kernel drains.
       uint32_t early = 0;
       if (g.static_w)
-        for (int tile = first_tile; tile < g.tiles_n && early < C::kStages; tile += tile_step)
+        for (int tile = first_tile; tile < num_tiles && early < C::kStages; tile += tile_step)
           for (int kb = kb0; kb < kb1 && early < C::kStages; ++kb, ++early) load_w(early, tile, kb);
       pdl_wait();
       uint32_t gs = 0;
       bool ok = true;
-      for (int tile = first_tile; ok && tile < g.tiles_n; tile += tile_step)
+      for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step)
         for (int kb = kb0; kb < kb1; ++kb, ++gs) {
           const uint32_t slot = gs % C::kStages;
           if (gs >= early) {
@@ -126,7 +130,7 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
             if (!ok) break;
             load_w(slot, tile, kb);
           }
-          load_x(slot, kb);
+          load_x(slot, tile, kb);
         }
     }
   } else if (warp == 1) {
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
       constexpr uint32_t idesc = make_idesc_e4m3(128, MR);
       uint32_t gs = 0;
       bool ok = true;
-      for (int tile = first_tile; ok && tile < g.tiles_n; tile += tile_step)
+      for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step)
         for (int kb = kb0; kb < kb1; ++kb, ++gs) {
           const uint32_t slot = gs % C::kStages, as = gs % C::kAcc;
           ok = mbar_wait_bounded(&acc_empty[as], ((gs / C::kAcc) & 1u) ^ 1u, abort_flag) &&
@@ -150,22 +154,24 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
         }
     }
   } else {
-    // ---- epilogue: thread = weight row; lane l of a warp carries the scales of activation rows l (and l + 32) ----
+    // ---- epilogue: thread = weight row; lane l of a warp fetches the scales of activation rows l (and l + 32) ----
     constexpr int kPer = MR > 32 ? 2 : 1;
     const int trow = (warp & 3) * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    float* my_factors = factors + (warp - 2) * MR;
     pdl_wait();
     uint32_t gs = 0;
     bool ok = true;
-    for (int tile = first_tile; ok && tile < g.tiles_n; tile += tile_step) {
+    for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
 #pragma unroll
       for (int j = 0; j < MR; ++j) acc[j] = 0.0f;
-      const float* sw = g.sw + static_cast<long long>(tile) * g.kb;
+      const int row0 = tile % g.tiles_m * MR;
+      const float* sw = g.sw + static_cast<long long>(tile / g.tiles_m) * g.kb;
       auto scale = [&](int kb, int p) {
         const int row = lane + 32 * p;
-        return kb < kb1 && row < g.m && row < MR ? g.sa[static_cast<long long>(row) * g.kb + kb] * sw[kb] : 0.0f;
+        return kb < kb1 && row0 + row < g.m && row < MR ? g.sa[static_cast<long long>(row0 + row) * g.kb + kb] * sw[kb] : 0.0f;
       };
-      float next[4][kPer];                       // scales of the next four K blocks, on their way
+      float next[4][kPer];                             // scales of the next four K blocks, on their way
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -179,60 +185,66 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (!ok || kb + i >= kb1) break;
+          __syncwarp();
+#pragma unroll
+          for (int p = 0; p < kPer; ++p)
+            if (lane + 32 * p < MR) my_factors[lane + 32 * p] = f[i][p];
           const uint32_t as = gs % C::kAcc;
-          ok = mbar_wait_bounded_warp(&acc_full[as], (gs / C::kAcc) & 1u, abort_flag);
+          ok = mbar_wait_bounded_lanes(&acc_full[as], (gs / C::kAcc) & 1u, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          uint32_t r[MR / 16][16];
 #pragma unroll
-          for (int c = 0; c < MR / 16; ++c) tc_ld_32x32b_x16(tmem_base + lane_base + as * MR + c * 16, r[c]);
-          tc_wait_ld();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[as]);
+          for (int c = 0; c < MR / 16; ++c) {
+            uint32_t r[16];
+            tc_ld_32x32b_x16(tmem_base + lane_base + as * MR + c * 16, r);
+            tc_wait_ld();
+            if (c == MR / 16 - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&acc_empty[as]);
+            }
 #pragma unroll
-          for (int j = 0; j < MR; ++j)
-            acc[j] = fmaf(__uint_as_float(r[j / 16][j & 15]), __shfl_sync(0xFFFFFFFFu, f[i][j / 32], j & 31), acc[j]);
+            for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(__uint_as_float(r[j]), my_factors[c * 16 + j], acc[c * 16 + j]);
+          }
           ++gs;
         }
       }
       if (nslice == 1 && ok) {
-        const long long row = static_cast<long long>(tile) * kBM + trow;
-        OUT* y = static_cast<OUT*>(g.y) + row;
+        const long long row = static_cast<long long>(tile / g.tiles_m) * kBM + trow;
+        OUT* y = static_cast<OUT*>(g.y) + row0 * g.ldy + row;
         if (row < g.n) {
 #pragma unroll
           for (int j = 0; j < MR; ++j)
-            if (j < g.m) y[j * g.ldy] = round_out<OUT>(acc[j]);
+            if (row0 + j < g.m) y[j * g.ldy] = round_out<OUT>(acc[j]);
         }
       }
     }
   }
-  if (nslice > 1) {
-    // One tile per cluster.  First barrier: CTA 0's MMAs have read its ring and nothing is on its way into it.
-    const bool sender = slice > 0 && warp >= 2, receiver = slice == 0 && warp >= 2;
-    const int trow = (warp & 3) * 32 + lane;
+  if (nslice > 1) {                                    // one tile per cluster
+    const int trow = (warp & 3) * 32 + lane, row0 = first_tile % g.tiles_m * MR, rows = min(MR, g.m - row0), per = (MR + nslice - 1) / nslice;
+    __syncwarp();
+    cluster_wait_acquire();                            // every CTA of the cluster is there
+    if (warp >= 2) {
+      const uint32_t own = smem_u32(slots) + static_cast<uint32_t>((slice * per * 128 + trow) * 4);
+      int cta = 0, at = 0;                             // row j: CTA j % S, its row j / S
+#pragma unroll
+      for (int j = 0; j < MR; ++j) {
+        if (j < rows) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(own + at * 512u, static_cast<uint32_t>(cta))), "f"(acc[j]) : "memory");
+        if (++cta == nslice) { cta = 0; ++at; }
+      }
+    }
     __syncwarp();
     cluster_arrive_release();
     cluster_wait_acquire();
-    if (sender) {
-      const uint32_t dst = map_to_cta(smem_base, 0u) + static_cast<uint32_t>((slice - 1) * C::kSlotBytes + trow * 4);
+    const long long row = static_cast<long long>(first_tile / g.tiles_m) * kBM + trow;
+    if (warp >= 2 && !*abort_flag && row < g.n) {
+      OUT* y = static_cast<OUT*>(g.y) + row0 * g.ldy + row;
+      for (int j = slice, at = 0; j < rows; j += nslice, ++at) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < MR; ++j) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + j * 512), "f"(acc[j]) : "memory");
-    }
-    cluster_arrive_release();
-    cluster_wait_acquire();
-    if (receiver && !*abort_flag) {
-      const float* slots = reinterpret_cast<const float*>(smem);
-      for (int s = 0; s < nslice - 1; ++s) {
-#pragma unroll
-        for (int j = 0; j < MR; ++j) acc[j] += slots[s * (C::kSlotBytes / 4) + j * 128 + trow];
-      }
-      const long long row = static_cast<long long>(first_tile) * kBM + trow;
-      OUT* y = static_cast<OUT*>(g.y) + row;
-      if (row < g.n) {
-#pragma unroll
-        for (int j = 0; j < MR; ++j)
-          if (j < g.m) y[j * g.ldy] = round_out<OUT>(acc[j]);
+        for (int s = 0; s < C::kMaxSlices; ++s)
+          if (s < nslice) sum += slots[(s * per + at) * 128 + trow];
+        y[j * g.ldy] = round_out<OUT>(sum);
       }
     }
   }
@@ -250,26 +262,24 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------
-// Persistent; warp 0 producer, warp 1 MMA issuer (leader CTA of a pair), warp 2 fetches scales, warps 4 - 11 epilogue: four
-// warps (the quadrants of tensor memory) for either half of the tile's columns, each thread one row x 64 or 128 float32 sums.
+// Persistent; warps 0 and 3 producers (alternate K blocks), warp 1 MMA issuer (leader CTA of a pair), warp 2 fetches scales, warps 4 and up epilogue: four
+// warps (the quadrants of tensor memory) for every 64 columns of the tile, each thread one row x 64 float32 sums.
 // Per K block an epilogue warp reads its columns from tensor memory and does one packed multiply-add per two of them,
 // beside the 256 (128 x 128) or 512 cycles of the block's MMAs.  The scales travel ahead of the epilogue through a ring of
 // their own (cp.async, 16 K blocks deep): loaded by the epilogue itself their latency was longer than a K block.
 template <int BN, int CG>
 struct GmCfg {
   static constexpr int kBRows = BN / CG;
-  static constexpr int kStageBytes = kABytes + kBRows * kStageKBytes;      // 32 KiB
-  static constexpr int kStages = 6;
+  static constexpr int kStageBytes = kABytes + kBRows * kStageKBytes;
+  static constexpr int kStages = 196608 / kStageBytes;                      // 6 x 32 KiB or 8 x 24 KiB
   static constexpr int kAcc = 512 / BN;
-  static constexpr int kCols = BN / 2;                                      // per epilogue warp
+  static constexpr int kCols = 64;                                          // per epilogue warp
+  static constexpr int kEpiWarps = 4 * BN / kCols;
   static constexpr int kSfSlots = 16;
   static constexpr int kSfBytes = 512 + 16;                                 // 128 row scales, the scales of the tile's weight blocks
-  static constexpr int kThreads = 384;
-  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kSfSlots * kSfBytes + 512;
-  static_assert(kStageBytes == 32768 && kSmemBytes <= 232448, "shared memory budget");
-  // Registers: 168 a thread at launch (384 x 168); the epilogue of 128 columns needs more, the other warpgroup less.
-  static constexpr int kRegsMain = 72, kRegsEpi = 216;
-  static_assert(128 * kRegsMain + 256 * kRegsEpi <= 384 * 168, "register split");
+  static constexpr int kThreads = 128 + 32 * kEpiWarps;
+  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kSfSlots * kSfBytes + 640;
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
 // Tile order: bands of `band` row tiles, M fastest inside a band, so that the CTAs running together share operands in L2.
@@ -299,8 +309,8 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
   const bool leader = rank == 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int s = 0; s < C::kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8 * CG); }
-    for (int s = 0; s < C::kSfSlots; ++s) { mbar_init(&sf_full[s], 32); mbar_init(&sf_empty[s], 8); }
+    for (int s = 0; s < C::kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], C::kEpiWarps * CG); }
+    for (int s = 0; s < C::kSfSlots; ++s) { mbar_init(&sf_full[s], 32); mbar_init(&sf_empty[s], C::kEpiWarps); }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -324,20 +334,19 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
   const int step = CG == 2 ? static_cast<int>(nclusters_x()) : static_cast<int>(gridDim.x);
   const uint32_t smem_base = smem_u32(smem);
 
-  if constexpr (BN == 256)
-    if (warp < 4) registers_down<C::kRegsMain>();
-  if (warp == 0) {
+  if (warp == 0 || warp == 3) {
     if (elect_one()) {
       pdl_wait();
+      const uint32_t mine = warp == 0 ? 0u : 1u;       // K blocks of this producer: every other one, over all tiles
       uint32_t gs = 0;
       bool ok = true;
       for (int tile = first; ok && tile < num_tiles; tile += step) {
         int tm, tn;
         fp8_tile(tile, g, tm, tn);
         const int row_a = (tm * CG + static_cast<int>(rank)) * kBM, row_b = tn * BN + static_cast<int>(rank) * C::kBRows;
-        for (int kb = 0; kb < g.kb; ++kb, ++gs) {
-          const uint32_t slot = gs % C::kStages;
-          ok = mbar_wait_bounded(&empty_bar[slot], ((gs / C::kStages) & 1u) ^ 1u, abort_flag);
+        for (int kb = static_cast<int>((gs ^ mine) & 1u); kb < g.kb; kb += 2) {
+          const uint32_t x = gs + kb, slot = x % C::kStages;
+          ok = mbar_wait_bounded(&empty_bar[slot], ((x / C::kStages) & 1u) ^ 1u, abort_flag);
           if (!ok) break;
           const uint32_t st = smem_base + slot * C::kStageBytes;
           // in a pair every load of both CTAs is counted on the leader's barrier
@@ -346,6 +355,7 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
           tma_load_2d_cg<CG>(st, &maps.a, kb * kStageKBytes, row_a, bar);
           tma_load_2d_cg<CG>(st + kABytes, &maps.w, kb * kStageKBytes, row_b, bar);
         }
+        gs += g.kb;
       }
     }
   } else if (warp == 1) {
@@ -401,7 +411,6 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
       }
     }
   } else if (warp >= 4) {
-    if constexpr (BN == 256) registers_up<C::kRegsEpi>();
     const int quad = warp & 3, cgp = (warp - 4) >> 2;
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t empty_addr = CG == 2 ? map_to_cta(smem_u32(acc_empty), 0u) : smem_u32(acc_empty);
@@ -421,31 +430,29 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
         ok = mbar_wait_bounded_lanes(&sf_full[slot], (gs / C::kSfSlots) & 1u, abort_flag);
         if (!ok) break;
         const float* sf = reinterpret_cast<const float*>(sf_ring + slot * C::kSfBytes);
-        const float f = sf[quad * 32 + lane] * sf[128 + (BN == 256 ? cgp : 0)];
+        const float f = sf[quad * 32 + lane] * sf[128 + cgp / 2];
         const float2 f2 = make_float2(f, f);
         ok = mbar_wait_bounded_lanes(&acc_full[as], (gs / C::kAcc) & 1u, abort_flag);
         if (!ok) break;
         tc_fence_after();
         const uint32_t taddr = tmem_base + lane_base + as * BN + cgp * C::kCols;
-        uint32_t r[2][32];
-        tc_ld_32x32b_x32(taddr, r[0]);
 #pragma unroll
-        for (int c = 0; c < C::kCols / 32; ++c) {
+        for (int c = 0; c < C::kCols / 16; ++c) {
+          uint32_t r[16];
+          tc_ld_32x32b_x16(taddr + c * 16, r);
           tc_wait_ld();
-          if (c + 1 < C::kCols / 32) {
-            tc_ld_32x32b_x32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
-          } else {
+          if (c == C::kCols / 16 - 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-              mbar_arrive(&sf_empty[slot]);
               if constexpr (CG == 2) mbar_arrive_relaxed_cluster(empty_addr + 8u * as);
               else mbar_arrive(&acc_empty[as]);
+              mbar_arrive(&sf_empty[slot]);
             }
           }
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[c * 16 + j] = __ffma2_rn(make_float2(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1])), f2, acc[c * 16 + j]);
+          for (int j = 0; j < 8; ++j)
+            acc[c * 8 + j] = __ffma2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), f2, acc[c * 8 + j]);
         }
       }
       if (!ok) break;
@@ -538,6 +545,37 @@ static int launch_clusters(K kernel, unsigned grid, unsigned cluster, unsigned t
 
 struct Fp8Ptrs { const void *a, *w; int64_t k; };
 
+// Clusters of `slices` CTAs that the device holds at once; looked up once per thread and device.
+template <int MR, typename OUT>
+static int gemv_clusters(int slices) {
+  using C = GvCfg<MR>;
+  static thread_local int cached_dev = -1;
+  static thread_local int table[C::kMaxSlices + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (cached_dev != dev) {
+    for (int s = 1; s <= C::kMaxSlices; ++s) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(static_cast<unsigned>(s * 64), 1, 1);
+      cfg.blockDim = dim3(C::kThreads, 1, 1);
+      cfg.dynamicSmemBytes = C::kSmemBytes;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = static_cast<unsigned>(s);
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, fp8_gemv_kernel<MR, OUT>, &cfg) != cudaSuccess) n = 0;
+      table[s] = n;
+    }
+    (void)cudaGetLastError();
+    cached_dev = dev;
+  }
+  return table[slices];
+}
+
 template <int MR, typename OUT>
 static int launch_gemv(const Fp8Ptrs& p, Fp8GemmArgs& g, void* stream) {
   using C = GvCfg<MR>;
@@ -550,12 +588,14 @@ static int launch_gemv(const Fp8Ptrs& p, Fp8GemmArgs& g, void* stream) {
   if ((st = make_tmap(&tm.w, p.w, g.n, p.k, kBM)) != PLQ_OK) return st;
   if ((st = make_tmap(&tm.a, p.a, g.m, p.k, MR)) != PLQ_OK) return st;
   g.tiles_n = (g.n + kBM - 1) / kBM;
-  const int slots = 2 * sm_count();
-  int slices = slots / g.tiles_n;
+  g.tiles_m = (g.m + MR - 1) / MR;
+  const int slots = 2 * sm_count(), tiles = g.tiles_n * g.tiles_m;
+  int slices = slots / tiles;
   if (slices > C::kMaxSlices) slices = C::kMaxSlices;
   if (slices > g.kb) slices = g.kb;
+  while (slices > 1 && gemv_clusters<MR, OUT>(slices) < tiles) --slices;       // all at once
   if (slices < 1) slices = 1;
-  const int grid = slices > 1 ? g.tiles_n * slices : (g.tiles_n < slots ? g.tiles_n : slots);
+  const int grid = slices > 1 ? tiles * slices : (tiles < slots ? tiles : slots);
   return launch_clusters(kernel, static_cast<unsigned>(grid), static_cast<unsigned>(slices), C::kThreads, C::kSmemBytes, stream, tm, g);
 }
 
@@ -589,12 +629,13 @@ static int launch_fp8(const Fp8Ptrs& p, Fp8GemmArgs& g, int variant, void* strea
     else variant = (wide + pairs - 1) / pairs * 2 <= (small + sms - 1) / sms ? PLQ_FP8_PAIR_256x256 : PLQ_FP8_128x128;
   }
   if (variant == PLQ_FP8_ROWS) {
-    if (g.m > 64) return PLQ_ERR_SHAPE;
+    if (g.m > 1024) return PLQ_ERR_SHAPE;
     if (g.m <= 16) return launch_gemv<16, OUT>(p, g, stream);
     return g.m <= 32 ? launch_gemv<32, OUT>(p, g, stream) : launch_gemv<64, OUT>(p, g, stream);
   }
   if (variant == PLQ_FP8_128x128) return launch_gemm_fp8<128, 1, OUT>(p, g, stream);
   if (variant == PLQ_FP8_PAIR_256x256) return launch_gemm_fp8<256, 2, OUT>(p, g, stream);
+  if (variant == PLQ_FP8_PAIR_256x128) return launch_gemm_fp8<128, 2, OUT>(p, g, stream);
   return PLQ_ERR_SHAPE;
 }
 
@@ -604,7 +645,7 @@ extern "C" int plq_fp8_gemm(const void* a_codes, const void* a_scales_f32, const
                             int64_t k, void* y, int64_t ldy, int y_is_f32, int32_t* dev_status, int flags, void* stream) {
   using namespace plq;
   const int variant = flags >> 4;
-  if (m < 1 || n < 1 || k < 16 || k % 16 != 0 || ldy < n || variant < 0 || variant > PLQ_FP8_PAIR_256x256) return PLQ_ERR_SHAPE;
+  if (m < 1 || n < 1 || k < 16 || k % 16 != 0 || ldy < n || variant < 0 || variant > PLQ_FP8_PAIR_256x128) return PLQ_ERR_SHAPE;
   if (m > (1 << 30) || n > (1 << 30) || k > (1 << 24) || (m + 127) / 128 * ((n + 127) / 128) > 0x7FFFFFFF) return PLQ_ERR_LIMIT;
   if (!a_codes || !a_scales_f32 || !w_codes || !w_scales_f32 || !y || !dev_status) return PLQ_ERR_NULL;
   const uintptr_t es = y_is_f32 ? 4 : 2;
