@@ -38,6 +38,17 @@ __device__ __forceinline__ uint32_t e4m3_split(float a, float b) {
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(lo) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
   return hi | static_cast<uint32_t>(lo) << 16;
 }
+// The same with the rest as E5M2 codes, whose smallest step is 2^-16.
+__device__ __forceinline__ uint32_t e4m3_e5m2_split(float a, float b) {
+  uint32_t x, back;
+  uint16_t hi, lo;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(hi) : "r"(x));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(hi));
+  const __half2 rest = __hsub2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&back));
+  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(lo) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
+  return hi | static_cast<uint32_t>(lo) << 16;
+}
 __device__ __forceinline__ uint2 e4m3x8(const float (&y)[8]) {
   return make_uint2(e4m3x2(y[0], y[1]) | e4m3x2(y[2], y[3]) << 16, e4m3x2(y[4], y[5]) | e4m3x2(y[6], y[7]) << 16);
 }
@@ -62,6 +73,24 @@ __device__ __forceinline__ void tc_mma_e4m3(uint32_t d_tmem, uint32_t a_lo, uint
                  "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p;\n\t}" ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo),
                  "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
 }
+
+// The same with A in tensor memory: row = lane, four consecutive elements of K per 32-bit column.
+__device__ __forceinline__ void tc_mma_e4m3_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 db, {%2, %3};\n\t"
+               "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], db, %4, p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc),
+               "r"(accumulate) : "memory");
+}
+constexpr uint32_t kIdescAE5m2 = 1u << 7;              // A as E5M2 instead of E4M3
+
+// 16 consecutive 32-bit columns of a warp's 32 lanes
+__device__ __forceinline__ void tc_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+      "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 32 lanes x 16 consecutive 32-bit columns
 __device__ __forceinline__ void tc_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {

@@ -774,17 +774,378 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
   dst[threadIdx.x] = __float2bfloat16_rn(weight == 0.0f ? 0.0f : sum / weight);
 }
 
+// ---- attention of many queries -----------------------------------------------------------------------------------------
+// The same sums with the queries as the 128 lanes: S = Q K^T, O = P V, a thread owning a row, so that a row's maximum and
+// weight need no exchange.  A CTA has two tiles of 128 rows (queries x heads of a group): while the tensor core works for
+// one, the other's warps turn scores into weights.
+//   q      hi + lo, both E4M3 at the scale of the row (a power of two that brings its largest element to [128, 256)): exact
+//          for what is at least 2^-10 of that, off by 2^-18 of it below
+//   p      hi + lo, E4M3 + E5M2, in tensor memory (A operand), in the place of the scores they come from: off by at most 2^-8
+//          of itself, or half a step of 2^-16
+//   O      stays in tensor memory.  The scale of a block of V is part of the weight's exponent: w = exp2(score + log2 vs - M + 2),
+//          with M within 2^6 of the row's largest such sum so far (only beyond that is O scaled, which is rare), and the sum of
+//          the weights takes w / vs.  So a block of large values that nobody looks at does not set the scale of the others.
+//   warp 0 producer, warp 1 MMA issuer, warps 4 - 7 and 8 - 11 one tile of rows each
+// Bound by the tensor core (four products of 128 x 128 x 128 per tile: 1024 cycles) and by exponentials (16 a cycle: 1024 cycles).
+struct PfCfg {
+  static constexpr int kTile = 128 * kHeadDim;          // 16 KiB
+  static constexpr int kStages = 3;
+  static constexpr size_t kSmemBytes = 1024 + 4 * kTile + 2 * kStages * kTile + 256;
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+constexpr float kHeadroom = 6.0f;                       // log2 of how far a weight may exceed that of M
+
+__global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                             const Fp8AttnArgs a) {
+  using C = PfCfg;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_s = smem;                                  // [row tile][hi | lo][128 x 128 bytes]
+  uint8_t* k_s = q_s + 4 * C::kTile;
+  uint8_t* v_s = k_s + C::kStages * C::kTile;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(v_s + C::kStages * C::kTile);
+  uint64_t* k_empty = k_full + C::kStages, *v_full = k_empty + C::kStages, *v_empty = v_full + C::kStages;
+  uint64_t* q_full = v_empty + C::kStages, *s_full = q_full + 2, *p_full = s_full + 2, *o_full = p_full + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_full + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+    for (int x = 0; x < 2; ++x) { mbar_init(&q_full[x], 4); mbar_init(&s_full[x], 1); mbar_init(&p_full[x], 4); mbar_init(&o_full[x], 1); }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && elect_one()) { prefetch_tmap(&map_k); prefetch_tmap(&map_v); }
+  if (warp == 1) {
+    tmem_alloc<1>(tmem_holder, 512);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;              // per row tile 128 columns of S (and P), 128 of O
+  pdl_launch_dependents();
+  pdl_wait();
+
+  const int b = static_cast<int>(blockIdx.y), kh = static_cast<int>(blockIdx.x) % a.kv_heads;
+  const int pair = a.row_tiles - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;       // the rows that see most first
+  const int rows = a.t * a.group, row0 = pair * 256;
+  const long long pos = a.pos_dev != nullptr ? a.pos_dev[static_cast<long long>(b) * a.pos_batch] : a.pos;
+  const bool fits = pos <= a.t_max - a.t;
+  if (!fits && threadIdx.x == 0 && a.status != nullptr) atomicExch(a.status, PLQ_DEV_RANGE);
+  // tiles of 128 positions that the rows of tile x see
+  auto tiles_of = [&](int x) {
+    const int first = row0 + 128 * x, last = min(first + 128, rows) - 1;
+    return first >= rows || pos < 0 || !fits ? 0 : static_cast<int>((pos + last / a.group) / 128) + 1;
+  };
+  const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+  const uint32_t q_base = smem_u32(q_s), k_base = smem_u32(k_s), v_base = smem_u32(v_s);
+
+  if (warp == 0) {
+    if (elect_one()) {
+      bool ok = true;
+      for (int j = 0; ok && j < n; ++j) {
+        const int st = j % C::kStages;
+        const uint32_t parity = ((j / C::kStages) & 1u) ^ 1u;
+        ok = mbar_wait_bounded(&k_empty[st], parity, abort_flag);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&k_full[st], C::kTile);
+        tma_load_3d(k_base + st * C::kTile, &map_k, kh * kHeadDim, j * 128, b, smem_u32(&k_full[st]));
+        ok = mbar_wait_bounded(&v_empty[st], parity, abort_flag);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&v_full[st], C::kTile);
+        tma_load_3d(v_base + st * C::kTile, &map_v, kh * kHeadDim, j * 128, b, smem_u32(&v_full[st]));
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one() && n > 0) {
+      constexpr uint32_t idesc_s = make_idesc_e4m3(128, 128), idesc_o = make_idesc_e4m3(128, 128, false, true);
+      bool ok = true;
+      // A tile of K (V) is free behind the second row tile's product, or the first's where the second does not reach it.
+      auto scores = [&](int x, int j) {
+        const int st = j % C::kStages;
+        ok = ok && mbar_wait_bounded(&k_full[st], (j / C::kStages) & 1u, abort_flag);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t q_lo = desc_lo_sw128(q_base + 2 * x * C::kTile), k_lo = desc_lo_sw128(k_base + st * C::kTile);
+#pragma unroll
+        for (int h = 0; h < 8; ++h)
+          tc_mma_e4m3<1>(tmem_base + 256 * x, q_lo + (h >> 2) * (C::kTile >> 4) + 2 * (h & 3), kDescHiSw128, k_lo + 2 * (h & 3), kDescHiSw128, idesc_s, h != 0);
+        tc_commit<1>(smem_u32(&s_full[x]));
+        if (x == 1 || j >= n1) tc_commit<1>(smem_u32(&k_empty[st]));
+      };
+      for (int x = 0; ok && x < 2; ++x)
+        if ((x ? n1 : n0) > 0) {
+          ok = mbar_wait_bounded(&q_full[x], 0, abort_flag);
+          scores(x, 0);
+        }
+      for (int j = 0; ok && j < n; ++j)
+        for (int x = 0; ok && x < 2; ++x) {
+          const int mine = x ? n1 : n0;
+          if (j >= mine) continue;
+          const int st = j % C::kStages;
+          ok = mbar_wait_bounded(&v_full[st], (j / C::kStages) & 1u, abort_flag) && mbar_wait_bounded(&p_full[x], j & 1u, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t v_lo = desc_lo_sw128(v_base + st * C::kTile), p = tmem_base + 256 * x, o = p + 128;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {                 // 32 positions each: codes of hi, then of lo
+            tc_mma_e4m3_ts(o, p + 16 * h, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, j > 0 || h > 0);
+            tc_mma_e4m3_ts(o, p + 16 * h + 8, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o | kIdescAE5m2, 1u);
+          }
+          if (x == 1 || j >= n1) tc_commit<1>(smem_u32(&v_empty[st]));
+          if (j + 1 == mine) tc_commit<1>(smem_u32(&o_full[x]));
+          else scores(x, j + 1);                        // behind the product that still reads P: same pipe, in order
+        }
+    }
+  } else if (warp >= 4) {
+    const int x = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, row = row0 + 128 * x + r;
+    const int mine = x ? n1 : n0, i = row / a.group, h = row - i * a.group;
+    const bool real = row < rows;
+    const uint32_t s_at = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + 256 * x, o_at = s_at + 128;
+    const long long at = (static_cast<long long>(b) * a.t + i) * a.heads + static_cast<long long>(kh) * a.group + h;
+
+    // ---- the row's query: scale, hi and lo codes ----
+    float down;
+    {
+      const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu;
+      uint4 qv[16];
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + at * kHeadDim);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) qv[c] = real ? src[c] : make_uint4(0, 0, 0, 0);
+      uint32_t top = 0;
+      uint32_t* w = reinterpret_cast<uint32_t*>(qv);
+#pragma unroll
+      for (int d = 0; d < 64; ++d) {
+        w[d] = (w[d] & keep) ^ flip;
+        const uint32_t lo = (w[d] << 16) & 0x7FFF0000u, hi = w[d] & 0x7FFF0000u;
+        if (lo < 0x7F800000u) top = max(top, lo);
+        if (hi < 0x7F800000u) top = max(top, hi);
+      }
+      const int e = top == 0 ? 0 : min(max(134 - static_cast<int>(top >> 23), -120), 120);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          uint32_t h2[2], l2[2];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            float f0 = bf16lo_to_f32(w[8 * c + 2 * d + y]) * up, f1 = bf16hi_to_f32(w[8 * c + 2 * d + y]) * up;
+            if (isinf(f0)) f0 = __uint_as_float(0x7FFFFFFFu);      // an infinite query is NaN, not the largest number
+            if (isinf(f1)) f1 = __uint_as_float(0x7FFFFFFFu);
+            h2[y] = e4m3x2(f0, f1);
+            const float2 back = e4m3x2_to_f32x2(h2[y]);
+            l2[y] = e4m3x2(f0 - back.x, f1 - back.y);
+          }
+          hi[d] = h2[0] | h2[1] << 16;
+          lo[d] = l2[0] | l2[1] << 16;
+        }
+        uint8_t* dst = q_s + 2 * x * C::kTile + (r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + C::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[x]);
+    }
+
+    // ---- the tiles ----
+    const long long scales = (static_cast<long long>(b) * a.kv_heads + kh) * a.scale_blocks;
+    const float* k_scale = a.k_scale + scales;
+    const float* v_scale = a.v_scale + scales;
+    const long long written = pos + a.t;                // positions behind may hold anything
+    const int last_block = static_cast<int>((written - 1) / kCacheBlock);
+    const float per_k = down * (a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2));
+    const long long lim = real ? pos + i : pos + a.t - 1;                             // last position the row sees
+    const long long lim_min = pos + (row0 + 128 * x) / a.group;                       // ... of any row of the tile
+    float M = 0.0f, weight = 0.0f;
+    bool ok = true;
+    float next_k[2] = {1.0f, 1.0f}, next_v[2] = {1.0f, 1.0f};
+    auto fetch = [&](int j) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        if (2 * j + y <= last_block) { next_k[y] = k_scale[2 * j + y]; next_v[y] = v_scale[2 * j + y]; }
+    };
+    if (mine > 0) fetch(0);
+    for (int j = 0; ok && j < mine; ++j) {
+      float ck[2], lv[2], inv_v[2];
+      const long long t0 = static_cast<long long>(j) * 128;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const bool sees = lim >= t0 + kCacheBlock * y;
+        ck[y] = sees ? next_k[y] * per_k : 1.0f;
+        if (ck[y] < 1.2e-38f) ck[y] = 1.2e-38f;         // a score of zero, and minus infinity stays what it is
+        float vs = sees ? next_v[y] : 1.0f;
+        if (vs < 1e-36f) vs = 1e-36f;
+        lv[y] = __log2f(vs);
+        inv_v[y] = 1.0f / vs;
+      }
+      if (j + 1 < mine) fetch(j + 1);
+      ok = mbar_wait_bounded_lanes(&s_full[x], j & 1u, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const bool masked = t0 + 127 > lim_min;           // the same for the whole row tile
+      const int cut = static_cast<int>(min(lim - t0, 127ll));                         // last visible position of the tile
+      float top[2] = {kNegInf, kNegInf};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tc_ld_32x32b_x32(s_at + 32 * c, v);
+        tc_wait_ld();
+        if (masked) {
+#pragma unroll
+          for (int d = 0; d < 32; ++d)
+            if (32 * c + d > cut) v[d] = 0xFF800000u;
+        }
+#pragma unroll
+        for (int d = 0; d < 32; ++d) top[c >> 1] = fmaxf(top[c >> 1], __uint_as_float(v[d]));
+      }
+      const float t_max = fmaxf(fmaf(top[0], ck[0], lv[0]), fmaf(top[1], ck[1], lv[1]));
+      if (j == 0) {
+        M = t_max > kNegInf ? t_max : 0.0f;
+      } else {
+        const bool grow = t_max > M + kHeadroom;
+        if (__any_sync(0xFFFFFFFFu, grow)) {            // O is at rest: its product ended before the scores'
+          const float alpha = grow ? ex2_approx(M - t_max) : 1.0f;
+          if (grow) M = t_max;
+          weight *= alpha;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t v[16];
+            tc_ld_32x32b_x16(o_at + 16 * c, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int d = 0; d < 16; ++d) v[d] = __float_as_uint(__uint_as_float(v[d]) * alpha);
+            tc_st_32x32b_x16(o_at + 16 * c, v);
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32], p[16];
+        tc_ld_32x32b_x32(s_at + 32 * c, v);
+        tc_wait_ld();
+        const float shift = lv[c >> 1] + (8.0f - kHeadroom) - M;
+        float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 32; d += 4) {
+          float w[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) w[y] = ex2_approx(fmaf(__uint_as_float(v[d + y]), ck[c >> 1], shift));
+          if (masked) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (32 * c + d + y > cut) w[y] = 0.0f;
+          }
+          sum0 += w[0] + w[1];
+          sum1 += w[2] + w[3];
+          const uint32_t c0 = e4m3_e5m2_split(w[0], w[1]), c1 = e4m3_e5m2_split(w[2], w[3]);
+          p[d / 4] = __byte_perm(c0, c1, 0x5410);
+          p[8 + d / 4] = __byte_perm(c0, c1, 0x7632);
+        }
+        weight = fmaf(sum0 + sum1, inv_v[c >> 1], weight);
+        tc_st_32x32b_x16(s_at + 16 * c, p);             // columns of S that have been read
+      }
+      if (t0 + 128 > written) {                         // positions that nobody has written: 0 x NaN would be NaN
+        const int st = j % C::kStages;
+        ok = mbar_wait_bounded_lanes(&v_full[st], (j / C::kStages) & 1u, abort_flag);
+        if (!ok) break;
+        if (t0 + r >= written) {
+          uint4* dst = reinterpret_cast<uint4*>(v_s + st * C::kTile + r * 128);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[x]);
+    }
+
+    // ---- out ----
+    uint4* dst = reinterpret_cast<uint4*>(a.out + at * kHeadDim);
+    if (mine == 0) {
+      if (real)
+#pragma unroll
+        for (int c = 0; c < 16; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+    } else {
+      if (ok) ok = mbar_wait_bounded_lanes(&o_full[x], 0, abort_flag);
+      tc_fence_after();
+      const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint32_t v[16], o[8];
+        tc_ld_32x32b_x16(o_at + 16 * c, v);
+        tc_wait_ld();
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d] = f32x2_to_bf16x2(__uint_as_float(v[2 * d]) * inv, __uint_as_float(v[2 * d + 1]) * inv);
+        if (real) {
+          dst[2 * c] = make_uint4(o[0], o[1], o[2], o[3]);
+          dst[2 * c + 1] = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0 && a.status != nullptr) atomicExch(a.status, PLQ_DEV_TIMEOUT);
+    const long long t0 = clock64();                     // copies still in flight get time to land
+    while (clock64() - t0 < 400000ll) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem_base, 512);
+  }
+}
+
 // ---- host side -------------------------------------------------------------------------------------------------------
 // u8 cache [batch, t_max, kv_heads * 128]: boxes of 128 tokens x 128 bytes, 128-byte swizzle, zeros behind t_max.
 static int make_cache_tmap(CUtensorMap* tm, const void* base, int64_t batch, int64_t t_max, int64_t kv_heads) {
   return make_tmap_3d(tm, base, kv_heads * kHeadDim, t_max, batch, kHeadDim, 128);
 }
 
+static int launch_prefill(const CUtensorMap& mk, const CUtensorMap& mv, const Fp8AttnArgs& a, void* stream) {
+  static thread_local int done_dev = -1;
+  int dev = 0;
+  PLQ_CUDA_TRY(cudaGetDevice(&dev));
+  if (done_dev != dev) {
+    PLQ_CUDA_TRY(cudaFuncSetAttribute(fp8_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PfCfg::kSmemBytes)));
+    done_dev = dev;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.kv_heads * a.row_tiles), static_cast<unsigned>(a.batch));
+  cfg.blockDim = dim3(384, 1, 1);
+  cfg.dynamicSmemBytes = PfCfg::kSmemBytes;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp8_prefill_kernel, mk, mv, a));
+  return PLQ_OK;
+}
+
 // Rows of a CTA, their tiles, and runs of the row of tiles (0: one CTA per sequence) for a call that sees up to `ctx` positions.
+// rows = 256: fp8_prefill_kernel.
 struct AttnPlan { int rows, row_tiles, runs; };
 static AttnPlan attn_plan(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t ctx) {
   AttnPlan p;
   const int64_t rows = t * (heads / kv_heads);
+  if (rows > 32 && batch * kv_heads * ((rows + 255) / 256) >= 18) {
+    p.rows = 256;
+    p.row_tiles = static_cast<int>((rows + 255) / 256);
+    p.runs = 0;
+    return p;
+  }
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
   p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
   // Two CTAs fit an SM: as many runs as fill the device once, none shorter than four tiles of 128 positions (a CTA's set-up
@@ -934,6 +1295,7 @@ extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const 
   memset(&mv, 0, sizeof(mv));
   if ((st = make_cache_tmap(&mk, k_codes, batch, t_max, kv_heads)) != PLQ_OK) return st;
   if ((st = make_cache_tmap(&mv, v_codes, batch, t_max, kv_heads)) != PLQ_OK) return st;
+  if (p.rows == 256) return launch_prefill(mk, mv, a, stream);
   if (p.rows == 8) return launch_attention<8>(mk, mv, a, stream);
   return p.rows == 16 ? launch_attention<16>(mk, mv, a, stream) : launch_attention<32>(mk, mv, a, stream);
 }

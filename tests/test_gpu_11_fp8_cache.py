@@ -189,9 +189,12 @@ def _filled(plq, batch, room, kv_heads, lengths, seed, gain=1.0):
 
 
 def _check_attention(out, q, cache, pos, scale=128 ** -0.5):
-    """Against float64.  Allowed: the rounding of the result (2^-8) and, relative to the largest value that a row sees: 2^-12
-    for weights of 12 bits, 2^-11 for their fixed step of 2^-18 of the tile's largest weight over 128 tokens, and twice the
-    error of a score, which is 2^-22 of max |q| sum |k| (query in 8 + 14 bits) and 2^-21 of its own size (float32, exp2)."""
+    """Against float64, within what the arithmetic allows of either kernel, element by element:
+      a weight w is two codes - off by 2^-8 of itself at most (E4M3: half of 2^-3; of that rest, E5M2: half of 2^-2 of at most
+      2^-4 = 2^-7 in all against the binade, 2^-8 of its largest value) - or by half a step: 2^-18 of the largest weight of its
+      128 positions (E4M3 alone, the largest brought to 256), 2^-19 of the row's largest w vs over its own vs (E5M2, 4 to 256);
+      a query's element that is below 2^-9 of the row's largest is off by 2^-17 of it or by itself, the others are exact;
+      the score's float32 arithmetic and exponential by 2^-21 of its size; the result's rounding by 2^-8."""
     b, t, heads, _ = q.shape
     group = heads // cache.kv_heads
     for i in range(b):
@@ -202,14 +205,22 @@ def _check_attention(out, q, cache, pos, scale=128 ** -0.5):
         s = lambda x: x[i].double().repeat_interleave(BLOCK, -1)[:, :n, None]        # noqa: E731
         k = cache.k[i, :n].contiguous().view(torch.float8_e4m3fn).double().transpose(0, 1) * s(cache.k_scale)
         v = cache.v[i, :n].contiguous().view(torch.float8_e4m3fn).double().transpose(0, 1) * s(cache.v_scale)
-        qq = q[i].double().view(t, cache.kv_heads, group, 128).permute(1, 2, 0, 3)                   # [kv, group, t, 128]
-        score = qq @ k[:, None].transpose(-1, -2) * scale
-        seen = torch.arange(n, device=q.device)[None, :] <= pos[i] + torch.arange(t, device=q.device)[:, None]
-        score = score.masked_fill(~seen, -math.inf)
-        want = (torch.softmax(score, -1) @ v[:, None]).permute(2, 0, 1, 3).reshape(t, heads, 128)
-        off = 2.0 ** -22 * scale * float(qq.abs().max()) * float(k.abs().sum(-1).max()) + 2.0 ** -21 * float(score[seen.expand_as(score)].abs().max())
-        bound = want.abs() * 2.0 ** -8 + (2.0 ** -12 + 2.0 ** -11 + 2 * off) * float(v.abs().max()) * (1 + 2.0 ** -8)
-        err = (out[i].double() - want).abs()
+        vs = s(cache.v_scale)[..., 0][:, None]                                                     # [kv, 1, n]
+        qq = q[i].double().view(t, cache.kv_heads, group, 128).permute(1, 2, 0, 3).reshape(cache.kv_heads, group * t, 128)
+        score = qq @ k.transpose(-1, -2) * scale
+        seen = (torch.arange(n, device=q.device)[None, :] <= pos[i] + torch.arange(t, device=q.device)[:, None]).repeat(group, 1)
+        w = torch.exp(score - score.masked_fill(~seen, -math.inf).amax(-1, keepdim=True)).masked_fill(~seen, 0.0)
+        total = w.sum(-1, keepdim=True)
+        want = w @ v / total
+        tile = torch.nn.functional.pad(w, (0, -n % 128)).unflatten(-1, (-1, 128)).amax(-1).repeat_interleave(128, -1)[..., :n]
+        step = torch.maximum(2.0 ** -18 * tile, 2.0 ** -19 * (w * vs).amax(-1, keepdim=True) / vs)
+        top = qq.abs().amax(-1, keepdim=True)
+        dq = torch.where(qq.abs() < 2.0 ** -9 * top, torch.minimum(qq.abs(), 2.0 ** -17 * top), torch.zeros_like(qq))
+        off = w * (torch.expm1(abs(scale) * (dq @ k.abs().transpose(-1, -2)) + 2.0 ** -21 * (1 + score.abs())))
+        err_w = torch.maximum(2.0 ** -8 * w, step) * seen + off
+        bound = want.abs() * (2.0 ** -8 + off.sum(-1, keepdim=True) / total) + err_w @ v.abs() / total
+        put = lambda x: x.view(cache.kv_heads, group, t, 128).permute(2, 0, 1, 3).reshape(t, heads, 128)      # noqa: E731
+        err, bound = (out[i].double() - put(want)).abs(), put(bound) * (1 + 2.0 ** -6) + 1e-37
         assert torch.all(err <= bound), (i, float((err / bound).max()))
 
 
@@ -311,6 +322,72 @@ def test_attention_keeps_what_is_not_finite_where_it_is_seen(plq):
     assert torch.all(got[hit].isnan()) and not got[~hit].isnan().any()
     # positions behind the last one may hold NaN codes and scales (every cache here does)
     plq.check_device_status()
+
+
+# ---- many queries: rows of a tile are queries x heads of a group --------------------------------------------------------
+@pytest.mark.parametrize("b,t,heads,kv_heads,pos", [(18, 9, 4, 1, 0), (18, 33, 1, 1, 0), (3, 129, 12, 6, 70), (5, 65, 16, 4, 1000), (2, 256, 9, 9, 127), (9, 64, 8, 2, 64),
+                                                    (1, 1000, 40, 8, 0), (2, 300, 16, 2, 5000), (18, 300, 5, 1, 63)])
+def test_attention_of_many_queries(plq, b, t, heads, kv_heads, pos):
+    cache = _filled(plq, b, pos + t + 5, kv_heads, [pos + t] * b, heads * 100 + t + pos)
+    q = _rand_q((b, t, heads, 128), t + pos).cuda()
+    out = plq.ops.fp8_cache_attention(q, cache, pos)
+    _check_attention(out, q, cache, [pos] * b)
+    assert torch.equal(plq.ops.fp8_cache_attention(q, cache, torch.tensor([pos], device="cuda")), out)
+    plq.check_device_status()
+
+
+@pytest.mark.parametrize("lengths", [[0, 129, 500, -1, 63, 64], [1000, 2, 1, 190, -1, 0]])
+def test_many_queries_of_ragged_batches(plq, lengths):
+    pos = [n - 1 if n == 0 else n for n in lengths]
+    cache = _filled(plq, 6, max(lengths) + 160, 3, [p + 100 if p >= 0 else 0 for p in pos], 50)
+    q = _rand_q((6, 100, 6, 128), 51).cuda()
+    _check_attention(plq.ops.fp8_cache_attention(q, cache, torch.tensor(pos, device="cuda")), q, cache, pos)
+    q = _rand_q((6, 100, 6, 128), 51).cuda()
+    over = torch.tensor([max(lengths) + 61] + pos[1:], device="cuda")
+    out = plq.ops.fp8_cache_attention(q, cache, over)
+    assert torch.all(out[0] == 0)
+    with pytest.raises(plq.PlqError):
+        plq.check_device_status()
+
+
+@pytest.mark.parametrize("gain,q_gain,scale", [(1.0, 30.0, None), (1e-3, 1.0, None), (1e4, 1e-4, None), (1.0, 1.0, 0.0), (1.0, 0.0, None), (1.0, 1.0, -0.3), (1e-30, 1e30, None)])
+def test_many_queries_of_sharp_flat_large_and_small_scores(plq, gain, q_gain, scale):
+    cache = _filled(plq, 5, 900, 4, [900] * 5, 52, gain)
+    q = _rand_q((5, 70, 16, 128), 53, q_gain).cuda()
+    out = plq.ops.fp8_cache_attention(q, cache, 830, scale=scale)
+    _check_attention(out, q, cache, [830] * 5, 128 ** -0.5 if scale is None else scale)
+
+
+def test_many_queries_where_the_maximum_moves(plq):
+    """Keys that grow along the cache: every tile's scores exceed those before, and then fall again; blocks of V of very
+    different size, the largest where nobody looks."""
+    cache = _filled(plq, 5, 1500, 4, [1500] * 5, 54)
+    ramp = torch.cat([torch.arange(12), torch.arange(12).flip(0)])[: cache.k_scale.shape[-1]]
+    cache.k_scale.mul_(torch.exp2((ramp - 8).float()).cuda())
+    q = _rand_q((5, 200, 16, 128), 55, 1.0).cuda()
+    _check_attention(plq.ops.fp8_cache_attention(q, cache, 1300), q, cache, [1300] * 5)
+    cache.v_scale[..., ::3] *= 2.0 ** -9
+    cache.k_scale[..., 1::3] *= 2.0 ** -12
+    _check_attention(plq.ops.fp8_cache_attention(q, cache, 1300), q, cache, [1300] * 5)
+
+
+def test_many_queries_keep_what_is_not_finite_where_it_is_seen(plq):
+    b, t, pos = 9, 100, 150
+    for side in ("k_scale", "v_scale"):
+        cache = _filled(plq, b, 256, 2, [250] * b, 56)
+        q = _rand_q((b, t, 8, 128), 57).cuda()
+        want = plq.ops.fp8_cache_attention(q, cache, pos)
+        getattr(cache, side)[1, 1, 3] = float("nan")              # positions 192 .. 255 of a sequence's second key head
+        got = plq.ops.fp8_cache_attention(q, cache, pos)
+        hit = torch.zeros(b, t, 8, dtype=torch.bool, device="cuda")
+        hit[1, 192 - pos:, 4:] = True
+        assert torch.all(got[hit].isnan()) and torch.equal(got[~hit], want[~hit])
+    cache = _filled(plq, b, 256, 2, [250] * b, 56)
+    q[0, 7, 3, 5], q[8, 9, 6, 0] = float("nan"), float("inf")
+    got = plq.ops.fp8_cache_attention(q, cache, pos)
+    hit = torch.zeros(b, t, 8, dtype=torch.bool, device="cuda")
+    hit[0, 7, 3] = hit[8, 9, 6] = True
+    assert torch.all(got[hit].isnan()) and torch.equal(got[~hit], want[~hit])
 
 
 def test_attention_reports_positions_outside_the_cache(plq):
