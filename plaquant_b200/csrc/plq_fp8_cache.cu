@@ -791,6 +791,9 @@ struct PfCfg {
   static constexpr int kTile = 128 * kHeadDim;          // 16 KiB
   static constexpr int kStages = 3;
   static constexpr size_t kSmemBytes = 1024 + 4 * kTile + 2 * kStages * kTile + 256;
+  // 168 registers a thread at launch (384 x 168); the warps with a row of scores per thread take what the others leave.
+  static constexpr int kRegsMain = 56, kRegsRows = 224;
+  static_assert(128 * kRegsMain + 256 * kRegsRows <= 384 * 168, "register split");
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 constexpr float kHeadroom = 6.0f;                       // log2 of how far a weight may exceed that of M
@@ -805,14 +808,14 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
   uint8_t* v_s = k_s + C::kStages * C::kTile;
   uint64_t* k_full = reinterpret_cast<uint64_t*>(v_s + C::kStages * C::kTile);
   uint64_t* k_empty = k_full + C::kStages, *v_full = k_empty + C::kStages, *v_empty = v_full + C::kStages;
-  uint64_t* q_full = v_empty + C::kStages, *s_full = q_full + 2, *p_full = s_full + 2, *o_full = p_full + 2;
+  uint64_t* q_full = v_empty + C::kStages, *s_full = q_full + 2, *p_half = s_full + 2, *p_full = p_half + 2, *o_full = p_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_full + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-    for (int x = 0; x < 2; ++x) { mbar_init(&q_full[x], 4); mbar_init(&s_full[x], 1); mbar_init(&p_full[x], 4); mbar_init(&o_full[x], 1); }
+    for (int x = 0; x < 2; ++x) { mbar_init(&q_full[x], 4); mbar_init(&s_full[x], 1); mbar_init(&p_full[x], 4); mbar_init(&p_half[x], 4); mbar_init(&o_full[x], 1); }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -842,6 +845,7 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
   const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
   const uint32_t q_base = smem_u32(q_s), k_base = smem_u32(k_s), v_base = smem_u32(v_s);
 
+  if (warp < 4) registers_down<C::kRegsMain>();
   if (warp == 0) {
     if (elect_one()) {
       bool ok = true;
@@ -885,21 +889,28 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
           const int mine = x ? n1 : n0;
           if (j >= mine) continue;
           const int st = j % C::kStages;
-          ok = mbar_wait_bounded(&v_full[st], (j / C::kStages) & 1u, abort_flag) && mbar_wait_bounded(&p_full[x], j & 1u, abort_flag);
+          ok = mbar_wait_bounded(&v_full[st], (j / C::kStages) & 1u, abort_flag) && mbar_wait_bounded(&p_half[x], j & 1u, abort_flag);
           if (!ok) break;
           tc_fence_after();
           const uint32_t v_lo = desc_lo_sw128(v_base + st * C::kTile), p = tmem_base + 256 * x, o = p + 128;
 #pragma unroll
           for (int h = 0; h < 4; ++h) {                 // 32 positions each: codes of hi, then of lo
+            if (h == 2) {
+              ok = mbar_wait_bounded(&p_full[x], j & 1u, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+            }
             tc_mma_e4m3_ts(o, p + 16 * h, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, j > 0 || h > 0);
             tc_mma_e4m3_ts(o, p + 16 * h + 8, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o | kIdescAE5m2, 1u);
           }
+          if (!ok) break;
           if (x == 1 || j >= n1) tc_commit<1>(smem_u32(&v_empty[st]));
           if (j + 1 == mine) tc_commit<1>(smem_u32(&o_full[x]));
           else scores(x, j + 1);                        // behind the product that still reads P: same pipe, in order
         }
     }
   } else if (warp >= 4) {
+    registers_up<C::kRegsRows>();
     const int x = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, row = row0 + 128 * x + r;
     const int mine = x ? n1 : n0, i = row / a.group, h = row - i * a.group;
     const bool real = row < rows;
@@ -990,19 +1001,26 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
       tc_fence_after();
       const bool masked = t0 + 127 > lim_min;           // the same for the whole row tile
       const int cut = static_cast<int>(min(lim - t0, 127ll));                         // last visible position of the tile
-      float top[2] = {kNegInf, kNegInf};
+      uint32_t v[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tc_ld_32x32b_x32(s_at + 32 * c, v);
-        tc_wait_ld();
-        if (masked) {
+      for (int c = 0; c < 4; ++c) tc_ld_32x32b_x32(s_at + 32 * c, v[c]);
+      tc_wait_ld();
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int d = 0; d < 32; ++d)
-            if (32 * c + d > cut) v[d] = 0xFF800000u;
-        }
+            if (32 * c + d > cut) v[c][d] = 0xFF800000u;
+      }
+      float top[2];
 #pragma unroll
-        for (int d = 0; d < 32; ++d) top[c >> 1] = fmaxf(top[c >> 1], __uint_as_float(v[d]));
+      for (int y = 0; y < 2; ++y) {
+        float m[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) m[d] = fmaxf(__uint_as_float(v[2 * y][d]), __uint_as_float(v[2 * y + 1][d]));
+#pragma unroll
+        for (int d = 4; d < 32; ++d) m[d & 3] = fmaxf(m[d & 3], fmaxf(__uint_as_float(v[2 * y][d]), __uint_as_float(v[2 * y + 1][d])));
+        top[y] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
       }
       const float t_max = fmaxf(fmaf(top[0], ck[0], lv[0]), fmaf(top[1], ck[1], lv[1]));
       if (j == 0) {
@@ -1013,42 +1031,16 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
           const float alpha = grow ? ex2_approx(M - t_max) : 1.0f;
           if (grow) M = t_max;
           weight *= alpha;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 8; ++c) {
-            uint32_t v[16];
-            tc_ld_32x32b_x16(o_at + 16 * c, v);
+            uint32_t w[16];
+            tc_ld_32x32b_x16(o_at + 16 * c, w);
             tc_wait_ld();
 #pragma unroll
-            for (int d = 0; d < 16; ++d) v[d] = __float_as_uint(__uint_as_float(v[d]) * alpha);
-            tc_st_32x32b_x16(o_at + 16 * c, v);
+            for (int d = 0; d < 16; ++d) w[d] = __float_as_uint(__uint_as_float(w[d]) * alpha);
+            tc_st_32x32b_x16(o_at + 16 * c, w);
           }
         }
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32], p[16];
-        tc_ld_32x32b_x32(s_at + 32 * c, v);
-        tc_wait_ld();
-        const float shift = lv[c >> 1] + (8.0f - kHeadroom) - M;
-        float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-        for (int d = 0; d < 32; d += 4) {
-          float w[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) w[y] = ex2_approx(fmaf(__uint_as_float(v[d + y]), ck[c >> 1], shift));
-          if (masked) {
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-              if (32 * c + d + y > cut) w[y] = 0.0f;
-          }
-          sum0 += w[0] + w[1];
-          sum1 += w[2] + w[3];
-          const uint32_t c0 = e4m3_e5m2_split(w[0], w[1]), c1 = e4m3_e5m2_split(w[2], w[3]);
-          p[d / 4] = __byte_perm(c0, c1, 0x5410);
-          p[8 + d / 4] = __byte_perm(c0, c1, 0x7632);
-        }
-        weight = fmaf(sum0 + sum1, inv_v[c >> 1], weight);
-        tc_st_32x32b_x16(s_at + 16 * c, p);             // columns of S that have been read
       }
       if (t0 + 128 > written) {                         // positions that nobody has written: 0 x NaN would be NaN
         const int st = j % C::kStages;
@@ -1061,10 +1053,32 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
         }
         fence_proxy_async_smem();
       }
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[x]);
+      // A block that the row sees and whose scale is NaN makes the row NaN, its masked positions included.
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t p[16];
+        const float shift = lv[c >> 1] + (8.0f - kHeadroom) - M;
+        float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 32; d += 4) {
+          float w[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) w[y] = ex2_approx(fmaf(__uint_as_float(v[c][d + y]), ck[c >> 1], shift));
+          sum0 += w[0] + w[1];
+          sum1 += w[2] + w[3];
+          const uint32_t c0 = e4m3_e5m2_split(w[0], w[1]), c1 = e4m3_e5m2_split(w[2], w[3]);
+          p[d / 4] = __byte_perm(c0, c1, 0x5410);
+          p[8 + d / 4] = __byte_perm(c0, c1, 0x7632);
+        }
+        weight = fmaf(sum0 + sum1, inv_v[c >> 1], weight);
+        tc_st_32x32b_x16(s_at + 16 * c, p);             // columns of S that have been read
+        if (c & 1) {                                    // the product may begin with the first 64 positions
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(c == 1 ? &p_half[x] : &p_full[x]);
+        }
+      }
     }
 
     // ---- out ----
