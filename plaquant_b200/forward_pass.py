@@ -29,7 +29,7 @@ import torch.nn.functional as F
 from torch.nn.attention.bias import causal_lower_right
 
 from . import _lib, kv_cache, ops, tp
-from .quantize import QuantizedLinear
+from .quantize import Fp8Linear, QuantizedLinear
 from .rotation import get_hadamard_matrix  # noqa: F401  (re-exported, as the reference module does)
 
 
@@ -98,19 +98,25 @@ class ResQForwardB200:
 
     `kv` holds the keys and values of each layer, [B, T, kv_heads, head_dim] (or packed rows).  What a caller keeps of it
     stays as it is in later steps and shares no memory with them (a step that finds its cache held copies it).  After a
-    step behind a prompt the sequences of a batch may lie further apart than T rows: `.contiguous()` where that matters."""
+    step behind a prompt the sequences of a batch may lie further apart than T rows: `.contiguous()` where that matters.
+    With kv_quant="fp8" it holds one kv_cache.Fp8Cache per layer, which later steps fill in place (`.clone()` keeps one)."""
     _kv_room = ()                           # per layer: (weak references to the tensors of self.kv, rows allocated)
     _rope_tables = _rope_for = None         # cos / sin rows, and the (theta, head size) they belong to; all three
                                             # also for objects pickled before they existed
+    head8 = None                            # the LM head in E4M3 (fp8_head)
 
     def __init__(self, cfg: LlamaConfig, device, ctx: Optional[tp.TPContext] = None, seed: int = 0,
                  num_layers: Optional[int] = None, fused_reduce_rows: int = 0, kv_quant: bool = False,
                  weights: Optional[Dict[str, torch.Tensor]] = None, packed: Optional[dict] = None,
-                 scatter_prefill_rows: int = 0):
+                 scatter_prefill_rows: int = 0, fp8_head: bool = False):
         """Weights come from one of three places: `packed` (the state a packed-weight container holds, see
         weight_packer.py), `weights` (a dict of full bf16 tensors under the reference's names, `l{i}.q_proj.weight`
         ... as `IndependentResQForward` takes them; every rank picks its own shard), or, with neither, a random
-        initialisation per layer from `seed` (no checkpoints are available offline)."""
+        initialisation per layer from `seed` (no checkpoints are available offline).
+
+        `kv_quant`: False (bf16 cache), True (packed NVFP4 rows), "fp8" (E4M3 with a scale per 64 positions and head, read
+        by the package's own attention), "fake" (the NVFP4 rows' bf16 values).  `fp8_head`: the LM head in E4M3, the last
+        residual add and the final norm in its quantiser; logits are float32 sums."""
         self.cfg, self.device, self.ctx = cfg, torch.device(device), ctx or tp.TPContext()
         c, r, s = cfg, self.ctx.rank, self.ctx.size
         assert c.num_heads % s == 0 and c.num_kv_heads % s == 0 and c.intermediate_size % (s * 128) == 0
@@ -142,12 +148,16 @@ class ResQForwardB200:
                 self.embed = (torch.randn(c.vocab_size, c.hidden_size, generator=g, device=self.device) * 0.02).to(torch.bfloat16)
                 self.final_norm = (torch.rand(c.hidden_size, generator=g, device=self.device) + 0.5).to(torch.bfloat16)
                 self.lm_head = (torch.randn(c.vocab_size, c.hidden_size, generator=g, device=self.device) * 0.02).to(torch.bfloat16)
+        if fp8_head:
+            self.head8 = Fp8Linear.from_weight(self.lm_head)
         self.kv: List[Tuple[torch.Tensor, torch.Tensor]] = []
         self.pos = 0
         self._decode_states: Dict[tuple, _DecodeState] = {}
         # keys go into the cache as NVFP4 (Hadamard over the head dimension, per-head rows), queries get the same
         # rotation: the reference's QKRotationWrapper with k_had (promix/quantize/kv_quant.py:244-279)
-        self.kv_quant = kv_quant                     # False | True (packed NVFP4 rows in the cache) | "fake" (their bf16 values)
+        if kv_quant not in (False, True, "fp8", "fake"):
+            raise ValueError(f"kv_quant is False, True, 'fp8' or 'fake', not {kv_quant!r}")
+        self.kv_quant = kv_quant                     # ... | "fake" (the packed rows' bf16 values)
         if kv_quant and c.head_dim != 128:
             raise ValueError("kv_quant needs head_dim = 128 (one Hadamard block per head)")
         self._make_rope_tables()
@@ -293,6 +303,11 @@ class ResQForwardB200:
         cache -> [B, T, heads * head_dim] (this rank's heads)."""
         c = self.cfg
         b, t, _ = qkv.shape
+        if self.kv_quant == "fp8":
+            cos, sin = cos_sin[0].reshape(t, c.head_dim), cos_sin[1].reshape(t, c.head_dim)
+            cache, pos = (self._fp8_room(li, b, t, pos0), pos0) if static is None else (static["cache"][li], static["pos"])
+            q = ops.rope_kv_append_fp8(qkv, cos, sin, self.heads, self.kv_heads, cache, pos)
+            return ops.fp8_cache_attention(q, cache, pos).view(b, t, self.heads * c.head_dim)
         if c.head_dim == 128 and self.kv_quant != "fake":
             # RoPE on q and k and the cache append in one kernel (the float32 arithmetic of _rope, bit for bit); into a
             # packed cache it also rotates the keys and quantises (the bytes of kv_cache.pack_head_rows)
@@ -394,6 +409,18 @@ class ResQForwardB200:
         self._kv_room[li] = (weakref.ref(k), weakref.ref(v), cap)
         return k, v, n, cap
 
+    def _fp8_room(self, li: int, b: int, t: int, pos0: int) -> kv_cache.Fp8Cache:
+        """The E4M3 cache of layer `li` with room for positions up to pos0 + t; a longer one takes over what it held."""
+        need = pos0 + t
+        if pos0 == 0:
+            self.kv[li] = kv_cache.Fp8Cache.empty(b, -(-need // 64) * 64 + 64, self.kv_heads, self.device)
+        cache = self.kv[li]
+        if not isinstance(cache, kv_cache.Fp8Cache) or cache.room < pos0:
+            raise RuntimeError(f"the cache of layer {li} does not hold the {pos0} positions in front of the new ones")
+        if cache.room < need:
+            cache = self.kv[li] = cache.grown(-(-(need + min(256, max(64, need // 8))) // 64) * 64)
+        return cache
+
     def _gate_up(self, L: _Layer, pa: ops.PackedMatrix, like: int) -> ops.PackedMatrix:
         """down_proj's packed input: gate_up, SiLU(gate) * up, rotation, quantisation.  Batches on the GEMM (more than 16
         rows in the whole pass, `like`, however few of them are left in `pa`) get the activation from the product's own
@@ -420,7 +447,7 @@ class ResQForwardB200:
         layer's attention nothing reads the other rows, and o_proj, norms and the MLP work row by row."""
         delta, c, chunk = None, self.cfg, {}
         b, t, _ = h.shape
-        native = (self.ctx.size == 1 and c.head_dim == 128 and self.kv_quant != "fake" and 0 < b * t <= NATIVE_LAYER_ROWS
+        native = (self.ctx.size == 1 and c.head_dim == 128 and self.kv_quant in (False, True) and 0 < b * t <= NATIVE_LAYER_ROWS
                   and (t == 1 or pos0 == 0 or t * (pos0 + t) <= CHUNK_MASK_ELEMENTS)
                   and h.dtype == torch.bfloat16 and h.is_contiguous())
         if native:
@@ -511,8 +538,8 @@ class ResQForwardB200:
         self.pos = pos0 + input_ids.shape[1]
         if not all_positions and isinstance(delta, torch.Tensor):
             h, delta = h[:, -1:], delta[:, -1:]
-        h = self._finish(h, delta)
-        return self._logits(h if all_positions else h[:, -1])
+        logits = self._head(h, delta)
+        return logits if all_positions else logits[:, -1]
 
     def _prefill_scattered(self, input_ids: torch.Tensor, all_positions: bool) -> torch.Tensor:
         """Prefill with the residual stream sharded by rows (sequence-parallel between the linears).  Rank r keeps
@@ -548,8 +575,18 @@ class ResQForwardB200:
             return self._logits(full.view(b, t, -1))
         return self._logits(gather_last_positions(h, b, t, self.ctx.rank, self.ctx.size, self.ctx.group))
 
+    def _head(self, h: torch.Tensor, delta) -> torch.Tensor:
+        """Logits of the rows of a residual stream whose last MLP output has not been added to it yet."""
+        if self.head8 is not None and isinstance(delta, torch.Tensor) and h.dtype == torch.bfloat16:
+            _, p = ops.add_rmsnorm_fp8_pack(delta, h, self.final_norm, self.cfg.rms_eps)
+            return self.head8(p, out_dtype=torch.float32).view(*h.shape[:-1], -1)
+        return self._logits(self._finish(h, delta))
+
     def _logits(self, h_last: torch.Tensor) -> torch.Tensor:
-        """Final norm + unquantised LM head in the model dtype, for rows [..., hidden] (inference/forward_pass.py:178-181 in the reference)."""
+        """Final norm + LM head for rows [..., hidden]: in the model dtype (inference/forward_pass.py:178-181 in the reference)
+        or, with `fp8_head`, in E4M3."""
+        if self.head8 is not None:
+            return self.head8(h_last, norm_weight=self.final_norm, eps=self.cfg.rms_eps, out_dtype=torch.float32)
         last = rms_norm(h_last, self.final_norm, self.cfg.rms_eps)
         return F.linear(last, self.lm_head).float()
 
@@ -584,7 +621,11 @@ class ResQForwardB200:
             S = _DecodeState()
             S.st = {"k": [], "v": [], "pos": torch.zeros(1, dtype=torch.int64, device=dev),
                     "mask": torch.zeros(1, 1, 1, t_max, dtype=nxt_dtype, device=dev)}      # additive: 0 / -inf
+            S.st["cache"] = []
             for li in range(len(self.layers)):
+                if self.kv_quant == "fp8":
+                    S.st["cache"].append(kv_cache.Fp8Cache.empty(b, t_max, self.kv_heads, dev))
+                    continue
                 for name, src in (("k", self.kv[li][0]), ("v", self.kv[li][1])):    # bf16 rows or packed rows
                     S.st[name].append(torch.zeros(b, t_max, self.kv_heads, src.shape[-1], dtype=src.dtype, device=dev))
             S.tok = torch.zeros_like(nxt)                                    # [B, 1] current token, updated in place
@@ -596,6 +637,9 @@ class ResQForwardB200:
             self._decode_states[(b, t0, steps)] = S
         st, tok, out, step_idx = S.st, S.tok, S.out, S.step_idx
         for li in range(len(self.layers)):
+            if self.kv_quant == "fp8":
+                st["cache"][li].copy_from(self.kv[li], t0)
+                continue
             st["k"][li][:, :t0].copy_(self.kv[li][0])
             st["v"][li][:, :t0].copy_(self.kv[li][1])
         self.kv = [None] * len(self.layers)
@@ -605,11 +649,12 @@ class ResQForwardB200:
 
         def decode_step():
             out.index_copy_(1, step_idx, tok)
-            st["mask"].copy_(torch.where(S.arange <= st["pos"], 0.0, float("-inf")).view(1, 1, 1, t_max))
+            if self.kv_quant != "fp8":
+                st["mask"].copy_(torch.where(S.arange <= st["pos"], 0.0, float("-inf")).view(1, 1, 1, t_max))
             h = F.embedding(tok, self.embed)
             cos_sin = self._rope_angles(st["pos"].to(torch.float32))
             h, delta = self._run_layers(h, 0, cos_sin, static=st)
-            tok.copy_(self._logits(self._finish(h, delta)[:, -1]).argmax(-1, keepdim=True))
+            tok.copy_(self._head(h, delta)[:, -1].argmax(-1, keepdim=True))
             st["pos"].add_(1)
             step_idx.add_(1)
 

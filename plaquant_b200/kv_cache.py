@@ -1,4 +1,4 @@
-"""NVFP4 / MXFP8 key and value cache on top of the quantise-and-pack kernel.
+"""Key and value caches: packed NVFP4 rows on top of the quantise-and-pack kernel, and E4M3 with block scales (Fp8Cache).
 
 The reference quantises keys after RoPE: Hadamard over the head dimension, then its activation quantiser on
 per-head rows `k.view(-1, head_dim)` with the last `high_bits_length` channels of every head in the
@@ -122,14 +122,22 @@ class Fp8Cache:
             if c.device != device or s.device != device:
                 raise RuntimeError(f"cache.{name} is on {c.device}, the call on {device}")
 
+    def clone(self) -> "Fp8Cache":
+        return Fp8Cache(self.k.clone(), self.k_scale.clone(), self.v.clone(), self.v_scale.clone())
+
     def grown(self, room: int) -> "Fp8Cache":
-        """A cache with room for `room` positions that holds what this one does."""
+        """A cache with room for `room` positions (at least this one's) that holds what this one does."""
         new = Fp8Cache.empty(self.batch, room, self.kv_heads, self.k.device)
-        for old, dst in ((self.k, new.k), (self.v, new.v)):
-            dst[:, : self.room].copy_(old)
-        for old, dst in ((self.k_scale, new.k_scale), (self.v_scale, new.v_scale)):
-            dst[..., : old.shape[-1]].copy_(old)
+        new.copy_from(self, self.room)
         return new
+
+    def copy_from(self, other: "Fp8Cache", t: int) -> None:
+        """Takes over the first `t` positions of another cache."""
+        blocks = -(-t // CACHE_BLOCK)
+        for dst, src in ((self.k, other.k), (self.v, other.v)):
+            dst[:, :t].copy_(src[:, :t])
+        for dst, src in ((self.k_scale, other.k_scale), (self.v_scale, other.v_scale)):
+            dst[..., :blocks].copy_(src[..., :blocks])
 
     def values(self, t: int):
         """bf16 keys and values [B, t, kv_heads, 128] of the first `t` positions."""

@@ -155,3 +155,64 @@ class QuantizedLinear:
             raise NotImplementedError(f"gemm_impl {impl!r}: plaquant_b200 only has the sm_100a CUDA path ('b200'), "
                                       "no PyTorch or CUTLASS fallback")
         self.gemm_impl = impl
+
+
+class Fp8Linear:
+    """A linear layer in E4M3: weights with a scale per 128 x 128 block, activations with one per row and 128 columns, float32
+    sums.  For layers that do not stand four bits - the LM head of the decoder - and checkpoints in this form.
+
+        codes    uint8 [N, K]                            E4M3, K a multiple of 16
+        scales   float32 [ceil(N / 128), ceil(K / 128)]
+    """
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] % 16 or codes.shape[1] == 0:
+            raise ValueError(f"codes must be uint8 [N, K] with K a multiple of 16, they are {codes.dtype} {list(codes.shape)}")
+        want = (-(-codes.shape[0] // ops.FP8_BLOCK), -(-codes.shape[1] // ops.FP8_BLOCK))
+        if scales.dtype != torch.float32 or tuple(scales.shape) != want:
+            raise ValueError(f"scales must be float32 {list(want)}, they are {scales.dtype} {list(scales.shape)}")
+        self.weight = ops.Fp8Matrix(codes.contiguous(), scales.contiguous(), ops.FP8_BLOCK)
+        self._settle()
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor) -> "Fp8Linear":
+        """Round-to-nearest quantisation of W[N, K] (bf16, CUDA) on the device."""
+        p = ops.fp8_pack_weight(weight)
+        return cls(p.codes, p.scales)
+
+    def _settle(self) -> None:
+        # forward() declares the weights static: what produced them must be complete by now
+        if self.weight.codes.is_cuda:
+            torch.cuda.current_stream(self.weight.device).synchronize()
+
+    @property
+    def out_features(self) -> int:
+        return self.weight.rows
+
+    @property
+    def in_features(self) -> int:
+        return self.weight.k
+
+    def to(self, device) -> "Fp8Linear":
+        w = self.weight
+        self.weight = ops.Fp8Matrix(w.codes.to(device), w.scales.to(device), ops.FP8_BLOCK)
+        self._settle()
+        return self
+
+    def quantize_input(self, x: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> ops.Fp8Matrix:
+        """[RMSNorm] -> E4M3 of x[..., K]."""
+        return ops.fp8_pack(x, gamma=norm_weight, eps=eps)
+
+    def forward(self, x, norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, out: Optional[torch.Tensor] = None,
+                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """x: bf16 [..., K], or an ops.Fp8Matrix.  `norm_weight` fuses the preceding RMSNorm.  `out`: bf16 or float32 [rows, N]
+        to write to; otherwise the result is `out_dtype`."""
+        if not self.weight.codes.is_cuda:
+            raise RuntimeError("Fp8Linear weights are not on a CUDA device; call .to('cuda') (no CPU path)")
+        if isinstance(x, ops.Fp8Matrix):
+            p, lead = x, (x.rows,)
+        else:
+            p, lead = self.quantize_input(x, norm_weight, eps), x.shape[:-1]
+        return ops.fp8_gemm(p, self.weight, out=out, out_dtype=out_dtype, static_weights=True).view(*lead, self.out_features)
+
+    __call__ = forward
