@@ -34,6 +34,7 @@ struct Fp8GemmArgs {
   int band;                    // row tiles per band of the tile order
 };
 struct Fp8GemmMaps { CUtensorMap a, w; };
+constexpr int kMaxSlices = 8;                          // CTAs that may share a tile along K
 
 template <typename T> __device__ __forceinline__ T round_out(float v);
 template <> __device__ __forceinline__ float round_out<float>(float v) { return v; }
@@ -47,17 +48,15 @@ template <> __device__ __forceinline__ __nv_bfloat16 round_out<__nv_bfloat16>(fl
 //   warp 0 producer, warp 1 MMA issuer, warps 2 - 5 epilogue (one weight row per thread)
 template <int MR>
 struct GvCfg {
-  static constexpr int kStages = MR == 64 ? 3 : MR == 32 ? 4 : 5;
+  static constexpr int kStages = 5;
   static constexpr int kXBytes = MR * kStageKBytes;
   static constexpr int kStageBytes = kABytes + kXBytes;
-  static constexpr int kAcc = MR == 64 ? 4 : 8;                       // accumulators in flight
-  static constexpr int kTmemCols = MR == 16 ? 128 : 256;              // two CTAs share an SM
-  static constexpr int kMaxSlices = 8;
+  static constexpr int kAcc = 8;                                      // accumulators in flight
+  static constexpr int kTmemCols = kAcc * MR;                         // two CTAs share an SM
   static constexpr int kSlotRows = MR + kMaxSlices;                   // S slices x ceil(MR / S) rows
   static constexpr int kSlotBytes = kSlotRows * 128 * 4;
   static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kSlotBytes + 4 * MR * 4 + 512;
   static constexpr int kThreads = 192;
-  static_assert(kAcc * MR <= kTmemCols, "tensor memory budget");
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
 
@@ -242,7 +241,7 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
       for (int j = slice, at = 0; j < rows; j += nslice, ++at) {
         float sum = 0.0f;
 #pragma unroll
-        for (int s = 0; s < C::kMaxSlices; ++s)
+        for (int s = 0; s < kMaxSlices; ++s)
           if (s < nslice) sum += slots[(s * per + at) * 128 + trow];
         y[j * g.ldy] = round_out<OUT>(sum);
       }
@@ -289,6 +288,35 @@ __device__ __forceinline__ void fp8_tile(int tile, const Fp8GemmArgs& g, int& tm
   tm = b * g.band + (r - tn * rows);
 }
 
+// 16 neighbouring columns of a row
+template <typename OUT>
+__device__ __forceinline__ void store16(const Fp8GemmArgs& g, int row, int col, const float2* s) {
+  OUT* y = static_cast<OUT*>(g.y) + row * g.ldy;
+  if (g.vec && col + 16 <= g.n) {
+    if constexpr (sizeof(OUT) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) __stcs(reinterpret_cast<float4*>(y + col) + i, make_float4(s[2 * i].x, s[2 * i].y, s[2 * i + 1].x, s[2 * i + 1].y));
+    } else {
+      uint32_t d[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d[i] = f32x2_to_bf16x2(s[i].x, s[i].y);
+      if (g.vec == 2) {
+        asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(y + col), "r"(d[0]), "r"(d[1]), "r"(d[2]), "r"(d[3]),
+                     "r"(d[4]), "r"(d[5]), "r"(d[6]), "r"(d[7]) : "memory");
+      } else {
+        __stcs(reinterpret_cast<uint4*>(y + col), make_uint4(d[0], d[1], d[2], d[3]));
+        __stcs(reinterpret_cast<uint4*>(y + col + 8), make_uint4(d[4], d[5], d[6], d[7]));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (col + 2 * i < g.n) y[col + 2 * i] = round_out<OUT>(s[i].x);
+      if (col + 2 * i + 1 < g.n) y[col + 2 * i + 1] = round_out<OUT>(s[i].y);
+    }
+  }
+}
+
 template <int BN, int CG, typename OUT>
 __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(const __grid_constant__ Fp8GemmMaps maps, const Fp8GemmArgs g) {
   using C = GmCfg<BN, CG>;
@@ -330,10 +358,15 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
   pdl_launch_dependents();
 
   const int num_tiles = g.tiles_m * g.tiles_n;
-  const int first = CG == 2 ? static_cast<int>(cluster_id_x()) : static_cast<int>(blockIdx.x);
-  const int step = CG == 2 ? static_cast<int>(nclusters_x()) : static_cast<int>(gridDim.x);
+  const int first = static_cast<int>(cluster_id_x()), step = static_cast<int>(nclusters_x());
+  // without a pair the CTAs of a cluster share a tile along K
+  uint32_t cluster_size;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(cluster_size));
+  const int slices = CG == 2 ? 1 : static_cast<int>(cluster_size), slice = CG == 2 ? 0 : static_cast<int>(cluster_ctarank());
+  const int kb0 = g.kb * slice / slices, kb1 = g.kb * (slice + 1) / slices, kbs = kb1 - kb0;
   const uint32_t smem_base = smem_u32(smem);
 
+  float2 acc[C::kCols / 2];                            // epilogue: 64 columns of this thread's row
   if (warp == 0 || warp == 3) {
     if (elect_one()) {
       pdl_wait();
@@ -344,8 +377,9 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
         int tm, tn;
         fp8_tile(tile, g, tm, tn);
         const int row_a = (tm * CG + static_cast<int>(rank)) * kBM, row_b = tn * BN + static_cast<int>(rank) * C::kBRows;
-        for (int kb = static_cast<int>((gs ^ mine) & 1u); kb < g.kb; kb += 2) {
-          const uint32_t x = gs + kb, slot = x % C::kStages;
+        for (int i = static_cast<int>((gs ^ mine) & 1u); i < kbs; i += 2) {
+          const uint32_t x = gs + i, slot = x % C::kStages;
+          const int kb = kb0 + i;
           ok = mbar_wait_bounded(&empty_bar[slot], ((x / C::kStages) & 1u) ^ 1u, abort_flag);
           if (!ok) break;
           const uint32_t st = smem_base + slot * C::kStageBytes;
@@ -355,7 +389,7 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
           tma_load_2d_cg<CG>(st, &maps.a, kb * kStageKBytes, row_a, bar);
           tma_load_2d_cg<CG>(st + kABytes, &maps.w, kb * kStageKBytes, row_b, bar);
         }
-        gs += g.kb;
+        gs += kbs;
       }
     }
   } else if (warp == 1) {
@@ -373,7 +407,7 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
       uint32_t gs = 0;
       bool ok = true;
       for (int tile = first; ok && tile < num_tiles; tile += step)
-        for (int kb = 0; kb < g.kb; ++kb, ++gs) {
+        for (int kb = kb0; kb < kb1; ++kb, ++gs) {
           const uint32_t slot = gs % C::kStages, as = gs % C::kAcc;
           ok = wait(&acc_empty[as], ((gs / C::kAcc) & 1u) ^ 1u) && wait(&full_bar[slot], (gs / C::kStages) & 1u);
           if (!ok) break;
@@ -399,7 +433,7 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
       for (int i = 0; i < 4; ++i)
         src[i] = g.sa + static_cast<long long>(min((tm * CG + static_cast<int>(rank)) * kBM + lane + 32 * i, g.m - 1)) * g.kb;
       const float* sw = g.sw + static_cast<long long>(min(tn * BN + (lane & 1) * 128, g.n - 1) / kFp8Block) * g.kb;
-      for (int kb = 0; kb < g.kb; ++kb, ++gs) {
+      for (int kb = kb0; kb < kb1; ++kb, ++gs) {
         const uint32_t slot = gs % C::kSfSlots;
         ok = mbar_wait_bounded_lanes(&sf_empty[slot], ((gs / C::kSfSlots) & 1u) ^ 1u, abort_flag);
         if (!ok) break;
@@ -422,10 +456,9 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
       fp8_tile(tile, g, tm, tn);
       const int row = (tm * CG + static_cast<int>(rank)) * kBM + quad * 32 + lane;
       const int col0 = tn * BN + cgp * C::kCols;
-      float2 acc[C::kCols / 2];
 #pragma unroll
       for (int j = 0; j < C::kCols / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
-      for (int kb = 0; kb < g.kb; ++kb, ++gs) {
+      for (int kb = kb0; kb < kb1; ++kb, ++gs) {
         const uint32_t as = gs % C::kAcc, slot = gs % C::kSfSlots;
         ok = mbar_wait_bounded_lanes(&sf_full[slot], (gs / C::kSfSlots) & 1u, abort_flag);
         if (!ok) break;
@@ -456,36 +489,53 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
         }
       }
       if (!ok) break;
-      if (row < g.m) {
-        OUT* y = static_cast<OUT*>(g.y) + row * g.ldy;
+      if (slices == 1 && row < g.m) {
 #pragma unroll
-        for (int v = 0; v < C::kCols / 16; ++v) {            // 16 columns at a time
-          const int col = col0 + v * 16;
-          const float2* s = acc + v * 8;
-          if (g.vec && col + 16 <= g.n) {
-            if constexpr (sizeof(OUT) == 4) {
+        for (int v = 0; v < C::kCols / 16; ++v) store16<OUT>(g, row, col0 + v * 16, acc + v * 8);
+      }
+    }
+  }
+  if constexpr (CG == 1) {
+    if (slices > 1) {
+      // One tile per cluster.  Each CTA adds, in the order of the slices, the 16-column groups g with g mod S = its rank; the
+      // others' sums come to it through its ring, which is idle in every CTA behind the first barrier.
+      const int quad = warp & 3, cgp = (warp - 4) >> 2, trow = quad * 32 + lane, per = (8 + slices - 1) / slices;
+      float* slots = reinterpret_cast<float*>(smem);             // [slice][owned group][16 columns][128 rows]: whole lines per store
+      __syncwarp();
+      cluster_arrive_release();
+      cluster_wait_acquire();
+      if (warp >= 4) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                __stcs(reinterpret_cast<float4*>(y + col) + i, make_float4(s[2 * i].x, s[2 * i].y, s[2 * i + 1].x, s[2 * i + 1].y));
-            } else {
-              uint32_t d[8];
+        for (int v = 0; v < 4; ++v) {
+          const int group = cgp * 4 + v, owner = group % slices;
+          const uint32_t dst = map_to_cta(smem_u32(slots + (slice * per + group / slices) * 2048 + trow), static_cast<uint32_t>(owner));
 #pragma unroll
-              for (int i = 0; i < 8; ++i) d[i] = f32x2_to_bf16x2(s[i].x, s[i].y);
-              if (g.vec == 2)
-                asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(y + col), "r"(d[0]), "r"(d[1]), "r"(d[2]),
-                             "r"(d[3]), "r"(d[4]), "r"(d[5]), "r"(d[6]), "r"(d[7]) : "memory");
-              else {
-                __stcs(reinterpret_cast<uint4*>(y + col), make_uint4(d[0], d[1], d[2], d[3]));
-                __stcs(reinterpret_cast<uint4*>(y + col + 8), make_uint4(d[4], d[5], d[6], d[7]));
-              }
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (col + 2 * i < g.n) y[col + 2 * i] = round_out<OUT>(s[i].x);
-              if (col + 2 * i + 1 < g.n) y[col + 2 * i + 1] = round_out<OUT>(s[i].y);
-            }
+          for (int i = 0; i < 8; ++i) {
+            const float2 x = acc[v * 8 + i];
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 1024 * i), "f"(x.x) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 1024 * i + 512), "f"(x.y) : "memory");
           }
+        }
+      }
+      __syncwarp();
+      cluster_arrive_release();
+      cluster_wait_acquire();
+      if (warp >= 4 && !*abort_flag) {
+        int tm, tn;
+        fp8_tile(first, g, tm, tn);
+        const int row = tm * kBM + trow;
+        for (int at = cgp; at < per; at += 2) {
+          const int group = at * slices + slice;
+          if (group >= 8) break;
+          float2 sum[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[i] = make_float2(0.0f, 0.0f);
+          for (int sl = 0; sl < slices; ++sl) {
+            const float* src = slots + (sl * per + at) * 2048 + trow;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] = make_float2(sum[i].x + src[256 * i], sum[i].y + src[256 * i + 128]);
+          }
+          if (row < g.m) store16<OUT>(g, row, tn * BN + group * 16, sum);
         }
       }
     }
@@ -545,20 +595,18 @@ static int launch_clusters(K kernel, unsigned grid, unsigned cluster, unsigned t
 
 struct Fp8Ptrs { const void *a, *w; int64_t k; };
 
-// Clusters of `slices` CTAs that the device holds at once; looked up once per thread and device.
-template <int MR, typename OUT>
-static int gemv_clusters(int slices) {
-  using C = GvCfg<MR>;
-  static thread_local int cached_dev = -1;
-  static thread_local int table[C::kMaxSlices + 1];
+// How many clusters of 1 .. kMaxSlices CTAs of a kernel the device holds at once; looked up once per thread and device.
+struct ClusterTable { int dev = -1, n[kMaxSlices + 1]; };
+template <typename K>
+static int clusters_at_once(K kernel, unsigned threads, size_t smem, int slices, ClusterTable* t) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (cached_dev != dev) {
-    for (int s = 1; s <= C::kMaxSlices; ++s) {
+  if (t->dev != dev) {
+    for (int s = 1; s <= kMaxSlices; ++s) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(static_cast<unsigned>(s * 64), 1, 1);
-      cfg.blockDim = dim3(C::kThreads, 1, 1);
-      cfg.dynamicSmemBytes = C::kSmemBytes;
+      cfg.blockDim = dim3(threads, 1, 1);
+      cfg.dynamicSmemBytes = smem;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
       attr[0].val.clusterDim.x = static_cast<unsigned>(s);
@@ -567,13 +615,23 @@ static int gemv_clusters(int slices) {
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, fp8_gemv_kernel<MR, OUT>, &cfg) != cudaSuccess) n = 0;
-      table[s] = n;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+      t->n[s] = n;
     }
     (void)cudaGetLastError();
-    cached_dev = dev;
+    t->dev = dev;
   }
-  return table[slices];
+  return t->n[slices];
+}
+
+// CTAs per tile: as many as keep all clusters on the device at once, none with fewer than `least` K blocks.
+template <typename K>
+static int k_slices(K kernel, unsigned threads, size_t smem, int64_t tiles, int64_t slots, int kb, int least, ClusterTable* t) {
+  int64_t s = slots / tiles;
+  if (s > kMaxSlices) s = kMaxSlices;
+  if (s > kb / least) s = kb / least;
+  while (s > 1 && clusters_at_once(kernel, threads, smem, static_cast<int>(s), t) < tiles) --s;
+  return s > 1 ? static_cast<int>(s) : 1;
 }
 
 template <int MR, typename OUT>
@@ -590,11 +648,8 @@ static int launch_gemv(const Fp8Ptrs& p, Fp8GemmArgs& g, void* stream) {
   g.tiles_n = (g.n + kBM - 1) / kBM;
   g.tiles_m = (g.m + MR - 1) / MR;
   const int slots = 2 * sm_count(), tiles = g.tiles_n * g.tiles_m;
-  int slices = slots / tiles;
-  if (slices > C::kMaxSlices) slices = C::kMaxSlices;
-  if (slices > g.kb) slices = g.kb;
-  while (slices > 1 && gemv_clusters<MR, OUT>(slices) < tiles) --slices;       // all at once
-  if (slices < 1) slices = 1;
+  static thread_local ClusterTable table;
+  const int slices = k_slices(kernel, C::kThreads, C::kSmemBytes, tiles, slots, g.kb, 1, &table);
   const int grid = slices > 1 ? tiles * slices : (tiles < slots ? tiles : slots);
   return launch_clusters(kernel, static_cast<unsigned>(grid), static_cast<unsigned>(slices), C::kThreads, C::kSmemBytes, stream, tm, g);
 }
@@ -617,21 +672,31 @@ static int launch_gemm_fp8(const Fp8Ptrs& p, Fp8GemmArgs& g, void* stream) {
   g.band = a_bytes > w_bytes && a_bytes > (32ll << 20) ? 4 : g.tiles_m;
   if (g.band > g.tiles_m) g.band = g.tiles_m;
   const int slots = sm_count() / CG, tiles = g.tiles_m * g.tiles_n;
+  if constexpr (CG == 1) {
+    static thread_local ClusterTable table;
+    const int slices = k_slices(kernel, C::kThreads, C::kSmemBytes, tiles, slots, g.kb, 4, &table);
+    if (slices > 1) return launch_clusters(kernel, static_cast<unsigned>(tiles * slices), static_cast<unsigned>(slices), C::kThreads, C::kSmemBytes, stream, tm, g);
+  }
   return launch_clusters(kernel, static_cast<unsigned>((tiles < slots ? tiles : slots) * CG), CG, C::kThreads, C::kSmemBytes, stream, tm, g);
 }
 
 template <typename OUT>
 static int launch_fp8(const Fp8Ptrs& p, Fp8GemmArgs& g, int variant, void* stream) {
   if (variant == PLQ_FP8_AUTO) {
-    const int64_t sms = sm_count(), pairs = sms / 2 > 0 ? sms / 2 : 1;
-    const int64_t wide = (g.m + 255ll) / 256 * ((g.n + 255ll) / 256), small = (g.m + 127ll) / 128 * ((g.n + 127ll) / 128);
-    if (g.m <= 64) variant = PLQ_FP8_ROWS;
-    else variant = (wide + pairs - 1) / pairs * 2 <= (small + sms - 1) / sms ? PLQ_FP8_PAIR_256x256 : PLQ_FP8_128x128;
+    // Up to 16 rows the weights' bytes count.  Above, the shape with the smallest waves x time of a wave; per K block of a wave,
+    // measured at 1024 x 8192 x 8192 and 8192 x 4096 x 14336: 128 x 128 0.34 us (the feed from L2: 14 TB/s), 256 x 128 of a pair
+    // 0.32, 256 x 256 0.60.  Tiles that leave half of the SMs idle are split along K instead (128 x 128): 128 x 4096 x 8192
+    // 22.2 -> 11.9 us, 77 x 6144 x 4096 12.8 -> 10.6.
+    const int64_t sms = sm_count(), pairs = sms / 2 > 0 ? sms / 2 : 1, mt = (g.m + 127ll) / 128, nt = (g.n + 127ll) / 128;
+    const auto waves = [](int64_t tiles, int64_t slots) { return (tiles + slots - 1) / slots; };
+    const int64_t small = waves(mt * nt, sms) * 34, wide = waves((mt + 1) / 2 * nt, pairs) * 32, square = waves((mt + 1) / 2 * ((nt + 1) / 2), pairs) * 60;
+    if (g.m <= 16) variant = PLQ_FP8_ROWS;
+    else if (2 * mt * nt <= sms) variant = PLQ_FP8_128x128;
+    else variant = square <= wide && square <= small ? PLQ_FP8_PAIR_256x256 : wide <= small && mt > 1 ? PLQ_FP8_PAIR_256x128 : PLQ_FP8_128x128;
   }
   if (variant == PLQ_FP8_ROWS) {
-    if (g.m > 1024) return PLQ_ERR_SHAPE;
-    if (g.m <= 16) return launch_gemv<16, OUT>(p, g, stream);
-    return g.m <= 32 ? launch_gemv<32, OUT>(p, g, stream) : launch_gemv<64, OUT>(p, g, stream);
+    if (g.m > 64) return PLQ_ERR_SHAPE;
+    return launch_gemv<16, OUT>(p, g, stream);
   }
   if (variant == PLQ_FP8_128x128) return launch_gemm_fp8<128, 1, OUT>(p, g, stream);
   if (variant == PLQ_FP8_PAIR_256x256) return launch_gemm_fp8<256, 2, OUT>(p, g, stream);

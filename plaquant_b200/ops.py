@@ -545,14 +545,14 @@ def fp8_unpack(p: Fp8Matrix) -> torch.Tensor:
     return y
 
 
-FP8_GEMM_VARIANTS = {None: 0, "auto": 0, "rows": 1, "128x128": 2, "pair256x256": 3}
+FP8_GEMM_VARIANTS = {None: 0, "auto": 0, "rows": 1, "128x128": 2, "pair256x256": 3, "pair256x128": 4}
 
 
 def fp8_gemm(a: Fp8Matrix, w: Fp8Matrix, out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16,
              static_weights: bool = False, variant: Optional[str] = None) -> torch.Tensor:
     """y[m, n] = deq(a) @ deq(w).T, float32 sums, bf16 or float32 (`out_dtype`, or that of `out`).  `static_weights`: w was
     complete long before this call, so that its first bytes may be fetched while the previous kernel of the stream drains.
-    `variant` picks the kernel ("rows" for up to 64 rows, "128x128", "pair256x256"); default: by the sizes."""
+    `variant` picks the kernel ("rows" for up to 64 rows, "128x128", "pair256x256", "pair256x128"); default: by the sizes."""
     flags = int(static_weights) | FP8_GEMM_VARIANTS[variant] << 4
     if out is None and (out_dtype is torch.bfloat16 or out_dtype is torch.float32):
         word = _status_words.get(a.codes.get_device())

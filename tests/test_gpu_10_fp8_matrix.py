@@ -149,11 +149,13 @@ def test_product_of_a_few_rows(plq, m, n, k):
     a, w = _operands(m, n, k, 10 * m + n)
     for dtype in (torch.bfloat16, torch.float32):
         _check_product(plq.ops.fp8_gemm(a, w, out_dtype=dtype), a, w)
+        _check_product(plq.ops.fp8_gemm(a, w, out_dtype=dtype, variant="rows"), a, w)
     plq.check_device_status()
 
 
-@pytest.mark.parametrize("variant", ["128x128", "pair256x256"])
-@pytest.mark.parametrize("m,n,k", [(1, 1, 16), (65, 100, 128), (128, 128, 400), (129, 257, 1040), (300, 1001, 2064), (513, 768, 1024), (256, 5000, 272)])
+@pytest.mark.parametrize("variant", ["128x128", "pair256x256", "pair256x128"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 16), (65, 100, 128), (128, 128, 400), (129, 257, 1040), (300, 1001, 2064), (513, 768, 1024), (256, 5000, 272),
+                                   (20, 300, 4112), (130, 1500, 8192)])
 def test_product_of_many_rows(plq, variant, m, n, k):
     a, w = _operands(m, n, k, m + n)
     for dtype in (torch.bfloat16, torch.float32):
