@@ -23,7 +23,7 @@ struct Fp8AppendArgs {
   float* scales[2];
   const long long* pos_dev;    // first new position, one for all sequences (pos_batch = 0) or one each; or nullptr
   long long pos, t_max, ld8, cs_batch;
-  long long q_threads;         // batch * t * heads * 8
+  long long q_threads;         // batch * t * heads * 8 / HT
   int* status;
   int t, heads, kv_heads, pos_batch, units_per_head;
   int scale_blocks;            // ceil(t_max / 64)
@@ -36,20 +36,20 @@ __device__ __forceinline__ float cache_scale(uint32_t bits) {
   return __uint_as_float(static_cast<uint32_t>(max(e, 127 - 100)) << 23);
 }
 
-// RoPE of four elements of a head: (2 l, 2 l + 1) and (64 + 2 l, 65 + 2 l) of lane l; every operation rounded on its own, then to
+// RoPE of two elements of a head's first half (x) and the two 64 behind them (y); every operation rounded on its own, then to
 // bf16, as rope_kv_append_kernel does it.
-__device__ __forceinline__ uint2 rope4(uint2 w, const float* cos, const float* sin, int lane) {
-  const float2 c1 = *reinterpret_cast<const float2*>(cos + 2 * lane), c2 = *reinterpret_cast<const float2*>(cos + 64 + 2 * lane);
-  const float2 s1 = *reinterpret_cast<const float2*>(sin + 2 * lane), s2 = *reinterpret_cast<const float2*>(sin + 64 + 2 * lane);
+__device__ __forceinline__ uint2 rope4(uint2 w, float2 c1, float2 c2, float2 s1, float2 s2) {
   const float ax = bf16lo_to_f32(w.x), ay = bf16hi_to_f32(w.x), bx = bf16lo_to_f32(w.y), by = bf16hi_to_f32(w.y);
   return make_uint2(f32x2_to_bf16x2(__fadd_rn(__fmul_rn(ax, c1.x), __fmul_rn(-bx, s1.x)), __fadd_rn(__fmul_rn(ay, c1.y), __fmul_rn(-by, s1.y))),
                     f32x2_to_bf16x2(__fadd_rn(__fmul_rn(bx, c2.x), __fmul_rn(ax, s2.x)), __fadd_rn(__fmul_rn(by, c2.y), __fmul_rn(ay, s2.y))));
 }
 
-// One launch: the first q_blocks blocks rotate the queries (eight threads per head, 16 elements each), every other block
+// One launch: the first q_blocks blocks rotate the queries (eight threads per head, 16 elements each of HT neighbouring heads:
+// the angles are four times the bytes of a head's elements and come from L1 once per thread), every other block
 // quantises one (sequence, head, keys or values, 64-token block) of the new rows, a warp per row and up to eight rows per
 // warp.  Bound by the bytes of the projection (read once) and of the outputs; a decode step by its launch and the chain
 // load -> maximum -> scale -> store.
+template <int HT>
 __global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8AppendArgs a) {
   __shared__ uint32_t warp_top[8];
   pdl_launch_dependents();
@@ -57,24 +57,38 @@ __global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8Append
   if (blockIdx.x < a.q_blocks) {
     const long long idx = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (idx >= a.q_threads) return;
-    const int j = static_cast<int>(idx & 7);
-    const long long hr = idx >> 3, row = hr / a.heads, b = row / a.t;
-    const int head = static_cast<int>(hr - row * a.heads), tt = static_cast<int>(row - b * a.t);
+    const int j = static_cast<int>(idx & 7), groups = a.heads / HT;
+    const long long hr = idx >> 3, row = hr / groups, b = row / a.t;
+    const int head = static_cast<int>(hr - row * groups) * HT, tt = static_cast<int>(row - b * a.t);
     const uint4* src = a.qkv + row * a.ld8 + head * 16 + j;
-    const uint4 lo = src[0], hi = src[8];
+    uint4 lo[HT], hi[HT];
+#pragma unroll
+    for (int x = 0; x < HT; ++x) { lo[x] = src[16 * x]; hi[x] = src[16 * x + 8]; }
     const float* cos = a.cos + b * a.cs_batch + static_cast<long long>(tt) * kHeadDim + 8 * j;
     const float* sin = a.sin + b * a.cs_batch + static_cast<long long>(tt) * kHeadDim + 8 * j;
-    const uint32_t lw[4] = {lo.x, lo.y, lo.z, lo.w}, hw[4] = {hi.x, hi.y, hi.z, hi.w};
-    uint32_t ol[4], oh[4];
+    uint4* dst = a.q_out + (row * a.heads + head) * 16 + j;
+    float c1[8], c2[8], s1[8], s2[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint2 o = rope4(make_uint2(lw[i], hw[i]), cos, sin, i);
-      ol[i] = o.x;
-      oh[i] = o.y;
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<float4*>(c1 + 4 * i) = *reinterpret_cast<const float4*>(cos + 4 * i);
+      *reinterpret_cast<float4*>(c2 + 4 * i) = *reinterpret_cast<const float4*>(cos + 64 + 4 * i);
+      *reinterpret_cast<float4*>(s1 + 4 * i) = *reinterpret_cast<const float4*>(sin + 4 * i);
+      *reinterpret_cast<float4*>(s2 + 4 * i) = *reinterpret_cast<const float4*>(sin + 64 + 4 * i);
     }
-    uint4* dst = a.q_out + hr * 16 + j;
-    dst[0] = make_uint4(ol[0], ol[1], ol[2], ol[3]);
-    dst[8] = make_uint4(oh[0], oh[1], oh[2], oh[3]);
+#pragma unroll
+    for (int x = 0; x < HT; ++x) {
+      uint32_t* lw = reinterpret_cast<uint32_t*>(&lo[x]);
+      uint32_t* hw = reinterpret_cast<uint32_t*>(&hi[x]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint2 o = rope4(make_uint2(lw[i], hw[i]), make_float2(c1[2 * i], c1[2 * i + 1]), make_float2(c2[2 * i], c2[2 * i + 1]),
+                              make_float2(s1[2 * i], s1[2 * i + 1]), make_float2(s2[2 * i], s2[2 * i + 1]));
+        lw[i] = o.x;
+        hw[i] = o.y;
+      }
+      dst[16 * x] = lo[x];
+      dst[16 * x + 8] = hi[x];
+    }
     return;
   }
   const unsigned unit = blockIdx.x - a.q_blocks;
@@ -107,7 +121,11 @@ __global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8Append
       const long long tt = start - pos + r;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(a.qkv + (b * a.t + tt) * a.ld8 + head * 16) + lane;
       w[i] = make_uint2(src[0], src[32]);
-      if (!side) w[i] = rope4(w[i], a.cos + b * a.cs_batch + tt * kHeadDim, a.sin + b * a.cs_batch + tt * kHeadDim, lane);
+      if (!side) {
+        const float2* cos = reinterpret_cast<const float2*>(a.cos + b * a.cs_batch + tt * kHeadDim) + lane;
+        const float2* sin = reinterpret_cast<const float2*>(a.sin + b * a.cs_batch + tt * kHeadDim) + lane;
+        w[i] = rope4(w[i], cos[0], cos[32], sin[0], sin[32]);
+      }
     }
   }
 #pragma unroll
@@ -748,6 +766,10 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
   const long long base = (unit * a.runs + r0) * 2 * rows_per_tile + (row - rt * rows_per_tile);
   const int late = r0 * length < before ? rows_per_tile : 0;
   auto slot = [&](int x) { return base + (x == 0 ? late : static_cast<long long>(x) * 2 * rows_per_tile); };
+  float4 ahead[4];                                     // the warp's first sums, on their way beside the runs' maxima
+#pragma unroll
+  for (int y = 0; y < 4; ++y)
+    ahead[y] = warp + 4 * y < n ? *reinterpret_cast<const float4*>(a.part + slot(warp + 4 * y) * kHeadDim + 4 * lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float top = kNegInf;
   for (int x = lane; x < n; x += 32) {
     const float2 s = stat[slot(x)];
@@ -756,15 +778,16 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
   top = warp_max(top);
   float weight = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-  for (int x = warp; x < n; x += 4) {                  // a run of which the row sees nothing left zeros
-    const long long sl = slot(x);
-    const float2 s = stat[sl];
-    const float4 v = *reinterpret_cast<const float4*>(a.part + sl * kHeadDim + 4 * lane);
+  auto add = [&](const float2 s, const float4 v) {     // a run of which the row sees nothing left zeros
     const float w = s.y == 0.0f ? 0.0f : ex2_approx(s.x - top);
     weight = fmaf(s.y, w, weight);
     acc = make_float4(fmaf(v.x, w, acc.x), fmaf(v.y, w, acc.y), fmaf(v.z, w, acc.z), fmaf(v.w, w, acc.w));
-  }
+  };
+#pragma unroll
+  for (int y = 0; y < 4; ++y)
+    if (warp + 4 * y < n) add(stat[slot(warp + 4 * y)], ahead[y]);
+#pragma unroll 4
+  for (int x = warp + 16; x < n; x += 4) add(stat[slot(x)], *reinterpret_cast<const float4*>(a.part + slot(x) * kHeadDim + 4 * lane));
   acc_s[warp][lane] = acc;
   if (lane == 0) weight_s[warp] = weight;
   __syncthreads();
@@ -1233,7 +1256,10 @@ extern "C" int plq_rope_kv_append_fp8(const void* qkv_bf16, int64_t ld, const vo
   a.t_max = t_max;
   a.ld8 = ld / 8;
   a.cs_batch = cs_batch_stride;
-  a.q_threads = batch * t * heads * 8;
+  // several heads per thread where there are enough of them for every SM
+  const int64_t head_rows = batch * t * heads;
+  const int ht = head_rows * 8 < 2 * 2048 * static_cast<int64_t>(sm_count()) ? 1 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+  a.q_threads = head_rows / ht * 8;
   a.status = dev_status;
   a.t = static_cast<int>(t);
   a.heads = static_cast<int>(heads);
@@ -1253,7 +1279,7 @@ extern "C" int plq_rope_kv_append_fp8(const void* qkv_bf16, int64_t ld, const vo
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, rope_kv_append_fp8_kernel, a));
+  PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, ht == 4 ? rope_kv_append_fp8_kernel<4> : ht == 2 ? rope_kv_append_fp8_kernel<2> : rope_kv_append_fp8_kernel<1>, a));
   return PLQ_OK;
 }
 
