@@ -49,9 +49,6 @@ __device__ __forceinline__ uint32_t e4m3_e5m2_split(float a, float b) {
   asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(lo) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
   return hi | static_cast<uint32_t>(lo) << 16;
 }
-__device__ __forceinline__ uint2 e4m3x8(const float (&y)[8]) {
-  return make_uint2(e4m3x2(y[0], y[1]) | e4m3x2(y[2], y[3]) << 16, e4m3x2(y[4], y[5]) | e4m3x2(y[6], y[7]) << 16);
-}
 
 // Instruction descriptor of kind::f8f6f4 with E4M3 operands and a float32 accumulator:
 //   [4,6) accumulator 1 = float32  [7,10), [10,13) operand formats 0 = E4M3  [15], [16] A, B with M / N contiguous instead of K

@@ -36,6 +36,12 @@ __device__ __forceinline__ float cache_scale(uint32_t bits) {
   return __uint_as_float(static_cast<uint32_t>(max(e, 127 - 100)) << 23);
 }
 
+// 16 bytes that are read once: not kept in L1, where the angles are
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 // RoPE of two elements of a head's first half (x) and the two 64 behind them (y); every operation rounded on its own, then to
 // bf16, as rope_kv_append_kernel does it.
 __device__ __forceinline__ uint2 rope4(uint2 w, float2 c1, float2 c2, float2 s1, float2 s2) {
@@ -63,7 +69,7 @@ __global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8Append
     const uint4* src = a.qkv + row * a.ld8 + head * 16 + j;
     uint4 lo[HT], hi[HT];
 #pragma unroll
-    for (int x = 0; x < HT; ++x) { lo[x] = src[16 * x]; hi[x] = src[16 * x + 8]; }
+    for (int x = 0; x < HT; ++x) { lo[x] = load_once(src + 16 * x); hi[x] = load_once(src + 16 * x + 8); }
     const float* cos = a.cos + b * a.cs_batch + static_cast<long long>(tt) * kHeadDim + 8 * j;
     const float* sin = a.sin + b * a.cs_batch + static_cast<long long>(tt) * kHeadDim + 8 * j;
     uint4* dst = a.q_out + (row * a.heads + head) * 16 + j;

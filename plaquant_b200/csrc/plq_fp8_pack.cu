@@ -28,18 +28,38 @@ struct Fp8PackArgs {
   float inv_k, eps;
 };
 
-__device__ __forceinline__ void widen8(const uint4& q, float (&f)[8]) {
+// eight bf16 -> four pairs of float32
+__device__ __forceinline__ void widen8(const uint4& q, float2 (&f)[4]) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = bf16lo_to_f32(w[i]);
-    f[2 * i + 1] = bf16hi_to_f32(w[i]);
-  }
+  for (int i = 0; i < 4; ++i) f[i] = make_float2(bf16lo_to_f32(w[i]), bf16hi_to_f32(w[i]));
 }
-
-// |y| as an unsigned integer: ordered like the values, with infinity and NaN above all of them
-__device__ __forceinline__ uint32_t abs_bits(float y) { return __float_as_uint(y) & 0x7FFFFFFFu; }
-constexpr uint32_t kInfBits = 0x7F800000u;
+__device__ __forceinline__ uint2 codes8(const float2 (&y)[4]) {
+  return make_uint2(e4m3x2(y[0].x, y[0].y) | e4m3x2(y[1].x, y[1].y) << 16, e4m3x2(y[2].x, y[2].y) | e4m3x2(y[3].x, y[3].y) << 16);
+}
+// the larger of a and |y|; NaN if one of them is
+__device__ __forceinline__ float max_abs(float a, float y) {
+  float r;
+  asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;\n\t}" : "=f"(r) : "f"(a), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float max_abs8(const float2 (&y)[4]) {
+  float a = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) a = max_abs(max_abs(a, y[j].x), y[j].y);
+  return a;
+}
+// What a block's codes are multiplied with, and its scale, from its largest magnitude.
+struct BlockScale {
+  float inv, scale;
+  bool finite;
+  __device__ __forceinline__ explicit BlockScale(float top) {
+    finite = top < __uint_as_float(0x7F800000u);
+    const float amax = fmaxf(top, kFp8Floor);              // a number for a top of NaN as well
+    inv = __fdiv_rn(kE4m3Max, amax);
+    scale = finite ? __fdiv_rn(amax, kE4m3Max) : __uint_as_float(0x7FFFFFFFu);
+  }
+};
 
 // One CTA per row; a thread holds VPT vectors of eight elements, 16 neighbouring lanes hold a block of 128 columns.
 template <int VPT, bool NORM, bool ADD>
@@ -66,26 +86,27 @@ __global__ void __launch_bounds__(512) fp8_pack_kernel(const Fp8PackArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float f[8], g[8];
+      float2 f[4], g[4];
       widen8(v[i], f);
       widen8(w[i], g);
       uint32_t* o = reinterpret_cast<uint32_t*>(&v[i]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = f32x2_to_bf16x2(g[2 * j] + f[2 * j], g[2 * j + 1] + f[2 * j + 1]);
+      for (int j = 0; j < 4; ++j) o[j] = f32x2_to_bf16x2(g[j].x + f[j].x, g[j].y + f[j].y);
       const int at = tid + i * step;
       if (at < a.vecs) a.h_out[row * a.vecs + at] = v[i];
     }
   }
   float r = 1.0f;
   if constexpr (NORM) {
-    float sum = 0.0f;
+    float2 sums = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float f[8];
+      float2 f[4];
       widen8(v[i], f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(f[j], f[j], sum);
+      for (int j = 0; j < 4; ++j) sums = __ffma2_rn(f[j], f[j], sums);
     }
+    float sum = sums.x + sums.y;
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
     if ((tid & 31) == 0) warp_sum[tid >> 5] = sum;
@@ -101,43 +122,41 @@ __global__ void __launch_bounds__(512) fp8_pack_kernel(const Fp8PackArgs a) {
   for (int i = 0; i < VPT; ++i) {
     const int at = tid + i * step;
     if (VPT > 1 && i * step >= a.vecs) break;              // the same for the whole CTA
-    float y[8];
+    float2 y[4];
     widen8(v[i], y);
     if constexpr (NORM) {
       const uint4 gv = at < a.vecs ? a.gamma[at] : make_uint4(0, 0, 0, 0);
-      float g[8];
+      float2 g[4];
       widen8(gv, g);
+      const float2 r2 = make_float2(r, r);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(g[j], __fmul_rn(y[j], r));
+      for (int j = 0; j < 4; ++j) y[j] = __fmul2_rn(g[j], __fmul2_rn(y[j], r2));
     }
-    uint32_t top = 0;
+    float top = max_abs8(y);
+    if (at >= a.vecs) top = 0.0f;                          // 0 * r is NaN where the row is not finite
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, abs_bits(y[j]));
-    if (at >= a.vecs) top = 0;                             // 0 * r is NaN where the row is not finite
+    for (int d = 8; d >= 1; d >>= 1) top = max_abs(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    const BlockScale s(top);
+    const float2 inv = make_float2(s.inv, s.inv);
 #pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    const bool finite = top < kInfBits;
-    const float amax = fmaxf(__uint_as_float(top), kFp8Floor);
-    const float inv = __fdiv_rn(kE4m3Max, amax);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = finite ? __fmul_rn(y[j], inv) : 0.0f;
+    for (int j = 0; j < 4; ++j) y[j] = s.finite ? __fmul2_rn(y[j], inv) : make_float2(0.0f, 0.0f);
     if (at < a.vecs) {
-      a.codes[row * a.vecs + at] = e4m3x8(y);
-      if ((tid & 15) == 0) a.scales[row * a.blocks + (at >> 4)] = finite ? __fdiv_rn(amax, kE4m3Max) : __uint_as_float(0x7FFFFFFFu);
+      a.codes[row * a.vecs + at] = codes8(y);
+      if ((tid & 15) == 0) a.scales[row * a.blocks + (at >> 4)] = s.scale;
     }
   }
 }
 
 // One CTA of 256 threads per 128 x 128 block: thread t has the 8-element vectors (row t / 16 + 16 i, column t % 16).
 __global__ void __launch_bounds__(256) fp8_pack_weight_kernel(const uint4* w, uint2* codes, float* scales, long long n, int vecs, int blocks) {
-  __shared__ uint32_t warp_top[8];
+  __shared__ float warp_top[8];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x;
   const long long row0 = static_cast<long long>(blockIdx.y) * kFp8Block + (tid >> 4);
   const int at = blockIdx.x * 16 + (tid & 15);
   uint4 v[8];
-  uint32_t top = 0;
+  float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const bool in = row0 + 16 * i < n && at < vecs;
@@ -145,28 +164,27 @@ __global__ void __launch_bounds__(256) fp8_pack_weight_kernel(const uint4* w, ui
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float f[8];
+    float2 f[4];
     widen8(v[i], f);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, abs_bits(f[j]));
+    top = max_abs(top, max_abs8(f));
   }
 #pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+  for (int d = 16; d >= 1; d >>= 1) top = max_abs(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
   if ((tid & 31) == 0) warp_top[tid >> 5] = top;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, warp_top[i]);
-  const bool finite = top < kInfBits;
-  const float amax = fmaxf(__uint_as_float(top), kFp8Floor), inv = __fdiv_rn(kE4m3Max, amax);
+  for (int i = 0; i < 8; ++i) top = max_abs(top, warp_top[i]);
+  const BlockScale s(top);
+  const float2 inv = make_float2(s.inv, s.inv);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float f[8];
+    float2 f[4];
     widen8(v[i], f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = finite ? __fmul_rn(f[j], inv) : 0.0f;
-    if (row0 + 16 * i < n && at < vecs) codes[(row0 + 16 * i) * vecs + at] = e4m3x8(f);
+    for (int j = 0; j < 4; ++j) f[j] = s.finite ? __fmul2_rn(f[j], inv) : make_float2(0.0f, 0.0f);
+    if (row0 + 16 * i < n && at < vecs) codes[(row0 + 16 * i) * vecs + at] = codes8(f);
   }
-  if (tid == 0) scales[static_cast<long long>(blockIdx.y) * blocks + blockIdx.x] = finite ? __fdiv_rn(amax, kE4m3Max) : __uint_as_float(0x7FFFFFFFu);
+  if (tid == 0) scales[static_cast<long long>(blockIdx.y) * blocks + blockIdx.x] = s.scale;
 }
 
 // code * scale, rounded to bf16
