@@ -124,4 +124,17 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int3
 }
 
 #endif  // __CUDACC__
+
+// Host side.  Raises the kernel's shared-memory limit, once per thread and device.
+template <typename K>
+int allow_smem(K kernel, size_t bytes, int* done_dev) {
+  int dev = 0;
+  PLQ_CUDA_TRY(cudaGetDevice(&dev));
+  if (*done_dev != dev) {
+    PLQ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    *done_dev = dev;
+  }
+  return PLQ_OK;
+}
+
 }  // namespace plq

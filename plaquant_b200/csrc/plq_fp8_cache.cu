@@ -1157,12 +1157,8 @@ static int make_cache_tmap(CUtensorMap* tm, const void* base, int64_t batch, int
 
 static int launch_prefill(const CUtensorMap& mk, const CUtensorMap& mv, const Fp8AttnArgs& a, void* stream) {
   static thread_local int done_dev = -1;
-  int dev = 0;
-  PLQ_CUDA_TRY(cudaGetDevice(&dev));
-  if (done_dev != dev) {
-    PLQ_CUDA_TRY(cudaFuncSetAttribute(fp8_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PfCfg::kSmemBytes)));
-    done_dev = dev;
-  }
+  const int st = allow_smem(fp8_prefill_kernel, PfCfg::kSmemBytes, &done_dev);
+  if (st != PLQ_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.kv_heads * a.row_tiles), static_cast<unsigned>(a.batch));
   cfg.blockDim = dim3(384, 1, 1);
@@ -1204,12 +1200,8 @@ template <int R>
 static int launch_attention(const CUtensorMap& mk, const CUtensorMap& mv, const Fp8AttnArgs& a, void* stream) {
   using C = AtCfg<R>;
   static thread_local int done_dev = -1;
-  int dev = 0;
-  PLQ_CUDA_TRY(cudaGetDevice(&dev));
-  if (done_dev != dev) {
-    PLQ_CUDA_TRY(cudaFuncSetAttribute(fp8_attention_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmemBytes)));
-    done_dev = dev;
-  }
+  const int st = allow_smem(fp8_attention_kernel<R>, C::kSmemBytes, &done_dev);
+  if (st != PLQ_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.kv_heads * a.row_tiles), static_cast<unsigned>(a.runs ? a.runs : a.batch));
   cfg.blockDim = dim3(192, 1, 1);
