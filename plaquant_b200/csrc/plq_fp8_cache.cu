@@ -202,6 +202,7 @@ struct Fp8AttnArgs {
   float scale_log2;            // scale * log2(e)
   int batch, t, heads, kv_heads, group, pos_batch, scale_blocks, row_tiles;
   int runs;                    // runs of the row of tiles, or 0: one CTA per sequence
+  int span;                    // fp8_prefill_kernel: rows of a CTA, 256 or 128
 };
 
 // Tiles of 128 positions that sequence b has (0: it sits out, or does not fit).
@@ -862,14 +863,14 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
 
   const int b = static_cast<int>(blockIdx.y), kh = static_cast<int>(blockIdx.x) % a.kv_heads;
   const int pair = a.row_tiles - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;       // the rows that see most first
-  const int rows = a.t * a.group, row0 = pair * 256;
+  const int rows = a.t * a.group, row0 = pair * a.span;
   const long long pos = a.pos_dev != nullptr ? a.pos_dev[static_cast<long long>(b) * a.pos_batch] : a.pos;
   const bool fits = pos <= a.t_max - a.t;
   if (!fits && threadIdx.x == 0 && a.status != nullptr) atomicExch(a.status, PLQ_DEV_RANGE);
   // tiles of 128 positions that the rows of tile x see
   auto tiles_of = [&](int x) {
     const int first = row0 + 128 * x, last = min(first + 128, rows) - 1;
-    return first >= rows || pos < 0 || !fits ? 0 : static_cast<int>((pos + last / a.group) / 128) + 1;
+    return first >= rows || 128 * x >= a.span || pos < 0 || !fits ? 0 : static_cast<int>((pos + last / a.group) / 128) + 1;
   };
   const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
   const uint32_t q_base = smem_u32(q_s), k_base = smem_u32(k_s), v_base = smem_u32(v_s);
@@ -942,7 +943,7 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
     registers_up<C::kRegsRows>();
     const int x = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, row = row0 + 128 * x + r;
     const int mine = x ? n1 : n0, i = row / a.group, h = row - i * a.group;
-    const bool real = row < rows;
+    const bool real = row < rows && 128 * x < a.span;
     const uint32_t s_at = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + 256 * x, o_at = s_at + 128;
     const long long at = (static_cast<long long>(b) * a.t + i) * a.heads + static_cast<long long>(kh) * a.group + h;
 
@@ -1174,14 +1175,17 @@ static int launch_prefill(const CUtensorMap& mk, const CUtensorMap& mv, const Fp
 }
 
 // Rows of a CTA, their tiles, and runs of the row of tiles (0: one CTA per sequence) for a call that sees up to `ctx` positions.
-// rows = 256: fp8_prefill_kernel.
+// rows = 128 or 256: fp8_prefill_kernel.
 struct AttnPlan { int rows, row_tiles, runs; };
 static AttnPlan attn_plan(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t ctx) {
   AttnPlan p;
   const int64_t rows = t * (heads / kv_heads);
+  // Many rows: the kernel with 128 or 256 of them per CTA.  A CTA of it takes 2.6 us for a tile of 128 positions with two row
+  // tiles, one of the other kernel 2.5 us for 32 rows with a second CTA on the SM: below 18 CTAs that one is faster.  Two CTAs
+  // of one row tile each take 3/5 of the time of one of two, as long as there are SMs for them.
   if (rows > 32 && batch * kv_heads * ((rows + 255) / 256) >= 18) {
-    p.rows = 256;
-    p.row_tiles = static_cast<int>((rows + 255) / 256);
+    p.rows = 2 * batch * kv_heads * ((rows + 255) / 256) <= sm_count() ? 128 : 256;
+    p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
     p.runs = 0;
     return p;
   }
@@ -1333,7 +1337,8 @@ extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const 
   memset(&mv, 0, sizeof(mv));
   if ((st = make_cache_tmap(&mk, k_codes, batch, t_max, kv_heads)) != PLQ_OK) return st;
   if ((st = make_cache_tmap(&mv, v_codes, batch, t_max, kv_heads)) != PLQ_OK) return st;
-  if (p.rows == 256) return launch_prefill(mk, mv, a, stream);
+  a.span = p.rows;
+  if (p.rows >= 128) return launch_prefill(mk, mv, a, stream);
   if (p.rows == 8) return launch_attention<8>(mk, mv, a, stream);
   return p.rows == 16 ? launch_attention<16>(mk, mv, a, stream) : launch_attention<32>(mk, mv, a, stream);
 }

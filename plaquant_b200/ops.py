@@ -473,7 +473,7 @@ def _rows_of(x: torch.Tensor, name: str):
 
 
 def _check_gamma(gamma: torch.Tensor, k: int, device) -> torch.Tensor:
-    if gamma.dtype != torch.bfloat16 or gamma.numel() != k:
+    if not isinstance(gamma, torch.Tensor) or gamma.dtype != torch.bfloat16 or gamma.numel() != k:
         raise TypeError("gamma must be bfloat16 [K]")
     if gamma.device != device:
         raise RuntimeError(f"gamma is on {gamma.device}, x on {device}")
@@ -646,12 +646,14 @@ def fp8_cache_attention(q: torch.Tensor, cache, pos, scale: Optional[float] = No
     if q.dtype != torch.bfloat16 or q.dim() != 4 or q.shape[-1] != 128 or not q.is_contiguous():
         raise TypeError("q must be contiguous bfloat16 [B, T, heads, 128]")
     b, t, heads, _ = q.shape
+    cache.check(b, cache.k.shape[-2], q.device)
     kv_heads = cache.kv_heads
-    cache.check(b, kv_heads, q.device)
+    if heads % kv_heads:
+        raise ValueError(f"{heads} query heads do not divide over {kv_heads} key heads")
     ptr, each, host = _positions(pos, b, q.device)
     if ptr is None and host >= 0:
         ctx = min(host + t, cache.room)
-    elif ctx is None:
+    elif not ctx:
         ctx = cache.room
     L = _lib.lib()
     out = torch.empty_like(q)

@@ -402,6 +402,62 @@ def test_attention_reports_positions_outside_the_cache(plq):
         plq.check_device_status()
 
 
+def test_nobody_attends(plq):
+    """A negative position given by the host, no queries, no sequences; split over the device or not."""
+    cache = _filled(plq, 3, 3000, 2, [3000] * 3, 60)
+    for t in (1, 40, 300):
+        assert torch.all(plq.ops.fp8_cache_attention(_rand_q((3, t, 8, 128), 61).cuda(), cache, -1) == 0)
+    before = _clone(plq, cache)
+    qkv, one = _qkv(3, 2, 8, 2, 62), torch.ones(2, 128, device="cuda")
+    plq.ops.rope_kv_append_fp8(qkv, one, one * 0, 8, 2, cache, -3)
+    assert _same(before, cache)
+    assert plq.ops.fp8_cache_attention(torch.empty(3, 0, 8, 128, dtype=torch.bfloat16, device="cuda"), cache, 5).shape == (3, 0, 8, 128)
+    none = plq.kv_cache.Fp8Cache.empty(0, 64, 2, "cuda")
+    assert plq.ops.fp8_cache_attention(torch.empty(0, 1, 8, 128, dtype=torch.bfloat16, device="cuda"), none, 5).shape == (0, 1, 8, 128)
+    plq.check_device_status()
+
+
+def test_refusals_on_the_device(plq):
+    cache = _filled(plq, 2, 100, 2, [100, 100], 63)
+    q = _rand_q((2, 1, 8, 128), 64).cuda()
+    attend = plq.ops.fp8_cache_attention
+    for bad in (q[:, :, :7], q.float(), q.transpose(1, 2), q[..., :64], q[:1]):
+        with pytest.raises((TypeError, ValueError)):
+            attend(bad, cache, 5)
+    for pos in (torch.tensor([1, 2, 3], device="cuda"), torch.tensor([1], dtype=torch.int32, device="cuda"), torch.tensor([1, 2])):
+        with pytest.raises(TypeError):
+            attend(q, cache, pos)
+    with pytest.raises(plq.PlqError):
+        attend(q, cache, torch.tensor([1], device="cuda"), ctx=101)
+    qkv, one = _qkv(2, 1, 8, 2, 65), torch.ones(1, 128, device="cuda")
+    with pytest.raises(TypeError):
+        plq.ops.rope_kv_append_fp8(qkv, one, torch.ones(2, 128, device="cuda"), 8, 2, cache, 0)
+    with pytest.raises(TypeError):
+        plq.ops.rope_kv_append_fp8(qkv[:, :, :-128], one, one, 8, 2, cache, 0)
+    with pytest.raises(TypeError):
+        plq.ops.rope_kv_append_fp8(qkv, one, one, 10, 1, cache, 0)
+    g = torch.ones(512, dtype=torch.bfloat16, device="cuda")
+    x = torch.ones(2, 512, dtype=torch.bfloat16, device="cuda")
+    for bad in (dict(gamma=g[:256]), dict(gamma=g.float())):
+        with pytest.raises(TypeError):
+            plq.ops.fp8_pack(x, **bad)
+    with pytest.raises(TypeError):
+        plq.ops.add_rmsnorm_fp8_pack(x, x, None, 1e-6)
+    with pytest.raises(plq.PlqError):
+        plq.ops.fp8_pack(x[:, :40].contiguous())
+    a, w = plq.ops.fp8_pack(x), plq.ops.fp8_pack_weight(x)
+    for bad in ((w, w), (a, a), (plq.ops.fp8_pack(x[:, :256]), w)):
+        with pytest.raises(ValueError):
+            plq.ops.fp8_gemm(*bad)
+    with pytest.raises(TypeError):
+        plq.ops.fp8_gemm(plq.ops.Fp8Matrix(a.codes, a.scales[:, :2], 1), w)
+    with pytest.raises(TypeError):
+        plq.ops.fp8_gemm(a, w, out_dtype=torch.float16)
+    for out in (torch.empty(2, 3, device="cuda"), torch.empty(3, 2, device="cuda"), torch.empty(2, 4, device="cuda")[:, ::2], torch.empty(1, 2, device="cuda").expand(2, 2)):
+        with pytest.raises(RuntimeError):
+            plq.ops.fp8_gemm(a, w, out=out)
+
+
 def test_step_in_a_graph_at_moving_positions(plq):
     """Append and attention captured once, replayed while the position in device memory moves; two graphs of different shapes
     and an eager stream beside them."""
