@@ -735,7 +735,6 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
 // no tiles: one CTA of four warps per row, a warp taking every fourth run and a lane four elements.
 __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnArgs a, int rows_per_tile) {
   __shared__ int sum_s[4][2];
-  __shared__ float weight_s[4];
   __shared__ float4 acc_s[4][32];
   pdl_launch_dependents();
   pdl_wait();
@@ -773,32 +772,43 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
   const long long base = (unit * a.runs + r0) * 2 * rows_per_tile + (row - rt * rows_per_tile);
   const int late = r0 * length < before ? rows_per_tile : 0;
   auto slot = [&](int x) { return base + (x == 0 ? late : static_cast<long long>(x) * 2 * rows_per_tile); };
-  float4 ahead[4];                                     // the warp's first sums, on their way beside the runs' maxima
+  // One round of loads: a warp's sums, and the maxima and weights of all runs in its lanes.
+  float4 ahead[4];
 #pragma unroll
   for (int y = 0; y < 4; ++y)
     ahead[y] = warp + 4 * y < n ? *reinterpret_cast<const float4*>(a.part + slot(warp + 4 * y) * kHeadDim + 4 * lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float2 own[2];
+#pragma unroll
+  for (int y = 0; y < 2; ++y) own[y] = lane + 32 * y < n ? stat[slot(lane + 32 * y)] : make_float2(kNegInf, 0.0f);
   float top = kNegInf;
-  for (int x = lane; x < n; x += 32) {
+#pragma unroll
+  for (int y = 0; y < 2; ++y)
+    if (own[y].y != 0.0f) top = fmaxf(top, own[y].x);
+  for (int x = lane + 64; x < n; x += 32) {
     const float2 s = stat[slot(x)];
     if (s.y != 0.0f) top = fmaxf(top, s.x);
   }
   top = warp_max(top);
-  float weight = 0.0f;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto add = [&](const float2 s, const float4 v) {     // a run of which the row sees nothing left zeros
-    const float w = s.y == 0.0f ? 0.0f : ex2_approx(s.x - top);
-    weight = fmaf(s.y, w, weight);
-    acc = make_float4(fmaf(v.x, w, acc.x), fmaf(v.y, w, acc.y), fmaf(v.z, w, acc.z), fmaf(v.w, w, acc.w));
-  };
+  auto factor = [&](const float2 s) { return s.y == 0.0f ? 0.0f : ex2_approx(s.x - top); };      // a run of which the row sees nothing left zeros
+  const float w0 = factor(own[0]), w1 = factor(own[1]);
+  float weight = fmaf(own[0].y, w0, own[1].y * w1);     // of the lane's runs
+  for (int x = lane + 64; x < n; x += 32) {
+    const float2 s = stat[slot(x)];
+    weight = fmaf(s.y, factor(s), weight);
+  }
 #pragma unroll
-  for (int y = 0; y < 4; ++y)
-    if (warp + 4 * y < n) add(stat[slot(warp + 4 * y)], ahead[y]);
+  for (int d = 16; d >= 1; d >>= 1) weight += __shfl_xor_sync(0xFFFFFFFFu, weight, d);
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](float w, const float4 v) { acc = make_float4(fmaf(v.x, w, acc.x), fmaf(v.y, w, acc.y), fmaf(v.z, w, acc.z), fmaf(v.w, w, acc.w)); };
+#pragma unroll
+  for (int y = 0; y < 4; ++y) add(__shfl_sync(0xFFFFFFFFu, w0, warp + 4 * y), ahead[y]);
 #pragma unroll 4
-  for (int x = warp + 16; x < n; x += 4) add(stat[slot(x)], *reinterpret_cast<const float4*>(a.part + slot(x) * kHeadDim + 4 * lane));
+  for (int x = warp + 16; x < n; x += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(a.part + slot(x) * kHeadDim + 4 * lane);
+    add(x < 64 ? __shfl_sync(0xFFFFFFFFu, x < 32 ? w0 : w1, x & 31) : factor(stat[slot(x)]), v);
+  }
   acc_s[warp][lane] = acc;
-  if (lane == 0) weight_s[warp] = weight;
   __syncthreads();
-  weight = (weight_s[0] + weight_s[1]) + (weight_s[2] + weight_s[3]);
   const float* part = reinterpret_cast<const float*>(acc_s) + threadIdx.x;
   const float sum = (part[0] + part[128]) + (part[256] + part[384]);
   dst[threadIdx.x] = __float2bfloat16_rn(weight == 0.0f ? 0.0f : sum / weight);
