@@ -202,7 +202,6 @@ struct Fp8AttnArgs {
   float scale_log2;            // scale * log2(e)
   int batch, t, heads, kv_heads, group, pos_batch, scale_blocks, row_tiles;
   int runs;                    // runs of the row of tiles, or 0: one CTA per sequence
-  int span;                    // fp8_prefill_kernel: rows of a CTA, 256 or 128
 };
 
 // Tiles of 128 positions that sequence b has (0: it sits out, or does not fit).
@@ -829,60 +828,62 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
 // Bound by the tensor core (four products of 128 x 128 x 128 per tile: 1024 cycles) and by exponentials (16 a cycle: 1024 cycles).
 struct PfCfg {
   static constexpr int kTile = 128 * kHeadDim;          // 16 KiB
-  static constexpr int kStages = 3;
-  static constexpr size_t kSmemBytes = 1024 + 4 * kTile + 2 * kStages * kTile + 256;
-  // 168 registers a thread at launch (384 x 168); the warps with a row of scores per thread take what the others leave.
-  static constexpr int kRegsMain = 56, kRegsRows = 224;
-  static_assert(128 * kRegsMain + 256 * kRegsRows <= 384 * 168, "register split");
-  static_assert(kSmemBytes <= 232448, "shared memory budget");
+  static constexpr int kBlock = kCacheBlock * kHeadDim; // 8 KiB: 64 positions of K or V
+  static constexpr int kStages = 4;
+  static constexpr size_t kSmemBytes = 1024 + 2 * kTile + 2 * kStages * kBlock + 256;
+  // 128 registers a thread at launch (256 x 128); the warps with a row of scores per thread take what the others leave.
+  static constexpr int kRegsMain = 56, kRegsRows = 200;
+  static_assert(128 * kRegsMain + 128 * kRegsRows <= 256 * 128, "register split");
+  static constexpr size_t kAlone = 116 * 1024;          // more than half of an SM's
+  static_assert(kAlone >= kSmemBytes && 2 * (kSmemBytes + 1024) <= 233472, "shared memory budget");
 };
 constexpr float kHeadroom = 6.0f;                       // log2 of how far a weight may exceed that of M
 
-__global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                              const Fp8AttnArgs a) {
   using C = PfCfg;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* q_s = smem;                                  // [row tile][hi | lo][128 x 128 bytes]
-  uint8_t* k_s = q_s + 4 * C::kTile;
-  uint8_t* v_s = k_s + C::kStages * C::kTile;
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(v_s + C::kStages * C::kTile);
+  uint8_t* q_s = smem;                                  // [hi | lo][128 x 128 bytes]
+  uint8_t* k_s = q_s + 2 * C::kTile;
+  uint8_t* v_s = k_s + C::kStages * C::kBlock;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(v_s + C::kStages * C::kBlock);
   uint64_t* k_empty = k_full + C::kStages, *v_full = k_empty + C::kStages, *v_empty = v_full + C::kStages;
-  uint64_t* q_full = v_empty + C::kStages, *s_full = q_full + 2, *p_half = s_full + 2, *p_full = p_half + 2, *o_full = p_full + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* q_full = v_empty + C::kStages, *s_full = q_full + 1, *p_full = s_full + 2, *o_done = p_full + 2, *o_full = o_done + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-    for (int x = 0; x < 2; ++x) { mbar_init(&q_full[x], 4); mbar_init(&s_full[x], 1); mbar_init(&p_full[x], 4); mbar_init(&p_half[x], 4); mbar_init(&o_full[x], 1); }
+    for (int x = 0; x < 2; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_full[x], 4); }
+    mbar_init(q_full, 4);
+    mbar_init(o_done, 1);
+    mbar_init(o_full, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == 0 && elect_one()) { prefetch_tmap(&map_k); prefetch_tmap(&map_v); }
   if (warp == 1) {
-    tmem_alloc<1>(tmem_holder, 512);
+    tmem_alloc<1>(tmem_holder, 256);
     tmem_relinquish<1>();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_holder;              // per row tile 128 columns of S (and P), 128 of O
+  const uint32_t tmem_base = *tmem_holder;              // two blocks of 64 columns of S (and P), 128 of O
   pdl_launch_dependents();
   pdl_wait();
 
-  const int b = static_cast<int>(blockIdx.y), kh = static_cast<int>(blockIdx.x) % a.kv_heads;
-  const int pair = a.row_tiles - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;       // the rows that see most first
-  const int rows = a.t * a.group, row0 = pair * a.span;
+  // the rows that see most first, of all sequences and key heads
+  const int pairs = a.batch * a.kv_heads, pair = static_cast<int>(blockIdx.x) % pairs, b = pair / a.kv_heads, kh = pair - b * a.kv_heads;
+  const int rt = a.row_tiles - 1 - static_cast<int>(blockIdx.x) / pairs;
+  const int rows = a.t * a.group, row0 = rt * 128;
   const long long pos = a.pos_dev != nullptr ? a.pos_dev[static_cast<long long>(b) * a.pos_batch] : a.pos;
   const bool fits = pos <= a.t_max - a.t;
   if (!fits && threadIdx.x == 0 && a.status != nullptr) atomicExch(a.status, PLQ_DEV_RANGE);
-  // tiles of 128 positions that the rows of tile x see
-  auto tiles_of = [&](int x) {
-    const int first = row0 + 128 * x, last = min(first + 128, rows) - 1;
-    return first >= rows || 128 * x >= a.span || pos < 0 || !fits ? 0 : static_cast<int>((pos + last / a.group) / 128) + 1;
-  };
-  const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+  // blocks of 64 positions that the rows see
+  const int n = pos < 0 || !fits ? 0 : static_cast<int>((pos + (min(row0 + 128, rows) - 1) / a.group) / kCacheBlock) + 1;
   const uint32_t q_base = smem_u32(q_s), k_base = smem_u32(k_s), v_base = smem_u32(v_s);
 
   if (warp < 4) registers_down<C::kRegsMain>();
@@ -894,100 +895,123 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
         const uint32_t parity = ((j / C::kStages) & 1u) ^ 1u;
         ok = mbar_wait_bounded(&k_empty[st], parity, abort_flag);
         if (!ok) break;
-        mbar_arrive_expect_tx(&k_full[st], C::kTile);
-        tma_load_3d(k_base + st * C::kTile, &map_k, kh * kHeadDim, j * 128, b, smem_u32(&k_full[st]));
-        ok = mbar_wait_bounded(&v_empty[st], parity, abort_flag);
+        mbar_arrive_expect_tx(&k_full[st], C::kBlock);
+        tma_load_3d(k_base + st * C::kBlock, &map_k, kh * kHeadDim, j * kCacheBlock, b, smem_u32(&k_full[st]));
+        ok = j == 0 ? mbar_wait_bounded(q_full, 0, abort_flag) : mbar_wait_bounded(&v_empty[st], parity, abort_flag);     // the queries lay there
         if (!ok) break;
-        mbar_arrive_expect_tx(&v_full[st], C::kTile);
-        tma_load_3d(v_base + st * C::kTile, &map_v, kh * kHeadDim, j * 128, b, smem_u32(&v_full[st]));
+        mbar_arrive_expect_tx(&v_full[st], C::kBlock);
+        tma_load_3d(v_base + st * C::kBlock, &map_v, kh * kHeadDim, j * kCacheBlock, b, smem_u32(&v_full[st]));
       }
     }
   } else if (warp == 1) {
     if (elect_one() && n > 0) {
-      constexpr uint32_t idesc_s = make_idesc_e4m3(128, 128), idesc_o = make_idesc_e4m3(128, 128, false, true);
+      constexpr uint32_t idesc_s = make_idesc_e4m3(128, 64), idesc_o = make_idesc_e4m3(128, 128, false, true);
       bool ok = true;
-      // A tile of K (V) is free behind the second row tile's product, or the first's where the second does not reach it.
-      auto scores = [&](int x, int j) {
+      auto scores = [&](int j) {
         const int st = j % C::kStages;
         ok = ok && mbar_wait_bounded(&k_full[st], (j / C::kStages) & 1u, abort_flag);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t q_lo = desc_lo_sw128(q_base + 2 * x * C::kTile), k_lo = desc_lo_sw128(k_base + st * C::kTile);
+        const uint32_t q_lo = desc_lo_sw128(q_base), k_lo = desc_lo_sw128(k_base + st * C::kBlock);
 #pragma unroll
         for (int h = 0; h < 8; ++h)
-          tc_mma_e4m3<1>(tmem_base + 256 * x, q_lo + (h >> 2) * (C::kTile >> 4) + 2 * (h & 3), kDescHiSw128, k_lo + 2 * (h & 3), kDescHiSw128, idesc_s, h != 0);
-        tc_commit<1>(smem_u32(&s_full[x]));
-        if (x == 1 || j >= n1) tc_commit<1>(smem_u32(&k_empty[st]));
+          tc_mma_e4m3<1>(tmem_base + 64 * (j & 1), q_lo + (h >> 2) * (C::kTile >> 4) + 2 * (h & 3), kDescHiSw128, k_lo + 2 * (h & 3), kDescHiSw128, idesc_s, h != 0);
+        tc_commit<1>(smem_u32(&s_full[j & 1]));
+        tc_commit<1>(smem_u32(&k_empty[st]));
       };
-      for (int x = 0; ok && x < 2; ++x)
-        if ((x ? n1 : n0) > 0) {
-          ok = mbar_wait_bounded(&q_full[x], 0, abort_flag);
-          scores(x, 0);
-        }
-      for (int j = 0; ok && j < n; ++j)
-        for (int x = 0; ok && x < 2; ++x) {
-          const int mine = x ? n1 : n0;
-          if (j >= mine) continue;
-          const int st = j % C::kStages;
-          ok = mbar_wait_bounded(&v_full[st], (j / C::kStages) & 1u, abort_flag) && mbar_wait_bounded(&p_half[x], j & 1u, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t v_lo = desc_lo_sw128(v_base + st * C::kTile), p = tmem_base + 256 * x, o = p + 128;
+      ok = mbar_wait_bounded(q_full, 0, abort_flag);
+      scores(0);
+      if (n > 1) scores(1);
+      for (int j = 0; ok && j < n; ++j) {
+        const int st = j % C::kStages;
+        ok = mbar_wait_bounded(&v_full[st], (j / C::kStages) & 1u, abort_flag) && mbar_wait_bounded(&p_full[j & 1], (j >> 1) & 1u, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v_lo = desc_lo_sw128(v_base + st * C::kBlock), p = tmem_base + 64 * (j & 1), o = tmem_base + 128;
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {                 // 32 positions each: codes of hi, then of lo
-            if (h == 2) {
-              ok = mbar_wait_bounded(&p_full[x], j & 1u, abort_flag);
-              if (!ok) break;
-              tc_fence_after();
-            }
-            tc_mma_e4m3_ts(o, p + 16 * h, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, j > 0 || h > 0);
-            tc_mma_e4m3_ts(o, p + 16 * h + 8, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o | kIdescAE5m2, 1u);
-          }
-          if (!ok) break;
-          if (x == 1 || j >= n1) tc_commit<1>(smem_u32(&v_empty[st]));
-          if (j + 1 == mine) tc_commit<1>(smem_u32(&o_full[x]));
-          else scores(x, j + 1);                        // behind the product that still reads P: same pipe, in order
+        for (int h = 0; h < 2; ++h) {                   // 32 positions each: codes of hi, then of lo
+          tc_mma_e4m3_ts(o, p + 16 * h, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, j > 0 || h > 0);
+          tc_mma_e4m3_ts(o, p + 16 * h + 8, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o | kIdescAE5m2, 1u);
         }
+        tc_commit<1>(smem_u32(&v_empty[st]));
+        tc_commit<1>(smem_u32(j + 1 == n ? o_full : o_done));
+        if (j + 2 < n) scores(j + 2);                   // behind the product that still reads P: same pipe, in order
+      }
     }
   } else if (warp >= 4) {
     registers_up<C::kRegsRows>();
-    const int x = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, row = row0 + 128 * x + r;
-    const int mine = x ? n1 : n0, i = row / a.group, h = row - i * a.group;
-    const bool real = row < rows && 128 * x < a.span;
-    const uint32_t s_at = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + 256 * x, o_at = s_at + 128;
-    const long long at = (static_cast<long long>(b) * a.t + i) * a.heads + static_cast<long long>(kh) * a.group + h;
+    const int quad = warp & 3, r = quad * 32 + lane, row = row0 + r;
+    const int i = row / a.group;
+    const bool real = row < rows;
+    const uint32_t s_at = tmem_base + (static_cast<uint32_t>(quad * 32) << 16), o_at = s_at + 128;
 
-    // ---- the row's query: scale, hi and lo codes ----
+    // ---- the queries: whole lines to where V will be, then a row per thread: scale, hi and lo codes ----
+    // Rolled loops: a CTA passes here once, and straight-line code costs more to fetch than to run.
+    const uint32_t raw = v_base + quad * 8192;          // the warp's 32 rows of 256 bytes, 16-byte pieces exchanged by row
+    // copies: two rows at a time, 16 bytes a lane
+    const int first = row0 + quad * 32 + (lane >> 4), first_i = first / a.group, first_h = first - first_i * a.group;
+    const int step_h = a.group == 1 ? 0 : a.group == 2 ? 0 : 2, step = (a.group == 1 ? 2 * a.heads : a.group == 2 ? a.heads : 2) * kHeadDim;
+    const int wrap = (a.heads - a.group) * kHeadDim;
+    const long long copy_at = ((static_cast<long long>(b) * a.t + first_i) * a.heads + static_cast<long long>(kh) * a.group + first_h) * kHeadDim + 8 * (lane & 15);
+    {
+      const __nv_bfloat16* src = a.q + copy_at;
+      int at_row = first, at_h = first_h;
+      uint32_t dst = raw + (lane >> 4) * 256;
+      const uint32_t piece = lane & 15;
+#pragma unroll 4
+      for (int y = 0; y < 16; ++y) {
+        const bool in = at_row < rows;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + ((piece ^ ((2 * y + (lane >> 4)) & 7)) << 4)), "l"(in ? src : a.q), "r"(in ? 16 : 0) : "memory");
+        dst += 512;
+        at_row += 2;
+        src += step;
+        at_h += step_h;
+        if (at_h >= a.group) { at_h -= a.group; src += wrap; }
+      }
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+    }
     float down;
     {
-      const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu;
-      uint4 qv[16];
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + at * kHeadDim);
-#pragma unroll
-      for (int c = 0; c < 16; ++c) qv[c] = real ? src[c] : make_uint4(0, 0, 0, 0);
-      uint32_t top = 0;
-      uint32_t* w = reinterpret_cast<uint32_t*>(qv);
-#pragma unroll
-      for (int d = 0; d < 64; ++d) {
-        w[d] = (w[d] & keep) ^ flip;
-        const uint32_t lo = (w[d] << 16) & 0x7FFF0000u, hi = w[d] & 0x7FFF0000u;
-        if (lo < 0x7F800000u) top = max(top, lo);
-        if (hi < 0x7F800000u) top = max(top, hi);
+      auto piece = [&](int c) {
+        uint4 w;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(raw + lane * 256 + ((c ^ (lane & 7)) << 4)));
+        return w;
+      };
+      uint32_t most = 0;                                // two magnitudes
+#pragma unroll 4
+      for (int c = 0; c < 16; ++c) {
+        const uint4 w = piece(c);
+        most = __vmaxu2(most, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
       }
-      const int e = top == 0 ? 0 : min(max(134 - static_cast<int>(top >> 23), -120), 120);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-#pragma unroll
+      uint32_t top = max(most & 0xFFFFu, most >> 16);
+      const bool finite = top < 0x7F80u;
+      if (!finite) {                                    // infinities and NaN do not set the scale
+        top = 0;
+#pragma unroll 1
+        for (int c = 0; c < 64; ++c) {
+          uint32_t w;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(raw + lane * 256 + (((c >> 2) ^ (lane & 7)) << 4) + 4 * (c & 3)));
+          if ((w & 0x7FFFu) < 0x7F80u) top = max(top, w & 0x7FFFu);
+          if ((w >> 16 & 0x7FFFu) < 0x7F80u) top = max(top, w >> 16 & 0x7FFFu);
+        }
+      }
+      const int e = top == 0 ? 0 : min(max(134 - static_cast<int>(top >> 7), -120), 120);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * (a.scale_log2 < 0.0f ? -1.0f : 1.0f);
+      const uint32_t keep = a.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu;
+      down = finite || a.scale_log2 == 0.0f ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) : __uint_as_float(0x7FFFFFFFu);      // such a row is NaN
+      const uint32_t dst = q_base + (r >> 3) * 1024 + (r & 7) * 128;
+#pragma unroll 1
       for (int c = 0; c < 8; ++c) {
+        const uint4 w0 = piece(2 * c), w1 = piece(2 * c + 1);
+        const uint32_t w[8] = {w0.x & keep, w0.y & keep, w0.z & keep, w0.w & keep, w1.x & keep, w1.y & keep, w1.z & keep, w1.w & keep};
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           uint32_t h2[2], l2[2];
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            float f0 = bf16lo_to_f32(w[8 * c + 2 * d + y]) * up, f1 = bf16hi_to_f32(w[8 * c + 2 * d + y]) * up;
-            if (isinf(f0)) f0 = __uint_as_float(0x7FFFFFFFu);      // an infinite query is NaN, not the largest number
-            if (isinf(f1)) f1 = __uint_as_float(0x7FFFFFFFu);
+            float f0 = bf16lo_to_f32(w[2 * d + y]) * up, f1 = bf16hi_to_f32(w[2 * d + y]) * up;
             h2[y] = e4m3x2(f0, f1);
             const float2 back = e4m3x2_to_f32x2(h2[y]);
             l2[y] = e4m3x2(f0 - back.x, f1 - back.y);
@@ -995,13 +1019,13 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
           hi[d] = h2[0] | h2[1] << 16;
           lo[d] = l2[0] | l2[1] << 16;
         }
-        uint8_t* dst = q_s + 2 * x * C::kTile + (r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(dst + C::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        const uint32_t at = dst + ((c ^ (r & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + C::kTile), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[x]);
+      if (lane == 0) mbar_arrive(q_full);
     }
 
     // ---- the tiles ----
@@ -1012,62 +1036,54 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
     const int last_block = static_cast<int>((written - 1) / kCacheBlock);
     const float per_k = down * (a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2));
     const long long lim = real ? pos + i : pos + a.t - 1;                             // last position the row sees
-    const long long lim_min = pos + (row0 + 128 * x) / a.group;                       // ... of any row of the tile
+    const long long lim_min = pos + row0 / a.group;                       // ... of any row of the tile
     float M = 0.0f, weight = 0.0f;
     bool ok = true;
-    float next_k[2] = {1.0f, 1.0f}, next_v[2] = {1.0f, 1.0f};
+    float next_k = 1.0f, next_v = 1.0f;
     auto fetch = [&](int j) {
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-        if (2 * j + y <= last_block) { next_k[y] = k_scale[2 * j + y]; next_v[y] = v_scale[2 * j + y]; }
+      if (j <= last_block) { next_k = k_scale[j]; next_v = v_scale[j]; }
     };
-    if (mine > 0) fetch(0);
-    for (int j = 0; ok && j < mine; ++j) {
-      float ck[2], lv[2], inv_v[2];
-      const long long t0 = static_cast<long long>(j) * 128;
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const bool sees = lim >= t0 + kCacheBlock * y;
-        ck[y] = sees ? next_k[y] * per_k : 1.0f;
-        if (ck[y] < 1.2e-38f) ck[y] = 1.2e-38f;         // a score of zero, and minus infinity stays what it is
-        float vs = sees ? next_v[y] : 1.0f;
-        if (vs < 1e-36f) vs = 1e-36f;
-        lv[y] = __log2f(vs);
-        inv_v[y] = 1.0f / vs;
-      }
-      if (j + 1 < mine) fetch(j + 1);
-      ok = mbar_wait_bounded_lanes(&s_full[x], j & 1u, abort_flag);
+    if (n > 0) fetch(0);
+    for (int j = 0; ok && j < n; ++j) {
+      const long long t0 = static_cast<long long>(j) * kCacheBlock;
+      const bool sees = lim >= t0;
+      float ck = sees ? next_k * per_k : 1.0f;
+      if (ck < 1.2e-38f) ck = 1.2e-38f;                 // a score of zero, and minus infinity stays what it is
+      float vs = sees ? next_v : 1.0f;
+      if (vs < 1e-36f) vs = 1e-36f;
+      const float lv = __log2f(vs), inv_v = 1.0f / vs;
+      if (j + 1 < n) fetch(j + 1);
+      ok = mbar_wait_bounded_lanes(&s_full[j & 1], (j >> 1) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const bool masked = t0 + 127 > lim_min;           // the same for the whole row tile
-      const int cut = static_cast<int>(min(lim - t0, 127ll));                         // last visible position of the tile
-      uint32_t v[4][32];
+      const bool masked = t0 + 63 > lim_min;            // the same for the whole row tile
+      const uint32_t sp_at = s_at + 64 * (j & 1);
+      uint32_t v[2][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tc_ld_32x32b_x32(s_at + 32 * c, v[c]);
+      for (int c = 0; c < 2; ++c) tc_ld_32x32b_x32(sp_at + 32 * c, v[c]);
       tc_wait_ld();
       if (masked) {
+        const int cut = static_cast<int>(max(-1ll, min(lim - t0, 63ll)));             // last visible position of the block
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int d = 0; d < 32; ++d)
             if (32 * c + d > cut) v[c][d] = 0xFF800000u;
       }
-      float top[2];
+      float m[4];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        float m[4];
+      for (int d = 0; d < 4; ++d) m[d] = fmaxf(__uint_as_float(v[0][d]), __uint_as_float(v[1][d]));
 #pragma unroll
-        for (int d = 0; d < 4; ++d) m[d] = fmaxf(__uint_as_float(v[2 * y][d]), __uint_as_float(v[2 * y + 1][d]));
-#pragma unroll
-        for (int d = 4; d < 32; ++d) m[d & 3] = fmaxf(m[d & 3], fmaxf(__uint_as_float(v[2 * y][d]), __uint_as_float(v[2 * y + 1][d])));
-        top[y] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-      }
-      const float t_max = fmaxf(fmaf(top[0], ck[0], lv[0]), fmaf(top[1], ck[1], lv[1]));
+      for (int d = 4; d < 32; ++d) m[d & 3] = fmaxf(m[d & 3], fmaxf(__uint_as_float(v[0][d]), __uint_as_float(v[1][d])));
+      const float t_max = fmaf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), ck, lv);
       if (j == 0) {
         M = t_max > kNegInf ? t_max : 0.0f;
       } else {
         const bool grow = t_max > M + kHeadroom;
-        if (__any_sync(0xFFFFFFFFu, grow)) {            // O is at rest: its product ended before the scores'
+        if (__any_sync(0xFFFFFFFFu, grow)) {
+          ok = mbar_wait_bounded_lanes(o_done, (j - 1) & 1u, abort_flag);        // the product of the block before is in O
+          if (!ok) break;
+          tc_fence_after();
           const float alpha = grow ? ex2_approx(M - t_max) : 1.0f;
           if (grow) M = t_max;
           weight *= alpha;
@@ -1082,68 +1098,89 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
           }
         }
       }
-      if (t0 + 128 > written) {                         // positions that nobody has written: 0 x NaN would be NaN
+      if (t0 + kCacheBlock > written) {                 // positions that nobody has written: 0 x NaN would be NaN
         const int st = j % C::kStages;
         ok = mbar_wait_bounded_lanes(&v_full[st], (j / C::kStages) & 1u, abort_flag);
         if (!ok) break;
-        if (t0 + r >= written) {
-          uint4* dst = reinterpret_cast<uint4*>(v_s + st * C::kTile + r * 128);
+        if (t0 + (r >> 1) >= written) {
+          uint4* dst = reinterpret_cast<uint4*>(v_s + st * C::kBlock + (r >> 1) * 128) + 4 * (r & 1);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < 4; ++c) dst[c] = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
       }
       // A block that the row sees and whose scale is NaN makes the row NaN, its masked positions included.
+      const float shift = lv + (8.0f - kHeadroom) - M;
+      const float2 ck2 = make_float2(ck, ck), shift2 = make_float2(shift, shift);
+      float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t p[16];
-        const float shift = lv[c >> 1] + (8.0f - kHeadroom) - M;
-        float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
         for (int d = 0; d < 32; d += 4) {
           float w[4];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) w[y] = ex2_approx(fmaf(__uint_as_float(v[c][d + y]), ck[c >> 1], shift));
-          sum0 += w[0] + w[1];
-          sum1 += w[2] + w[3];
+          for (int y = 0; y < 4; y += 2) {
+            const float2 z = __ffma2_rn(make_float2(__uint_as_float(v[c][d + y]), __uint_as_float(v[c][d + y + 1])), ck2, shift2);
+            w[y] = ex2_approx(z.x);
+            w[y + 1] = ex2_approx(z.y);
+            sum = __fadd2_rn(sum, make_float2(w[y], w[y + 1]));
+          }
           const uint32_t c0 = e4m3_e5m2_split(w[0], w[1]), c1 = e4m3_e5m2_split(w[2], w[3]);
           p[d / 4] = __byte_perm(c0, c1, 0x5410);
           p[8 + d / 4] = __byte_perm(c0, c1, 0x7632);
         }
-        weight = fmaf(sum0 + sum1, inv_v[c >> 1], weight);
-        tc_st_32x32b_x16(s_at + 16 * c, p);             // columns of S that have been read
-        if (c & 1) {                                    // the product may begin with the first 64 positions
-          tc_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(c == 1 ? &p_half[x] : &p_full[x]);
-        }
+        tc_st_32x32b_x16(sp_at + 16 * c, p);            // columns of S that have been read
       }
+      weight = fmaf(sum.x + sum.y, inv_v, weight);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[j & 1]);
     }
 
-    // ---- out ----
-    uint4* dst = reinterpret_cast<uint4*>(a.out + at * kHeadDim);
-    if (mine == 0) {
-      if (real)
-#pragma unroll
-        for (int c = 0; c < 16; ++c) dst[c] = make_uint4(0, 0, 0, 0);
-    } else {
-      if (ok) ok = mbar_wait_bounded_lanes(&o_full[x], 0, abort_flag);
+    // ---- out: by way of the queries' memory, so that the stores are whole lines ----
+    const uint32_t o_base = q_base + quad * 8192;       // 32 rows of 256 bytes; nothing reads the queries any more
+    if (n > 0) {
+      if (ok) ok = mbar_wait_bounded_lanes(o_full, 0, abort_flag);
       tc_fence_after();
       const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint32_t v[16], o[8];
-        tc_ld_32x32b_x16(o_at + 16 * c, v);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tc_ld_32x32b_x32(o_at + 32 * c, v);
         tc_wait_ld();
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[d] = f32x2_to_bf16x2(__uint_as_float(v[2 * d]) * inv, __uint_as_float(v[2 * d + 1]) * inv);
-        if (real) {
-          dst[2 * c] = make_uint4(o[0], o[1], o[2], o[3]);
-          dst[2 * c + 1] = make_uint4(o[4], o[5], o[6], o[7]);
+        for (int d = 0; d < 4; ++d) {
+          uint32_t o[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) o[y] = f32x2_to_bf16x2(__uint_as_float(v[8 * d + 2 * y]) * inv, __uint_as_float(v[8 * d + 2 * y + 1]) * inv);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(o_base + lane * 256 + (((4 * c + d) ^ (lane & 7)) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
         }
       }
       tc_fence_before();
+      __syncwarp();
+    }
+    __nv_bfloat16* dst = a.out + copy_at;
+    int at_row = first, at_h = first_h;
+#pragma unroll 1
+    for (int y0 = 0; y0 < 32; y0 += 8) {
+      uint4 o[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int y = y0 + 2 * d + (lane >> 4);
+        o[d] = make_uint4(0, 0, 0, 0);
+        if (n > 0)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o[d].x), "=r"(o[d].y), "=r"(o[d].z), "=r"(o[d].w) : "r"(o_base + y * 256 + (((lane & 15) ^ (y & 7)) << 4)) : "memory");
+      }
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        if (at_row < rows) *reinterpret_cast<uint4*>(dst) = o[d];
+        at_row += 2;
+        dst += step;
+        at_h += step_h;
+        if (at_h >= a.group) { at_h -= a.group; dst += wrap; }
+      }
     }
   }
 
@@ -1156,24 +1193,24 @@ __global__ void __launch_bounds__(384, 1) fp8_prefill_kernel(const __grid_consta
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc<1>(tmem_base, 512);
+    tmem_dealloc<1>(tmem_base, 256);
   }
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
-// u8 cache [batch, t_max, kv_heads * 128]: boxes of 128 tokens x 128 bytes, 128-byte swizzle, zeros behind t_max.
-static int make_cache_tmap(CUtensorMap* tm, const void* base, int64_t batch, int64_t t_max, int64_t kv_heads) {
-  return make_tmap_3d(tm, base, kv_heads * kHeadDim, t_max, batch, kHeadDim, 128);
+// u8 cache [batch, t_max, kv_heads * 128]: boxes of `box` tokens x 128 bytes, 128-byte swizzle, zeros behind t_max.
+static int make_cache_tmap(CUtensorMap* tm, const void* base, int64_t batch, int64_t t_max, int64_t kv_heads, int box) {
+  return make_tmap_3d(tm, base, kv_heads * kHeadDim, t_max, batch, kHeadDim, box);
 }
 
 static int launch_prefill(const CUtensorMap& mk, const CUtensorMap& mv, const Fp8AttnArgs& a, void* stream) {
   static thread_local int done_dev = -1;
-  const int st = allow_smem(fp8_prefill_kernel, PfCfg::kSmemBytes, &done_dev);
+  const int st = allow_smem(fp8_prefill_kernel, PfCfg::kAlone, &done_dev);
   if (st != PLQ_OK) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.kv_heads * a.row_tiles), static_cast<unsigned>(a.batch));
-  cfg.blockDim = dim3(384, 1, 1);
-  cfg.dynamicSmemBytes = PfCfg::kSmemBytes;
+  cfg.gridDim = dim3(static_cast<unsigned>(a.batch) * a.kv_heads * a.row_tiles);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.dynamicSmemBytes = cfg.gridDim.x <= static_cast<unsigned>(sm_count()) ? PfCfg::kAlone : PfCfg::kSmemBytes;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1194,7 +1231,7 @@ static AttnPlan attn_plan(int64_t batch, int64_t t, int64_t heads, int64_t kv_he
   // tiles, one of the other kernel 2.5 us for 32 rows with a second CTA on the SM: below 18 CTAs that one is faster.  Two CTAs
   // of one row tile each take 3/5 of the time of one of two, as long as there are SMs for them.
   if (rows > 32 && batch * kv_heads * ((rows + 255) / 256) >= 18) {
-    p.rows = 2 * batch * kv_heads * ((rows + 255) / 256) <= sm_count() ? 128 : 256;
+    p.rows = 128;
     p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
     p.runs = 0;
     return p;
@@ -1345,9 +1382,9 @@ extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const 
   CUtensorMap mk, mv;
   memset(&mk, 0, sizeof(mk));
   memset(&mv, 0, sizeof(mv));
-  if ((st = make_cache_tmap(&mk, k_codes, batch, t_max, kv_heads)) != PLQ_OK) return st;
-  if ((st = make_cache_tmap(&mv, v_codes, batch, t_max, kv_heads)) != PLQ_OK) return st;
-  a.span = p.rows;
+  const int box = p.rows >= 128 ? kCacheBlock : 128;
+  if ((st = make_cache_tmap(&mk, k_codes, batch, t_max, kv_heads, box)) != PLQ_OK) return st;
+  if ((st = make_cache_tmap(&mv, v_codes, batch, t_max, kv_heads, box)) != PLQ_OK) return st;
   if (p.rows >= 128) return launch_prefill(mk, mv, a, stream);
   if (p.rows == 8) return launch_attention<8>(mk, mv, a, stream);
   return p.rows == 16 ? launch_attention<16>(mk, mv, a, stream) : launch_attention<32>(mk, mv, a, stream);
