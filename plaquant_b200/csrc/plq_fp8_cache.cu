@@ -814,18 +814,28 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
 }
 
 // ---- attention of many queries -----------------------------------------------------------------------------------------
-// The same sums with the queries as the 128 lanes: S = Q K^T, O = P V, a thread owning a row, so that a row's maximum and
-// weight need no exchange.  A CTA has two tiles of 128 rows (queries x heads of a group): while the tensor core works for
-// one, the other's warps turn scores into weights.
+// The same sums with the queries as the 128 lanes: S = Q K^T, O = P V, a thread owning a row (a query and a head of the group),
+// so that a row's maximum and weight need no exchange.  A CTA has 128 rows and two CTAs share an SM: while one of them begins
+// or ends, or turns scores into weights, the tensor core works for the other.
 //   q      hi + lo, both E4M3 at the scale of the row (a power of two that brings its largest element to [128, 256)): exact
 //          for what is at least 2^-10 of that, off by 2^-18 of it below
+//   S      of 64 positions, twice in tensor memory: the product of block j + 2 is issued behind the one that reads the weights
+//          of block j, so the scores of j + 1 lie ready when the weights of j are done
 //   p      hi + lo, E4M3 + E5M2, in tensor memory (A operand), in the place of the scores they come from: off by at most 2^-8
-//          of itself, or half a step of 2^-16
+//          of itself, or by 2^-14 below 2^-6 (the row's largest is 4 to 256): E4M3 leaves up to 2^-10 there, and E5M2 half of
+//          2^-3 of that
 //   O      stays in tensor memory.  The scale of a block of V is part of the weight's exponent: w = exp2(score + log2 vs - M + 2),
 //          with M within 2^6 of the row's largest such sum so far (only beyond that is O scaled, which is rare), and the sum of
 //          the weights takes w / vs.  So a block of large values that nobody looks at does not set the scale of the others.
-//   warp 0 producer, warp 1 MMA issuer, warps 4 - 7 and 8 - 11 one tile of rows each
-// Bound by the tensor core (four products of 128 x 128 x 128 per tile: 1024 cycles) and by exponentials (16 a cycle: 1024 cycles).
+//   warp 0 producer, warp 1 MMA issuer, warps 4 - 7 the rows
+// 128 positions of two row tiles are 2048 cycles of the tensor core (four products of 128 x 128 x 128 each) and as many of
+// exponentials (16 a cycle).  They take 2.2 us (about 4000 cycles): without the weights' arithmetic 1.2 us, with exponentials
+// alone 1.9 us.  Bound by the instructions that turn scores into weights (some 11 an element, of which 3 the two codes), not by
+// their latency: twice the warps with half of the blocks each took 5 % longer, codes by integer arithmetic 3 to 5 % longer.
+// 8192 tokens of 32 heads on 8: 495 us (1.11 PFLOP/s); two prompts of 2048: 85 us.  Of these a CTA's beginning and end take
+// 6 us each; they were 12 with the loops over queries and output unrolled, since code that runs once costs its fetch, and with
+// both row tiles in one CTA nothing hid them: 102 us.  A CTA that took further work over from CTAs that had not started yet
+// (the next queries prepared meanwhile by two warps) was slower, 110 us: two warps take longer for that than the tiles before.
 struct PfCfg {
   static constexpr int kTile = 128 * kHeadDim;          // 16 KiB
   static constexpr int kBlock = kCacheBlock * kHeadDim; // 8 KiB: 64 positions of K or V
@@ -1222,28 +1232,32 @@ static int launch_prefill(const CUtensorMap& mk, const CUtensorMap& mv, const Fp
 }
 
 // Rows of a CTA, their tiles, and runs of the row of tiles (0: one CTA per sequence) for a call that sees up to `ctx` positions.
-// rows = 128 or 256: fp8_prefill_kernel.
+// rows = 128: fp8_prefill_kernel.
 struct AttnPlan { int rows, row_tiles, runs; };
 static AttnPlan attn_plan(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t ctx) {
   AttnPlan p;
-  const int64_t rows = t * (heads / kv_heads);
-  // Many rows: the kernel with 128 or 256 of them per CTA.  A CTA of it takes 2.6 us for a tile of 128 positions with two row
-  // tiles, one of the other kernel 2.5 us for 32 rows with a second CTA on the SM: below 18 CTAs that one is faster.  Two CTAs
-  // of one row tile each take 3/5 of the time of one of two, as long as there are SMs for them.
-  if (rows > 32 && batch * kv_heads * ((rows + 255) / 256) >= 18) {
-    p.rows = 128;
-    p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
-    p.runs = 0;
-    return p;
-  }
+  const int64_t rows = t * (heads / kv_heads), slots = 2 * static_cast<int64_t>(sm_count()), tiles = (ctx + 127) / 128;
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
   p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
   // Two CTAs fit an SM: as many runs as fill the device once, none shorter than four tiles of 128 positions (a CTA's set-up
   // and its share of the join cost about what two tiles do).
-  const int64_t tiles = (ctx + 127) / 128, units = kv_heads * p.row_tiles;
-  int64_t runs = 2 * static_cast<int64_t>(sm_count()) / units;
+  const int64_t units = kv_heads * p.row_tiles;
+  int64_t runs = slots / units;
   if (runs > batch * tiles / 4) runs = batch * tiles / 4;
   p.runs = batch > kMaxFlat || batch * tiles > (1 << 30) || tiles <= 4 || runs < 2 ? 0 : static_cast<int>(runs);
+  if (rows <= 32) return p;
+  // More rows: the kernel with 128 of them per CTA, where it is the faster one.  Both take so many tenths of a microsecond for a
+  // tile: 14 (22 with a second CTA on the SM) for 128 rows, 26 for 32 of them, which the runs spread over the device.  One key
+  // head of 8 with 4 heads each behind 8000 positions: 9 tokens 93 and 24 us, 64 tokens 93 and 55 us, 128 tokens 94 and 103 us,
+  // 256 tokens 96 and 181 us; behind 1000: 9 tokens 16 and 16 us, 256 tokens 20 and 34 us.
+  const int64_t many = batch * kv_heads * ((rows + 127) / 128), few = units * batch;
+  const int64_t time_many = 50 + tiles * (2 * many <= slots ? 14 : 22 * ((many + slots - 1) / slots));
+  const int64_t time_few = 150 + 26 * (p.runs ? (batch * tiles + p.runs - 1) / p.runs : tiles * ((few + slots - 1) / slots));
+  if (time_many <= time_few) {
+    p.rows = 128;
+    p.row_tiles = static_cast<int>((rows + 127) / 128);
+    p.runs = 0;
+  }
   return p;
 }
 

@@ -192,7 +192,8 @@ def _check_attention(out, q, cache, pos, scale=128 ** -0.5):
     """Against float64, within what the arithmetic allows of either kernel, element by element:
       a weight w is two codes - off by 2^-8 of itself at most (E4M3: half of 2^-3; of that rest, E5M2: half of 2^-2 of at most
       2^-4 = 2^-7 in all against the binade, 2^-8 of its largest value) - or by half a step: 2^-18 of the largest weight of its
-      128 positions (E4M3 alone, the largest brought to 256), 2^-19 of the row's largest w vs over its own vs (E5M2, 4 to 256);
+      128 positions (E4M3 alone, the largest brought to 256), 2^-16 of the row's largest w vs over its own vs (E4M3 + E5M2,
+      the largest at 4 or more: below 2^-6 E4M3 leaves up to 2^-10, of which E5M2 is off by 2^-4, together 2^-14 = 2^-16 of 4);
       a query's element that is below 2^-9 of the row's largest is off by 2^-17 of it or by itself, the others are exact;
       the score's float32 arithmetic and exponential by 2^-21 of its size; the result's rounding by 2^-8."""
     b, t, heads, _ = q.shape
@@ -213,7 +214,7 @@ def _check_attention(out, q, cache, pos, scale=128 ** -0.5):
         total = w.sum(-1, keepdim=True)
         want = w @ v / total
         tile = torch.nn.functional.pad(w, (0, -n % 128)).unflatten(-1, (-1, 128)).amax(-1).repeat_interleave(128, -1)[..., :n]
-        step = torch.maximum(2.0 ** -18 * tile, 2.0 ** -19 * (w * vs).amax(-1, keepdim=True) / vs)
+        step = torch.maximum(2.0 ** -18 * tile, 2.0 ** -16 * (w * vs).amax(-1, keepdim=True) / vs)
         top = qq.abs().amax(-1, keepdim=True)
         dq = torch.where(qq.abs() < 2.0 ** -9 * top, torch.minimum(qq.abs(), 2.0 ** -17 * top), torch.zeros_like(qq))
         off = w * (torch.expm1(abs(scale) * (dq @ k.abs().transpose(-1, -2)) + 2.0 ** -21 * (1 + score.abs())))
@@ -333,6 +334,18 @@ def test_attention_of_many_queries(plq, b, t, heads, kv_heads, pos):
     out = plq.ops.fp8_cache_attention(q, cache, pos)
     _check_attention(out, q, cache, [pos] * b)
     assert torch.equal(plq.ops.fp8_cache_attention(q, cache, torch.tensor([pos], device="cuda")), out)
+    plq.check_device_status()
+
+
+# ---- more rows than a tile of the split kernel has, behind positions enough for it to be the faster one ------------------
+@pytest.mark.parametrize("b,t,heads,kv_heads,pos", [(1, 9, 8, 2, 9000), (2, 33, 4, 4, 5001), (1, 40, 10, 2, 8191)])
+def test_several_row_tiles_behind_a_long_past(plq, b, t, heads, kv_heads, pos):
+    cache = _filled(plq, b, pos + t + 70, kv_heads, [pos + t] * b, t + pos)
+    q = _rand_q((b, t, heads, 128), t + pos).cuda()
+    out = plq.ops.fp8_cache_attention(q, cache, pos)
+    _check_attention(out, q, cache, [pos] * b)
+    at = torch.tensor([pos - 4100 * i for i in range(b)], device="cuda")
+    _check_attention(plq.ops.fp8_cache_attention(q, cache, at), q, cache, at.tolist())
     plq.check_device_status()
 
 
