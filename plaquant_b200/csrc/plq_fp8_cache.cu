@@ -290,8 +290,6 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  pdl_launch_dependents();
-  pdl_wait();
 
   // ---- this CTA's work: rows [row0, row0 + nrows) of key head kh, tiles [run0, run1) of the row of tiles ----
   const int unit = static_cast<int>(blockIdx.x), run = static_cast<int>(blockIdx.y);
@@ -299,6 +297,8 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   const int row0 = rt * R, nrows = min(R, a.t * a.group - row0);
   const int i_min = row0 / a.group, i_max = (row0 + nrows - 1) / a.group;
   int run0 = 0, run1 = 0;
+  pdl_wait();
+  pdl_launch_dependents();                             // behind the wait: what joins the sums reads the positions before its own
   if (a.runs) {
     if (warp == 0) {                                   // prefix sums of the sequences' tiles
       int sum = 0;
@@ -736,12 +736,14 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
   __shared__ int sum_s[4][2];
   __shared__ float4 acc_s[4][32];
   pdl_launch_dependents();
-  pdl_wait();
+  // Up to the wait only the positions are read, which are older than the kernel before: that one lets this one begin when all
+  // of its CTAs have waited for them.
   const int at = static_cast<int>(blockIdx.x), bi = at / a.heads, b = bi / a.t;
   const int head = at - bi * a.heads, i = bi - b * a.t, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = sequence_tiles(a, b);
   __nv_bfloat16* dst = a.out + static_cast<long long>(at) * kHeadDim;
   if (tiles == 0) {
+    pdl_wait();
     dst[threadIdx.x] = __float2bfloat16_rn(0.0f);
     return;
   }
@@ -763,7 +765,6 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
     all = tiles * a.batch;
   }
   const int length = run_length(all, a.runs), r0 = before / length, n = (before + tiles - 1) / length - r0 + 1;
-  if (n == 1) return;                                  // written whole
   const int kh = head / a.group, row = i * a.group + (head - kh * a.group), rt = row / rows_per_tile;
   const long long unit = static_cast<long long>(a.row_tiles - 1 - rt) * a.kv_heads + kh;
   const float2* stat = reinterpret_cast<const float2*>(a.part + static_cast<long long>(a.row_tiles) * a.kv_heads * a.runs * 2 * rows_per_tile * kHeadDim);
@@ -771,6 +772,8 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
   const long long base = (unit * a.runs + r0) * 2 * rows_per_tile + (row - rt * rows_per_tile);
   const int late = r0 * length < before ? rows_per_tile : 0;
   auto slot = [&](int x) { return base + (x == 0 ? late : static_cast<long long>(x) * 2 * rows_per_tile); };
+  pdl_wait();
+  if (n == 1) return;                                  // written whole
   // One round of loads: a warp's sums, and the maxima and weights of all runs in its lanes.
   float4 ahead[4];
 #pragma unroll
