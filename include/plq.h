@@ -391,9 +391,9 @@ PLQ_API int plq_fp8_unpack(const void* codes, const void* scales_f32, int64_t ro
  */
 #define PLQ_FP8_STATIC_W       1
 #define PLQ_FP8_AUTO           0
-#define PLQ_FP8_ROWS           1   /* m <= 64: streams the weights once */
-#define PLQ_FP8_128x128        2
-#define PLQ_FP8_PAIR_256x256   3
+#define PLQ_FP8_ROWS           1   /* m <= 64: groups of 16 rows, streams the weights once */
+#define PLQ_FP8_128x128        2   /* one CTA per tile, or a cluster of them along K */
+#define PLQ_FP8_PAIR_256x256   3   /* two CTAs per tile */
 #define PLQ_FP8_PAIR_256x128   4
 #define PLQ_FP8_VARIANT(v)     ((v) << 4)
 PLQ_API int plq_fp8_gemm(const void* a_codes, const void* a_scales_f32, const void* w_codes, const void* w_scales_f32, int64_t m,

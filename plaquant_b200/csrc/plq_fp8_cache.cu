@@ -54,7 +54,8 @@ __device__ __forceinline__ uint2 rope4(uint2 w, float2 c1, float2 c2, float2 s1,
 // the angles are four times the bytes of a head's elements and come from L1 once per thread), every other block
 // quantises one (sequence, head, keys or values, 64-token block) of the new rows, a warp per row and up to eight rows per
 // warp.  Bound by the bytes of the projection (read once) and of the outputs; a decode step by its launch and the chain
-// load -> maximum -> scale -> store.
+// load -> maximum -> scale -> store.  4 x 2048 tokens of 32 + 2 x 8 heads: 67 us (4.8 TB/s; the queries' blocks stream, the
+// others wait for their maximum); 16 tokens of 16 sequences 2.8 us.
 template <int HT>
 __global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8AppendArgs a) {
   __shared__ uint32_t warp_top[8];
@@ -188,6 +189,11 @@ __global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8Append
 // different lengths load it evenly and no length has to be known on the host.  A run is one or several segments (tiles of one
 // sequence); a sequence that lies in several runs leaves partial sums, at most two per run (its first and its last segment),
 // which fp8_attention_join_kernel adds in a fixed order.
+// Bound by the cache's bytes for long ones: one sequence of 131072 positions (64 heads on 8) 52 us, 5.1 TB/s; 16 of 4096 (32 on 8)
+// 32 us, 4.2 TB/s, and 25 us of different lengths.  A tile is a chain of some 2000 cycles for a CTA (scores, maxima over the
+// lanes, weights, product), which two CTAs per SM turn into the memory's rate; about 2.5 us before the first tile and 4 us for
+// the join come on top, which is what a short cache consists of (1 x 4096: 9.4 us).  A join in the kernel itself by the
+// last CTA of a sequence took 64 and 36 us: its counters are six round trips to L2.
 constexpr int kMaxFlat = 256;                          // sequences whose tiles are cut as one row
 
 struct Fp8AttnArgs {

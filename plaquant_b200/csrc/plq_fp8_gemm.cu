@@ -8,10 +8,10 @@
 // scale, to float32 sums in registers while the next block's MMAs run into another accumulator.
 //
 // Two kernels:
-//   fp8_gemv_kernel<MR>     m <= 64: the weights are the 128-row side of the MMA and the activations the narrow one, so
+//   fp8_gemv_kernel         up to 16 rows (64 on request): the weights are the 128-row side of the MMA and the activations the narrow one, so
 //                           that a few rows stream the weights once; bound by HBM (n k bytes).
-//   fp8_gemm_kernel<BN, CG> more rows: 128 x 128 tiles of one CTA or 256 x 256 tiles of a CTA pair; bound by the tensor
-//                           pipe (2 m n k) or, for few tiles, by the chain of one tile.
+//   fp8_gemm_kernel<BN, CG> more rows: 128 x 128 tiles of one CTA, 256 x 128 or 256 x 256 of a CTA pair; bound by the
+//                           tensor pipe (2 m n k) and the epilogue next to it or, for few tiles, by the chain of one tile.
 //
 // Every wait is bounded; on expiry PLQ_DEV_TIMEOUT goes to the caller's status word and all roles leave their loops.
 #include <cstring>
@@ -41,33 +41,37 @@ template <> __device__ __forceinline__ float round_out<float>(float v) { return 
 template <> __device__ __forceinline__ __nv_bfloat16 round_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // ---- a few rows ------------------------------------------------------------------------------------------------------
-// MR: activation rows of a tile (accumulator columns), 16, 32 or 64; more rows are several groups of 64.  A tile is 128 weight
-// rows x one group.  Where there are fewer tiles than CTA slots a cluster of S CTAs shares a tile along K; each leaves its
+// A tile is 128 weight rows x a group of 16 activation rows (accumulator columns); groups of the same weight rows are
+// neighbours.  Where there are fewer tiles than CTA slots a cluster of S CTAs shares a tile along K; each leaves its
 // sums in the shared memory of the CTA that owns the activation row (row j: CTA j mod S), which adds them in the order of the
-// slices: results do not depend on timing and no scratch in HBM is needed.
+// slices: results do not depend on timing and no scratch in HBM is needed.  They are stored there as whole 128-byte lines, one
+// activation row of 32 neighbouring weight rows (scattered 16-byte stores cost 2 us more).
 //   warp 0 producer, warp 1 MMA issuer, warps 2 - 5 epilogue (one weight row per thread)
-template <int MR>
+// Bound by the weights' bytes: 1 x 4096 -> 128256 in 85.8 us (6.1 TB/s, 0.95 of the measured copy rate), 16 x 8192 -> 8192 in
+// 14.1 us (4.8 TB/s); the rest is the launch, the first load and the reduction, 3 - 4 us.
 struct GvCfg {
+  static constexpr int kRows = 16;
   static constexpr int kStages = 5;
-  static constexpr int kXBytes = MR * kStageKBytes;
+  static constexpr int kXBytes = kRows * kStageKBytes;
   static constexpr int kStageBytes = kABytes + kXBytes;
   static constexpr int kAcc = 8;                                      // accumulators in flight
-  static constexpr int kTmemCols = kAcc * MR;                         // two CTAs share an SM
-  static constexpr int kSlotRows = MR + kMaxSlices;                   // S slices x ceil(MR / S) rows
+  static constexpr int kTmemCols = kAcc * kRows;                      // two CTAs share an SM
+  static constexpr int kSlotRows = kRows + kMaxSlices;                // S slices x ceil(kRows / S) rows
   static constexpr int kSlotBytes = kSlotRows * 128 * 4;
-  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kSlotBytes + 4 * MR * 4 + 512;
+  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kSlotBytes + 4 * kRows * 4 + 512;
   static constexpr int kThreads = 192;
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
 
-template <int MR, typename OUT>
+template <typename OUT>
 __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant__ Fp8GemmMaps maps, const Fp8GemmArgs g) {
-  using C = GvCfg<MR>;
+  using C = GvCfg;
+  constexpr int kRows = C::kRows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* slots = reinterpret_cast<float*>(smem + static_cast<size_t>(C::kStages) * C::kStageBytes);       // [slice][owned row][128]
-  float* factors = slots + C::kSlotBytes / 4;                         // [4 warps][MR] scales of the K block at hand
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(factors + 4 * MR);
+  float* factors = slots + C::kSlotBytes / 4;                         // [4 warps][kRows] scales of the K block at hand
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(factors + 4 * kRows);
   uint64_t* empty_bar = full_bar + C::kStages;
   uint64_t* acc_full = empty_bar + C::kStages;
   uint64_t* acc_empty = acc_full + C::kAcc;
@@ -102,7 +106,7 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
   const int num_tiles = g.tiles_n * g.tiles_m;         // tiles_m: groups of activation rows, neighbours share a weight tile
   const uint32_t smem_base = smem_u32(smem);
 
-  float acc[MR];                                       // epilogue: this weight row's sums
+  float acc[kRows];                                       // epilogue: this weight row's sums
 
   if (warp == 0) {
     if (elect_one()) {
@@ -111,7 +115,7 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
         tma_load_2d_cg<1>(smem_base + slot * C::kStageBytes, &maps.w, kb * kStageKBytes, tile / g.tiles_m * kBM, smem_u32(&full_bar[slot]));
       };
       auto load_x = [&](uint32_t slot, int tile, int kb) {
-        tma_load_2d_cg<1>(smem_base + slot * C::kStageBytes + kABytes, &maps.a, kb * kStageKBytes, tile % g.tiles_m * MR, smem_u32(&full_bar[slot]));
+        tma_load_2d_cg<1>(smem_base + slot * C::kStageBytes + kABytes, &maps.a, kb * kStageKBytes, tile % g.tiles_m * kRows, smem_u32(&full_bar[slot]));
       };
       // Static weights: the first ring fill of weight bytes is requested while the previous kernel drains.
       uint32_t early = 0;
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
     }
   } else if (warp == 1) {
     if (elect_one()) {
-      constexpr uint32_t idesc = make_idesc_e4m3(128, MR);
+      constexpr uint32_t idesc = make_idesc_e4m3(128, kRows);
       uint32_t gs = 0;
       bool ok = true;
       for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step)
@@ -147,64 +151,51 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
           const uint32_t w_lo = desc_lo_sw128(smem_base + slot * C::kStageBytes), x_lo = desc_lo_sw128(smem_base + slot * C::kStageBytes + kABytes);
 #pragma unroll
           for (int h = 0; h < 4; ++h)
-            tc_mma_e4m3<1>(tmem_base + as * MR, w_lo + 2 * h, kDescHiSw128, x_lo + 2 * h, kDescHiSw128, idesc, h != 0);
+            tc_mma_e4m3<1>(tmem_base + as * kRows, w_lo + 2 * h, kDescHiSw128, x_lo + 2 * h, kDescHiSw128, idesc, h != 0);
           tc_commit<1>(smem_u32(&empty_bar[slot]));
           tc_commit<1>(smem_u32(&acc_full[as]));
         }
     }
   } else {
-    // ---- epilogue: thread = weight row; lane l of a warp fetches the scales of activation rows l (and l + 32) ----
-    constexpr int kPer = MR > 32 ? 2 : 1;
+    // ---- epilogue: thread = weight row; lane l of a warp fetches the scales of activation row l ----
     const int trow = (warp & 3) * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    float* my_factors = factors + (warp - 2) * MR;
+    float* my_factors = factors + (warp - 2) * kRows;
     pdl_wait();
     uint32_t gs = 0;
     bool ok = true;
     for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
 #pragma unroll
-      for (int j = 0; j < MR; ++j) acc[j] = 0.0f;
-      const int row0 = tile % g.tiles_m * MR;
+      for (int j = 0; j < kRows; ++j) acc[j] = 0.0f;
+      const int row0 = tile % g.tiles_m * kRows;
       const float* sw = g.sw + static_cast<long long>(tile / g.tiles_m) * g.kb;
-      auto scale = [&](int kb, int p) {
-        const int row = lane + 32 * p;
-        return kb < kb1 && row0 + row < g.m && row < MR ? g.sa[static_cast<long long>(row0 + row) * g.kb + kb] * sw[kb] : 0.0f;
+      auto scale = [&](int kb) {
+        return kb < kb1 && row0 + lane < g.m && lane < kRows ? g.sa[static_cast<long long>(row0 + lane) * g.kb + kb] * sw[kb] : 0.0f;
       };
-      float next[4][kPer];                             // scales of the next four K blocks, on their way
+      float next[4];                                   // scales of the next four K blocks, on their way
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int p = 0; p < kPer; ++p) next[i][p] = scale(kb0 + i, p);
+      for (int i = 0; i < 4; ++i) next[i] = scale(kb0 + i);
       for (int kb = kb0; ok && kb < kb1; kb += 4) {
-        float f[4][kPer];
+        float f[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int p = 0; p < kPer; ++p) { f[i][p] = next[i][p]; next[i][p] = scale(kb + 4 + i, p); }
+        for (int i = 0; i < 4; ++i) { f[i] = next[i]; next[i] = scale(kb + 4 + i); }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (!ok || kb + i >= kb1) break;
           __syncwarp();
-#pragma unroll
-          for (int p = 0; p < kPer; ++p)
-            if (lane + 32 * p < MR) my_factors[lane + 32 * p] = f[i][p];
+          if (lane < kRows) my_factors[lane] = f[i];
           const uint32_t as = gs % C::kAcc;
           ok = mbar_wait_bounded_lanes(&acc_full[as], (gs / C::kAcc) & 1u, abort_flag);
           if (!ok) break;
           tc_fence_after();
+          uint32_t r[kRows];
+          tc_ld_32x32b_x16(tmem_base + lane_base + as * kRows, r);
+          tc_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[as]);
 #pragma unroll
-          for (int c = 0; c < MR / 16; ++c) {
-            uint32_t r[16];
-            tc_ld_32x32b_x16(tmem_base + lane_base + as * MR + c * 16, r);
-            tc_wait_ld();
-            if (c == MR / 16 - 1) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&acc_empty[as]);
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(__uint_as_float(r[j]), my_factors[c * 16 + j], acc[c * 16 + j]);
-          }
+          for (int j = 0; j < kRows; ++j) acc[j] = fmaf(__uint_as_float(r[j]), my_factors[j], acc[j]);
           ++gs;
         }
       }
@@ -213,21 +204,21 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
         OUT* y = static_cast<OUT*>(g.y) + row0 * g.ldy + row;
         if (row < g.n) {
 #pragma unroll
-          for (int j = 0; j < MR; ++j)
+          for (int j = 0; j < kRows; ++j)
             if (row0 + j < g.m) y[j * g.ldy] = round_out<OUT>(acc[j]);
         }
       }
     }
   }
   if (nslice > 1) {                                    // one tile per cluster
-    const int trow = (warp & 3) * 32 + lane, row0 = first_tile % g.tiles_m * MR, rows = min(MR, g.m - row0), per = (MR + nslice - 1) / nslice;
+    const int trow = (warp & 3) * 32 + lane, row0 = first_tile % g.tiles_m * kRows, rows = min(kRows, g.m - row0), per = (kRows + nslice - 1) / nslice;
     __syncwarp();
     cluster_wait_acquire();                            // every CTA of the cluster is there
     if (warp >= 2) {
       const uint32_t own = smem_u32(slots) + static_cast<uint32_t>((slice * per * 128 + trow) * 4);
       int cta = 0, at = 0;                             // row j: CTA j % S, its row j / S
 #pragma unroll
-      for (int j = 0; j < MR; ++j) {
+      for (int j = 0; j < kRows; ++j) {
         if (j < rows) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(own + at * 512u, static_cast<uint32_t>(cta))), "f"(acc[j]) : "memory");
         if (++cta == nslice) { cta = 0; ++at; }
       }
@@ -266,6 +257,10 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
 // Per K block an epilogue warp reads its columns from tensor memory and does one packed multiply-add per two of them,
 // beside the 256 (128 x 128) or 512 cycles of the block's MMAs.  The scales travel ahead of the epilogue through a ring of
 // their own (cp.async, 16 K blocks deep): loaded by the epilogue itself their latency was longer than a K block.
+// 8192 x 14336 -> 4096 in 476 us as a burst (2.0 PFLOP/s; 570 - 590 under the power cap).  The sums bound it: a 256 x 256 tile has
+// two accumulators, so the epilogue of a K block has to be done within the MMAs of the next one, and the chain commit, wait,
+// load, add, release is longer than these 512 cycles (600 in all; without the additions 334 us).  Eight warps of 128 columns took
+// 575 us, accumulators of 128 columns 533 (A read twice), 256 x 128 tiles 507, 128 x 128 tiles 524 (feed from L2: 14 TB/s).
 template <int BN, int CG>
 struct GmCfg {
   static constexpr int kBRows = BN / CG;
@@ -623,19 +618,19 @@ static int k_slices(K kernel, unsigned threads, size_t smem, int64_t tiles, int 
   return s > 1 ? static_cast<int>(s) : 1;
 }
 
-template <int MR, typename OUT>
+template <typename OUT>
 static int launch_gemv(const Fp8Ptrs& p, Fp8GemmArgs& g, void* stream) {
-  using C = GvCfg<MR>;
-  auto kernel = fp8_gemv_kernel<MR, OUT>;
+  using C = GvCfg;
+  auto kernel = fp8_gemv_kernel<OUT>;
   static thread_local int done_dev = -1;
   int st = allow_smem(kernel, C::kSmemBytes, &done_dev);
   if (st != PLQ_OK) return st;
   Fp8GemmMaps tm;
   memset(&tm, 0, sizeof(tm));
   if ((st = make_tmap(&tm.w, p.w, g.n, p.k, kBM)) != PLQ_OK) return st;
-  if ((st = make_tmap(&tm.a, p.a, g.m, p.k, MR)) != PLQ_OK) return st;
+  if ((st = make_tmap(&tm.a, p.a, g.m, p.k, C::kRows)) != PLQ_OK) return st;
   g.tiles_n = (g.n + kBM - 1) / kBM;
-  g.tiles_m = (g.m + MR - 1) / MR;
+  g.tiles_m = (g.m + C::kRows - 1) / C::kRows;
   const int slots = 2 * sm_count(), tiles = g.tiles_n * g.tiles_m;
   static thread_local ClusterTable table;
   const int slices = k_slices(kernel, C::kThreads, C::kSmemBytes, tiles, 2, g.kb, 1, &table);
@@ -685,7 +680,7 @@ static int launch_fp8(const Fp8Ptrs& p, Fp8GemmArgs& g, int variant, void* strea
   }
   if (variant == PLQ_FP8_ROWS) {
     if (g.m > 64) return PLQ_ERR_SHAPE;
-    return launch_gemv<16, OUT>(p, g, stream);
+    return launch_gemv<OUT>(p, g, stream);
   }
   if (variant == PLQ_FP8_128x128) return launch_gemm_fp8<128, 1, OUT>(p, g, stream);
   if (variant == PLQ_FP8_PAIR_256x256) return launch_gemm_fp8<256, 2, OUT>(p, g, stream);

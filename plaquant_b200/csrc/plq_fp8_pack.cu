@@ -9,7 +9,9 @@
 // NaN and codes of zero: its values are NaN, and no code ever is.  The floor keeps 448 / a finite; a block below it keeps
 // steps of 2^-109, far below anything a bf16 product can show.
 //
-// Bound by memory: 7 bytes per element with a residual (two bf16 in, one bf16 and one code out), 3 without.
+// Bound by memory: 7 bytes per element with a residual (two bf16 in, one bf16 and one code out), 3 without.  8192 x 8192 with
+// residual and norm: 71.5 us replayed from a graph (6.6 TB/s), 333 x 4112 2.5 us, one row of 4096 2.1 us (a launch and the
+// chain load, sum, maximum, store).  The row stays in registers between its sum and its codes, so it is read once.
 #include "plq_fp8.cuh"
 #include "plq_quant.cuh"
 

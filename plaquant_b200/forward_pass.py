@@ -6,8 +6,10 @@ What runs where.  The hot path of this repository - RMSNorm + rotation + quantis
 quantised linears - runs on the CUDA library (fused: the two RMSNorms of a layer never produce a
 bf16 tensor, they feed the pack kernel, which also absorbs the residual add in front of each norm and
 SiLU(gate) * up in front of the down projection).  Everything else the reference leaves to PyTorch
-stays in PyTorch: embedding, RoPE, scaled-dot-product attention (forward_pass.py:249 there), the final
-norm and the LM head (forward_pass.py:178-181 there).
+stays in PyTorch by default: embedding, scaled-dot-product attention (forward_pass.py:249 there), the final
+norm and the LM head (forward_pass.py:178-181 there).  With `kv_quant="fp8"` the cache is in E4M3 and attention over it
+is the library's; with `fp8_head=True` the last layer's output goes through one norm-and-quantise launch into an E4M3
+LM head.
 
 Tensor parallelism (Megatron): QKV and gate_up are column-parallel (N sharded by heads / by FFN
 columns, no exchange), O and down are row-parallel (K sharded, one all-reduce each), see tp.py.  With
