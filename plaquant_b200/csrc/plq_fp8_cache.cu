@@ -229,7 +229,7 @@ struct AtCfg {
   static constexpr int kDCol0 = 2 * kN;                // two S accumulators, then one D per 64-token block
   static constexpr int kTmemCols = 8 * R;
   static constexpr int kStatFloats = 2 * 4 * R /* warp maxima */ + 4 * 2 * 2 * R /* per warp: factors */ + 4 * R /* per warp: maxima */ + 4 * R;
-  static constexpr size_t kSmemBytes = 1024 + kQBytes + kPBytes + static_cast<size_t>(kKStages + kVStages) * kTile + kStatFloats * 4 + R * 4 + (kMaxFlat + 1) * 4 + 256;
+  static constexpr size_t kSmemBytes = 1024 + kQBytes + kPBytes + static_cast<size_t>(kKStages + kVStages) * kTile + kStatFloats * 4 + R * 4 + (2 * kMaxFlat + 6) * 4 + 256;
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
 
@@ -270,7 +270,9 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   float* red = mloc + 4 * R;                                      // [4 warps][R]
   int* lim_s = reinterpret_cast<int*>(red + 4 * R);               // [R] last position a row sees, relative to the tile loop's base
   int* first_s = lim_s + R;                                       // [batch + 1] first tile of each sequence in the row of tiles
-  uint64_t* bars = reinterpret_cast<uint64_t*>(first_s + kMaxFlat + 2);
+  int* pos_s = first_s + kMaxFlat + 1;                            // their positions
+  int* start_s = pos_s + kMaxFlat;                                // the run: first and last tile, sequence of the first
+  uint64_t* bars = reinterpret_cast<uint64_t*>(start_s + 5);
   uint64_t* k_full = bars, *k_empty = k_full + C::kKStages, *v_full = k_empty + C::kKStages, *v_empty = v_full + C::kVStages;
   uint64_t* s_full = v_empty + C::kVStages, *s_empty = s_full + 2, *p_full = s_empty + 2, *d_full = p_full + 1, *q_full = d_full + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_full + 1);
@@ -309,29 +311,39 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     if (warp == 0) {                                   // prefix sums of the sequences' tiles
       int sum = 0;
       for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        const int own = b0 + lane < a.batch ? sequence_tiles(a, b0 + lane) : 0;
+        long long pos = -1;
+        const int own = b0 + lane < a.batch ? sequence_tiles(a, b0 + lane, &pos) : 0;
         int x = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
           const int y = __shfl_up_sync(0xFFFFFFFFu, x, d);
           if (lane >= d) x += y;
         }
-        if (b0 + lane < a.batch) first_s[b0 + lane] = sum + x - own;
+        if (b0 + lane < a.batch) {
+          first_s[b0 + lane] = sum + x - own;
+          pos_s[b0 + lane] = own ? static_cast<int>(pos) : -1;
+        }
         sum += __shfl_sync(0xFFFFFFFFu, x, 31);
       }
-      if (lane == 0) first_s[a.batch] = sum;
+      const int length = run_length(sum, a.runs), from = min(run * length, sum);
+      __syncwarp();
+      int begun = 0;                                   // sequences that start at or before the run's first tile
+      for (int b0 = 0; b0 < a.batch; b0 += 32)
+        begun += __popc(__ballot_sync(0xFFFFFFFFu, b0 + lane < a.batch && first_s[b0 + lane] <= from));
+      if (lane == 0) {
+        first_s[a.batch] = sum;
+        start_s[0] = from;
+        start_s[1] = min(from + length, sum);
+        start_s[2] = begun - 1;
+      }
     }
     __syncthreads();
-    const int length = run_length(first_s[a.batch], a.runs);
-    run0 = min(run * length, first_s[a.batch]);
-    run1 = min(run0 + length, first_s[a.batch]);
+    run0 = start_s[0];
+    run1 = start_s[1];
   }
   // the segments of the run, in order; false behind the last one
   struct Segment { int b, tile0, n; long long pos; bool whole; };
-  int next_b = a.runs ? 0 : run;
-  if (a.runs)
-    for (int step = kMaxFlat / 2; step >= 1; step >>= 1)          // the last sequence that starts at or before run0
-      if (next_b + step < a.batch && first_s[next_b + step] <= run0) next_b += step;
+  int next_b = a.runs ? start_s[2] : run;
   auto next_segment = [&](Segment& g) {
     if (!a.runs) {
       if (next_b != run) return false;
@@ -344,7 +356,8 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
       while (next_b < a.batch && first_s[next_b] < run1 && first_s[next_b + 1] <= max(run0, first_s[next_b])) ++next_b;     // empty ones
       if (next_b >= a.batch || first_s[next_b] >= run1) return false;
       g.b = next_b++;
-      const int f = first_s[g.b], all = sequence_tiles(a, g.b, &g.pos);
+      const int f = first_s[g.b], all = first_s[g.b + 1] - f;
+      g.pos = pos_s[g.b];
       g.tile0 = max(run0 - f, 0);
       const int end = min(run1 - f, all);
       g.whole = g.tile0 == 0 && end == all;

@@ -258,8 +258,8 @@ __global__ void __launch_bounds__(192, 2) fp8_gemv_kernel(const __grid_constant_
 // beside the 256 (128 x 128) or 512 cycles of the block's MMAs.  The scales travel ahead of the epilogue through a ring of
 // their own (cp.async, 16 K blocks deep): loaded by the epilogue itself their latency was longer than a K block.
 // 8192 x 14336 -> 4096 in 476 us as a burst (2.0 PFLOP/s; 570 - 590 under the power cap).  The sums bound it: a 256 x 256 tile has
-// two accumulators, so the epilogue of a K block has to be done within the MMAs of the next one, and the chain commit, wait,
-// load, add, release is longer than these 512 cycles (600 in all; without the additions 334 us).  Eight warps of 128 columns took
+// two accumulators, so the epilogue of a K block has to be done within the MMAs of the next one (512 cycles), and the chain commit,
+// wait, load, add, release is longer: 0.60 us a K block, without the additions 0.43 us (334 us in all).  Eight warps of 128 columns took
 // 575 us, accumulators of 128 columns 533 (A read twice), 256 x 128 tiles 507, 128 x 128 tiles 524 (feed from L2: 14 TB/s).
 template <int BN, int CG>
 struct GmCfg {
