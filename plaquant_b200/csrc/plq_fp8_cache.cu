@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
 // exponentials (16 a cycle).  They take 2.2 us (about 4000 cycles): without the weights' arithmetic 1.2 us, with exponentials
 // alone 1.9 us.  Bound by the instructions that turn scores into weights (some 11 an element, of which 3 the two codes), not by
 // their latency: twice the warps with half of the blocks each took 5 % longer, codes by integer arithmetic 3 to 5 % longer.
-// 8192 tokens of 32 heads on 8: 495 us (1.11 PFLOP/s); two prompts of 2048: 85 us.  Of these a CTA's beginning and end take
+// 8192 tokens of 32 heads on 8: 487 us (1.13 PFLOP/s); two prompts of 2048: 81 us.  Of these a CTA's beginning and end take
 // 6 us each; they were 12 with the loops over queries and output unrolled, since code that runs once costs its fetch, and with
 // both row tiles in one CTA nothing hid them: 102 us.  A CTA that took further work over from CTAs that had not started yet
 // (the next queries prepared meanwhile by two warps) was slower, 110 us: two warps take longer for that than the tiles before.
@@ -1064,11 +1064,12 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
     const long long scales = (static_cast<long long>(b) * a.kv_heads + kh) * a.scale_blocks;
     const float* k_scale = a.k_scale + scales;
     const float* v_scale = a.v_scale + scales;
-    const long long written = pos + a.t;                // positions behind may hold anything
-    const int last_block = static_cast<int>((written - 1) / kCacheBlock);
+    // a sequence with positions ends below 2^31
+    const int written = static_cast<int>(n > 0 ? pos + a.t : 0);                      // positions behind may hold anything
+    const int last_block = (written - 1) / kCacheBlock;
     const float per_k = down * (a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2));
-    const long long lim = real ? pos + i : pos + a.t - 1;                             // last position the row sees
-    const long long lim_min = pos + row0 / a.group;                       // ... of any row of the tile
+    const int lim = real ? written - a.t + i : written - 1;                             // last position the row sees
+    const int lim_min = written - a.t + row0 / a.group;                       // ... of any row of the tile
     float M = 0.0f, weight = 0.0f;
     bool ok = true;
     float next_k = 1.0f, next_v = 1.0f;
@@ -1077,13 +1078,13 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
     };
     if (n > 0) fetch(0);
     for (int j = 0; ok && j < n; ++j) {
-      const long long t0 = static_cast<long long>(j) * kCacheBlock;
+      const int t0 = j * kCacheBlock;
       const bool sees = lim >= t0;
       float ck = sees ? next_k * per_k : 1.0f;
       if (ck < 1.2e-38f) ck = 1.2e-38f;                 // a score of zero, and minus infinity stays what it is
       float vs = sees ? next_v : 1.0f;
       if (vs < 1e-36f) vs = 1e-36f;
-      const float lv = __log2f(vs), inv_v = 1.0f / vs;
+      const float lv = __log2f(vs), inv_v = rcp_approx(vs);
       if (j + 1 < n) fetch(j + 1);
       ok = mbar_wait_bounded_lanes(&s_full[j & 1], (j >> 1) & 1u, abort_flag);
       if (!ok) break;
@@ -1095,7 +1096,7 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
       for (int c = 0; c < 2; ++c) tc_ld_32x32b_x32(sp_at + 32 * c, v[c]);
       tc_wait_ld();
       if (masked) {
-        const int cut = static_cast<int>(max(-1ll, min(lim - t0, 63ll)));             // last visible position of the block
+        const int cut = max(-1, min(lim - t0, 63));         // last visible position of the block
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
