@@ -27,7 +27,7 @@ struct Fp8AppendArgs {
   int* status;
   int t, heads, kv_heads, pos_batch, units_per_head;
   int scale_blocks;            // ceil(t_max / 64)
-  unsigned q_blocks;
+  unsigned long long unit_rate;  // 2^32 * units / blocks, rounded up: block i has floor(i * rate / 2^32) units before it
 };
 
 // The smallest 2^e with amax <= 448 * 2^e, e >= -100; `bits`: amax as an integer.
@@ -50,19 +50,22 @@ __device__ __forceinline__ uint2 rope4(uint2 w, float2 c1, float2 c2, float2 s1,
                     f32x2_to_bf16x2(__fadd_rn(__fmul_rn(bx, c2.x), __fmul_rn(ax, s2.x)), __fadd_rn(__fmul_rn(by, c2.y), __fmul_rn(ay, s2.y))));
 }
 
-// One launch: the first q_blocks blocks rotate the queries (eight threads per head, 16 elements each of HT neighbouring heads:
-// the angles are four times the bytes of a head's elements and come from L1 once per thread), every other block
-// quantises one (sequence, head, keys or values, 64-token block) of the new rows, a warp per row and up to eight rows per
-// warp.  Bound by the bytes of the projection (read once) and of the outputs; a decode step by its launch and the chain
-// load -> maximum -> scale -> store.  4 x 2048 tokens of 32 + 2 x 8 heads: 67 us (4.8 TB/s; the queries' blocks stream, the
-// others wait for their maximum); 16 tokens of 16 sequences 2.8 us.
+// One launch.  Most blocks rotate queries (eight threads per head, 16 elements each of HT neighbouring heads: the angles are
+// four times the bytes of a head's elements and come from L1 once per thread); a unit quantises one (sequence, head, keys or
+// values, 64-token block) of the new rows, a warp per row and up to eight rows per warp.  Units lie evenly between the others:
+// their chain load -> maximum -> scale -> store leaves time that the queries' streams fill.  Bound by the bytes of the
+// projection (read once) and of the outputs; a decode step by its launch and that chain.  4 x 2048 tokens of 64 + 2 x 8 heads:
+// 56 us (0.88 of the measured copy rate; 68 with the units last and the rows of a unit loaded one after the other); 16 tokens of 16
+// sequences 2.6 us.
 template <int HT>
-__global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8AppendArgs a) {
+__global__ void __launch_bounds__(256, 4) rope_kv_append_fp8_kernel(const Fp8AppendArgs a) {
   __shared__ uint32_t warp_top[8];
   pdl_launch_dependents();
   pdl_wait();
-  if (blockIdx.x < a.q_blocks) {
-    const long long idx = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  // blocks of either kind alternate, so that the ones' waits are filled by the others' streams
+  const unsigned units_before = static_cast<unsigned>(blockIdx.x * a.unit_rate >> 32);
+  if (static_cast<unsigned>((blockIdx.x + 1) * a.unit_rate >> 32) == units_before) {
+    const long long idx = static_cast<long long>(blockIdx.x - units_before) * blockDim.x + threadIdx.x;
     if (idx >= a.q_threads) return;
     const int j = static_cast<int>(idx & 7), groups = a.heads / HT;
     const long long hr = idx >> 3, row = hr / groups, b = row / a.t;
@@ -98,7 +101,7 @@ __global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8Append
     }
     return;
   }
-  const unsigned unit = blockIdx.x - a.q_blocks;
+  const unsigned unit = units_before;
   const int u = static_cast<int>(unit % a.units_per_head);
   const unsigned rest = unit / a.units_per_head;
   const int side = static_cast<int>(rest & 1u), kh = static_cast<int>((rest >> 1) % a.kv_heads);
@@ -120,18 +123,42 @@ __global__ void __launch_bounds__(256) rope_kv_append_fp8_kernel(const Fp8Append
 
   uint2 w[8];
   uint32_t top = 0;
+  if (fresh == kCacheBlock) {                          // a whole block: all loads are on their way before the first is used
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(a.qkv + (b * a.t + (start - pos) + warp) * a.ld8 + head * 16) + lane;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = warp + 8 * i;
-    w[i] = make_uint2(0, 0);
-    if (r < fresh) {
-      const long long tt = start - pos + r;
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(a.qkv + (b * a.t + tt) * a.ld8 + head * 16) + lane;
-      w[i] = make_uint2(src[0], src[32]);
-      if (!side) {
-        const float2* cos = reinterpret_cast<const float2*>(a.cos + b * a.cs_batch + tt * kHeadDim) + lane;
-        const float2* sin = reinterpret_cast<const float2*>(a.sin + b * a.cs_batch + tt * kHeadDim) + lane;
-        w[i] = rope4(w[i], cos[0], cos[32], sin[0], sin[32]);
+    for (int i = 0; i < 8; ++i) w[i] = make_uint2(src[32 * i * a.ld8], src[32 * i * a.ld8 + 32]);
+    if (!side) {
+      const long long at = b * a.cs_batch + (start - pos + warp) * kHeadDim;
+      const float2* cos = reinterpret_cast<const float2*>(a.cos + at) + lane;
+      const float2* sin = reinterpret_cast<const float2*>(a.sin + at) + lane;
+#pragma unroll
+      for (int g = 0; g < 8; g += 4) {
+        float2 c[4][2], n[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            c[i][x] = cos[8 * (g + i) * (kHeadDim / 2) + 32 * x];
+            n[i][x] = sin[8 * (g + i) * (kHeadDim / 2) + 32 * x];
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[g + i] = rope4(w[g + i], c[i][0], c[i][1], n[i][0], n[i][1]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = warp + 8 * i;
+      w[i] = make_uint2(0, 0);
+      if (r < fresh) {
+        const long long tt = start - pos + r;
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(a.qkv + (b * a.t + tt) * a.ld8 + head * 16) + lane;
+        w[i] = make_uint2(src[0], src[32]);
+        if (!side) {
+          const float2* cos = reinterpret_cast<const float2*>(a.cos + b * a.cs_batch + tt * kHeadDim) + lane;
+          const float2* sin = reinterpret_cast<const float2*>(a.sin + b * a.cs_batch + tt * kHeadDim) + lane;
+          w[i] = rope4(w[i], cos[0], cos[32], sin[0], sin[32]);
+        }
       }
     }
   }
@@ -1342,9 +1369,9 @@ extern "C" int plq_rope_kv_append_fp8(const void* qkv_bf16, int64_t ld, const vo
   a.t_max = t_max;
   a.ld8 = ld / 8;
   a.cs_batch = cs_batch_stride;
-  // several heads per thread where there are enough of them for every SM
+  // two heads per thread where there are enough of them for every SM (four need 80 registers: three CTAs per SM, 60 us for 56)
   const int64_t head_rows = batch * t * heads;
-  const int ht = head_rows * 8 < 2 * 2048 * static_cast<int64_t>(sm_count()) ? 1 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+  const int ht = head_rows * 8 < 2 * 2048 * static_cast<int64_t>(sm_count()) ? 1 : heads % 2 == 0 ? 2 : 1;
   a.q_threads = head_rows / ht * 8;
   a.status = dev_status;
   a.t = static_cast<int>(t);
@@ -1355,7 +1382,7 @@ extern "C" int plq_rope_kv_append_fp8(const void* qkv_bf16, int64_t ld, const vo
   a.units_per_head = static_cast<int>((t + kCacheBlock - 2) / kCacheBlock + 1);      // blocks that t rows can touch
   const int64_t q_blocks = (a.q_threads + 255) / 256, blocks = q_blocks + batch * kv_heads * 2 * a.units_per_head;
   if (blocks > 0x7FFFFFFF) return PLQ_ERR_LIMIT;
-  a.q_blocks = static_cast<unsigned>(q_blocks);
+  a.unit_rate = ((static_cast<unsigned long long>(blocks - q_blocks) << 32) + blocks - 1) / blocks;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(256, 1, 1);
@@ -1365,7 +1392,7 @@ extern "C" int plq_rope_kv_append_fp8(const void* qkv_bf16, int64_t ld, const vo
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, ht == 4 ? rope_kv_append_fp8_kernel<4> : ht == 2 ? rope_kv_append_fp8_kernel<2> : rope_kv_append_fp8_kernel<1>, a));
+  PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, ht == 2 ? rope_kv_append_fp8_kernel<2> : rope_kv_append_fp8_kernel<1>, a));
   return PLQ_OK;
 }
 
