@@ -29,7 +29,8 @@ struct Fp8GemmArgs {
   int32_t* status;
   int m, n, kb;                // kb: K blocks of 128
   int tiles_m, tiles_n;
-  int vec;                     // rows of y allow stores of 32 (2), 16 (1) bytes or of single elements (0)
+  int vec;                     // rows of y allow stores of 32 (2), 16 (1) bytes or neither (0)
+  int pairs;                   // bf16: rows begin at multiples of four bytes and n is even
   int static_w;                // weights may be read before the programmatic dependency wait
   int band;                    // row tiles per band of the tile order
 };
@@ -272,7 +273,7 @@ struct GmCfg {
   static constexpr int kSfSlots = 16;
   static constexpr int kSfBytes = 512 + 16;                                 // 128 row scales, the scales of the tile's weight blocks
   static constexpr int kThreads = 128 + 32 * kEpiWarps;
-  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kSfSlots * kSfBytes + 640;
+  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kSfSlots * kSfBytes + 640 + kEpiWarps * 32 * 36;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 
@@ -283,11 +284,15 @@ __device__ __forceinline__ void fp8_tile(int tile, const Fp8GemmArgs& g, int& tm
   tm = b * g.band + (r - tn * rows);
 }
 
-// 16 neighbouring columns of a row
+// 16 neighbouring columns of 32 rows, a row per lane.  Where rows or the edge do not allow wide stores the columns go through
+// 1152 bytes of the warp's own (rows 36 bytes apart: no bank twice), so that neighbouring lanes still store neighbouring columns:
+// 2549 x 336 -> 5057 takes 25 us, with each lane storing its row by elements 135; 1079 x 816 -> 12188 30 and 150.
+constexpr int kStoreBytes = 32 * 36;
 template <typename OUT>
-__device__ __forceinline__ void store16(const Fp8GemmArgs& g, int row, int col, const float2* s) {
-  OUT* y = static_cast<OUT*>(g.y) + row * g.ldy;
+__device__ __forceinline__ void store16(const Fp8GemmArgs& g, int row0, int lane, int col, const float2* s, uint8_t* scratch) {
   if (g.vec && col + 16 <= g.n) {
+    OUT* y = static_cast<OUT*>(g.y) + (row0 + lane) * g.ldy;
+    if (row0 + lane >= g.m) return;
     if constexpr (sizeof(OUT) == 4) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) __stcs(reinterpret_cast<float4*>(y + col) + i, make_float4(s[2 * i].x, s[2 * i].y, s[2 * i + 1].x, s[2 * i + 1].y));
@@ -303,11 +308,37 @@ __device__ __forceinline__ void store16(const Fp8GemmArgs& g, int row, int col, 
         __stcs(reinterpret_cast<uint4*>(y + col + 8), make_uint4(d[4], d[5], d[6], d[7]));
       }
     }
-  } else {
+    return;
+  }
+  constexpr int kPart = 32 / static_cast<int>(sizeof(OUT));          // columns that go through at a time
+  const uint32_t base = smem_u32(scratch);
+#pragma unroll
+  for (int part = 0; part < 16; part += kPart) {
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (col + 2 * i < g.n) y[col + 2 * i] = round_out<OUT>(s[i].x);
-      if (col + 2 * i + 1 < g.n) y[col + 2 * i + 1] = round_out<OUT>(s[i].y);
+      uint32_t d;
+      if constexpr (sizeof(OUT) == 4) d = __float_as_uint(i & 1 ? s[(part + i) / 2].y : s[(part + i) / 2].x);
+      else d = f32x2_to_bf16x2(s[i].x, s[i].y);
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + lane * 36 + i * 4), "r"(d) : "memory");
+    }
+    __syncwarp();
+    if (sizeof(OUT) == 4 || g.pairs) {                  // eight words a row, four rows at a time
+      const int c = col + part + (lane & 7) * (4 / static_cast<int>(sizeof(OUT)));
+#pragma unroll 1
+      for (int i = lane >> 3; i < 32; i += 4) {
+        uint32_t d;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(d) : "r"(base + i * 36 + (lane & 7) * 4) : "memory");
+        if (row0 + i < g.m && c < g.n) *reinterpret_cast<uint32_t*>(static_cast<OUT*>(g.y) + (row0 + i) * g.ldy + c) = d;
+      }
+    } else {                                            // sixteen elements a row, two rows at a time
+      const int c = col + (lane & 15);
+#pragma unroll 1
+      for (int i = lane >> 4; i < 32; i += 2) {
+        uint16_t d;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(d) : "r"(base + i * 36 + (lane & 15) * 2) : "memory");
+        if (row0 + i < g.m && c < g.n) *reinterpret_cast<uint16_t*>(static_cast<OUT*>(g.y) + (row0 + i) * g.ldy + c) = d;
+      }
     }
   }
 }
@@ -325,6 +356,7 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
   uint64_t* sf_full = acc_empty + C::kAcc;
   uint64_t* sf_empty = sf_full + C::kSfSlots;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sf_empty + C::kSfSlots);
+  uint8_t* store_s = smem + C::kSmemBytes - 1024 - C::kEpiWarps * kStoreBytes;        // the epilogue warps' way out
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
@@ -449,7 +481,7 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
     for (int tile = first; ok && tile < num_tiles; tile += step) {
       int tm, tn;
       fp8_tile(tile, g, tm, tn);
-      const int row = (tm * CG + static_cast<int>(rank)) * kBM + quad * 32 + lane;
+      const int row0 = (tm * CG + static_cast<int>(rank)) * kBM + quad * 32;
       const int col0 = tn * BN + cgp * C::kCols;
 #pragma unroll
       for (int j = 0; j < C::kCols / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
@@ -484,9 +516,9 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
         }
       }
       if (!ok) break;
-      if (slices == 1 && row < g.m) {
+      if (slices == 1) {
 #pragma unroll
-        for (int v = 0; v < C::kCols / 16; ++v) store16<OUT>(g, row, col0 + v * 16, acc + v * 8);
+        for (int v = 0; v < C::kCols / 16; ++v) store16<OUT>(g, row0, lane, col0 + v * 16, acc + v * 8, store_s + (warp - 4) * kStoreBytes);
       }
     }
   }
@@ -518,7 +550,6 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
       if (warp >= 4 && !*abort_flag) {
         int tm, tn;
         fp8_tile(first, g, tm, tn);
-        const int row = tm * kBM + trow;
         for (int at = cgp; at < per; at += 2) {
           const int group = at * slices + slice;
           if (group >= 8) break;
@@ -530,7 +561,7 @@ __global__ void __launch_bounds__(GmCfg<BN, CG>::kThreads, 1) fp8_gemm_kernel(co
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] = make_float2(sum[i].x + src[256 * i], sum[i].y + src[256 * i + 128]);
           }
-          if (row < g.m) store16<OUT>(g, row, tn * BN + group * 16, sum);
+          store16<OUT>(g, tm * kBM + quad * 32, lane, tn * BN + group * 16, sum, store_s + (warp - 4) * kStoreBytes);
         }
       }
     }
@@ -716,6 +747,7 @@ extern "C" int plq_fp8_gemm(const void* a_codes, const void* a_scales_f32, const
   g.static_w = flags & PLQ_FP8_STATIC_W;
   const auto fits = [&](uintptr_t bytes) { return reinterpret_cast<uintptr_t>(y) % bytes == 0 && static_cast<uintptr_t>(ldy) * es % bytes == 0; };
   g.vec = fits(32) ? 2 : fits(16) ? 1 : 0;
+  g.pairs = reinterpret_cast<uintptr_t>(y) % 4 == 0 && ldy % 2 == 0 && n % 2 == 0;
   const Fp8Ptrs p = {a_codes, w_codes, k};
   return y_is_f32 ? launch_fp8<float>(p, g, variant, stream) : launch_fp8<__nv_bfloat16>(p, g, variant, stream);
 }

@@ -189,6 +189,24 @@ def test_product_into_a_buffer(plq):
     assert tuple(plq.ops.fp8_gemm(empty, w).shape) == (0, 16)
 
 
+@pytest.mark.parametrize("variant", ["128x128", "pair256x256", "pair256x128"])
+@pytest.mark.parametrize("m,n", [(129, 258), (200, 301), (33, 70), (257, 15), (64, 500)])
+def test_many_rows_at_any_edge_and_alignment(plq, variant, m, n):
+    """Rows that allow stores of 32, 16, four and two bytes, both types, edges inside a group of 16 columns."""
+    for k in (256, 4096):
+        a, w = _operands(m, n, k, m + n)
+        for dtype in (torch.bfloat16, torch.float32):
+            want = plq.ops.fp8_gemm(a, w, out_dtype=dtype, variant=variant)
+            _check_product(want, a, w)
+            for stride, shift in ((n, 1), (n + 1, 0), (n + 1, 1), (n + 2, 2), (n + 16 - n % 16, 0), (n + 24 - n % 8, 8)):
+                store = torch.full((m * stride + shift + 8,), 7.0, dtype=dtype, device="cuda")
+                out = store[shift: shift + m * stride].view(m, stride)[:, :n]
+                assert torch.equal(plq.ops.fp8_gemm(a, w, out=out, variant=variant), want)
+                out[:] = 7.0
+                assert torch.all(store == 7.0)
+    plq.check_device_status()
+
+
 def test_rows_do_not_depend_on_each_other(plq):
     """A row or column that is not finite stays alone; a row's result does not depend on the rows around it."""
     for m in (9, 200):
