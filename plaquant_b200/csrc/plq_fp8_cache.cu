@@ -776,6 +776,20 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   }
 }
 
+// fp8_prefill_kernel, below
+struct PfCfg {
+  static constexpr int kRows = 128;
+  static constexpr int kTile = 128 * kHeadDim;          // 16 KiB
+  static constexpr int kBlock = kCacheBlock * kHeadDim; // 8 KiB: 64 positions of K or V
+  static constexpr int kStages = 4;
+  static constexpr size_t kSmemBytes = 1024 + 2 * kTile + 2 * kStages * kBlock + 256;
+  // 128 registers a thread at launch (256 x 128); the warps with a row of scores per thread take what the others leave.
+  static constexpr int kRegsMain = 56, kRegsRows = 200;
+  static_assert(128 * kRegsMain + 128 * kRegsRows <= 256 * 128, "register split");
+  static constexpr size_t kAlone = 116 * 1024;          // more than half of an SM's
+  static_assert(kAlone >= kSmemBytes && 2 * (kSmemBytes + 1024) <= 233472, "shared memory budget");
+};
+
 // Adds the partial sums of the sequences that lie in several runs, in a fixed order, and clears the output of those that have
 // no tiles: one CTA of four warps per row, a warp taking every fourth run and a lane four elements.
 __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnArgs a, int rows_per_tile) {
@@ -794,7 +808,10 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
     return;
   }
   int before = 0, all = 0;                             // tiles of the sequences in front, of all
-  if (a.pos_dev != nullptr && a.pos_batch) {
+  const bool own_runs = rows_per_tile == PfCfg::kRows;  // every sequence is cut into runs of its own
+  if (own_runs) {
+    all = tiles;
+  } else if (a.pos_dev != nullptr && a.pos_batch) {
     for (int x = threadIdx.x; x < a.batch; x += 128) {
       const int n = sequence_tiles(a, x);
       all += n;
@@ -813,11 +830,13 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
   const int length = run_length(all, a.runs), r0 = before / length, n = (before + tiles - 1) / length - r0 + 1;
   const int kh = head / a.group, row = i * a.group + (head - kh * a.group), rt = row / rows_per_tile;
   const long long unit = static_cast<long long>(a.row_tiles - 1 - rt) * a.kv_heads + kh;
-  const float2* stat = reinterpret_cast<const float2*>(a.part + static_cast<long long>(a.row_tiles) * a.kv_heads * a.runs * 2 * rows_per_tile * kHeadDim);
+  const long long units = static_cast<long long>(a.row_tiles) * a.kv_heads;
+  const int each = own_runs ? rows_per_tile : 2 * rows_per_tile;                 // partial sums of a run
+  const float2* stat = reinterpret_cast<const float2*>(a.part + (own_runs ? a.batch : 1) * units * a.runs * each * kHeadDim);
   // the sequence is the first segment of every run but perhaps of the one it starts in
-  const long long base = (unit * a.runs + r0) * 2 * rows_per_tile + (row - rt * rows_per_tile);
+  const long long base = ((own_runs ? b * units + unit : unit) * a.runs + r0) * each + (row - rt * rows_per_tile);
   const int late = r0 * length < before ? rows_per_tile : 0;
-  auto slot = [&](int x) { return base + (x == 0 ? late : static_cast<long long>(x) * 2 * rows_per_tile); };
+  auto slot = [&](int x) { return base + (x == 0 ? late : static_cast<long long>(x) * each); };
   pdl_wait();
   if (n == 1) return;                                  // written whole
   // One round of loads: a warp's sums, and the maxima and weights of all runs in its lanes.
@@ -881,23 +900,16 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
 // exponentials (16 a cycle).  They take 2.2 us (about 4000 cycles): without the weights' arithmetic 1.2 us, with exponentials
 // alone 1.9 us.  Bound by the instructions that turn scores into weights (some 11 an element, of which 3 the two codes), not by
 // their latency: twice the warps with half of the blocks each took 5 % longer, codes by integer arithmetic 3 to 5 % longer.
-// 8192 tokens of 32 heads on 8: 487 us (1.13 PFLOP/s); two prompts of 2048: 81 us.  Of these a CTA's beginning and end take
+// 8192 tokens of 32 heads on 8: 474 us (1.16 PFLOP/s); two prompts of 2048: 80 us.  Of these a CTA's beginning and end take
 // 6 us each; they were 12 with the loops over queries and output unrolled, since code that runs once costs its fetch, and with
 // both row tiles in one CTA nothing hid them: 102 us.  A CTA that took further work over from CTAs that had not started yet
 // (the next queries prepared meanwhile by two warps) was slower, 110 us: two warps take longer for that than the tiles before.
-struct PfCfg {
-  static constexpr int kTile = 128 * kHeadDim;          // 16 KiB
-  static constexpr int kBlock = kCacheBlock * kHeadDim; // 8 KiB: 64 positions of K or V
-  static constexpr int kStages = 4;
-  static constexpr size_t kSmemBytes = 1024 + 2 * kTile + 2 * kStages * kBlock + 256;
-  // 128 registers a thread at launch (256 x 128); the warps with a row of scores per thread take what the others leave.
-  static constexpr int kRegsMain = 56, kRegsRows = 200;
-  static_assert(128 * kRegsMain + 128 * kRegsRows <= 256 * 128, "register split");
-  static constexpr size_t kAlone = 116 * 1024;          // more than half of an SM's
-  static_assert(kAlone >= kSmemBytes && 2 * (kSmemBytes + 1024) <= 233472, "shared memory budget");
-};
+// Few CTAs and a long past: each sequence is cut into runs, whose sums O and weight at their M go to the join (64 tokens of 32
+// heads on 8 behind 8000 positions 88 -> 25 us).
 constexpr float kHeadroom = 6.0f;                       // log2 of how far a weight may exceed that of M
 
+// RUNS: every sequence in a.runs runs of its own, for the join; as a branch it would cost the other calls 4 %
+template <bool RUNS>
 __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                              const Fp8AttnArgs a) {
   using C = PfCfg;
@@ -931,8 +943,9 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;              // two blocks of 64 columns of S (and P), 128 of O
-  pdl_launch_dependents();
+  if constexpr (!RUNS) pdl_launch_dependents();
   pdl_wait();
+  if constexpr (RUNS) pdl_launch_dependents();          // behind the wait where the join follows, as in fp8_attention_kernel
 
   // the rows that see most first, of all sequences and key heads
   const int pairs = a.batch * a.kv_heads, pair = static_cast<int>(blockIdx.x) % pairs, b = pair / a.kv_heads, kh = pair - b * a.kv_heads;
@@ -942,7 +955,17 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
   const bool fits = pos <= a.t_max - a.t;
   if (!fits && threadIdx.x == 0 && a.status != nullptr) atomicExch(a.status, PLQ_DEV_RANGE);
   // blocks of 64 positions that the rows see
-  const int n = pos < 0 || !fits ? 0 : static_cast<int>((pos + (min(row0 + 128, rows) - 1) / a.group) / kCacheBlock) + 1;
+  const int seen = pos < 0 || !fits ? 0 : static_cast<int>((pos + (min(row0 + 128, rows) - 1) / a.group) / kCacheBlock) + 1;
+  // of these the CTA's run: blocks [j0, j0 + n)
+  int j0 = 0, n = seen;
+  bool whole = true, idle = false;
+  if constexpr (RUNS) {
+    const int tiles = sequence_tiles(a, b), length = run_length(tiles, a.runs), run = static_cast<int>(blockIdx.y);
+    j0 = 2 * run * length;
+    idle = run * length >= tiles;
+    whole = tiles <= length;
+    n = idle ? 0 : max(0, min(seen, j0 + 2 * length) - j0);
+  }
   const uint32_t q_base = smem_u32(q_s), k_base = smem_u32(k_s), v_base = smem_u32(v_s);
 
   if (warp < 4) registers_down<C::kRegsMain>();
@@ -955,11 +978,11 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
         ok = mbar_wait_bounded(&k_empty[st], parity, abort_flag);
         if (!ok) break;
         mbar_arrive_expect_tx(&k_full[st], C::kBlock);
-        tma_load_3d(k_base + st * C::kBlock, &map_k, kh * kHeadDim, j * kCacheBlock, b, smem_u32(&k_full[st]));
+        tma_load_3d(k_base + st * C::kBlock, &map_k, kh * kHeadDim, (j0 + j) * kCacheBlock, b, smem_u32(&k_full[st]));
         ok = j == 0 ? mbar_wait_bounded(q_full, 0, abort_flag) : mbar_wait_bounded(&v_empty[st], parity, abort_flag);     // the queries lay there
         if (!ok) break;
         mbar_arrive_expect_tx(&v_full[st], C::kBlock);
-        tma_load_3d(v_base + st * C::kBlock, &map_v, kh * kHeadDim, j * kCacheBlock, b, smem_u32(&v_full[st]));
+        tma_load_3d(v_base + st * C::kBlock, &map_v, kh * kHeadDim, (j0 + j) * kCacheBlock, b, smem_u32(&v_full[st]));
       }
     }
   } else if (warp == 1) {
@@ -1101,11 +1124,11 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
     bool ok = true;
     float next_k = 1.0f, next_v = 1.0f;
     auto fetch = [&](int j) {
-      if (j <= last_block) { next_k = k_scale[j]; next_v = v_scale[j]; }
+      if (j0 + j <= last_block) { next_k = k_scale[j0 + j]; next_v = v_scale[j0 + j]; }
     };
     if (n > 0) fetch(0);
     for (int j = 0; ok && j < n; ++j) {
-      const int t0 = j * kCacheBlock;
+      const int t0 = (j0 + j) * kCacheBlock;
       const bool sees = lim >= t0;
       float ck = sees ? next_k * per_k : 1.0f;
       if (ck < 1.2e-38f) ck = 1.2e-38f;                 // a score of zero, and minus infinity stays what it is
@@ -1199,9 +1222,37 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
       if (lane == 0) mbar_arrive(&p_full[j & 1]);
     }
 
-    // ---- out: by way of the queries' memory, so that the stores are whole lines ----
+    // ---- out: a run's sums as they are, for the join ----
+    if (RUNS && !whole) {
+      if (ok && n > 0) ok = mbar_wait_bounded_lanes(o_full, 0, abort_flag);
+      tc_fence_after();
+      const long long units = static_cast<long long>(a.row_tiles) * a.kv_heads;
+      const long long slot = ((b * units + static_cast<long long>(a.row_tiles - 1 - rt) * a.kv_heads + kh) * a.runs + blockIdx.y) * C::kRows + r;
+      float* dst = a.part + slot * kHeadDim;
+#pragma unroll 1
+      for (int c = 0; c < 8; ++c) {
+        uint32_t v[16];
+        if (n > 0) {
+          tc_ld_32x32b_x16(o_at + 16 * c, v);
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int d = 0; d < 16; ++d) v[d] = 0;
+        }
+        if (real && !idle) {
+#pragma unroll
+          for (int d = 0; d < 16; d += 8)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 16 * c + d), "r"(v[d]), "r"(v[d + 1]), "r"(v[d + 2]), "r"(v[d + 3]),
+                         "r"(v[d + 4]), "r"(v[d + 5]), "r"(v[d + 6]), "r"(v[d + 7]) : "memory");
+        }
+      }
+      if (real && !idle)                                // weights are in units of exp2(M + 2 - headroom), see above
+        *reinterpret_cast<float2*>(a.part + a.batch * units * a.runs * C::kRows * kHeadDim + 2 * slot) = make_float2(M - (8.0f - kHeadroom), weight);
+      tc_fence_before();
+    }
+    // ---- or the result: by way of the queries' memory, so that the stores are whole lines ----
     const uint32_t o_base = q_base + quad * 8192;       // 32 rows of 256 bytes; nothing reads the queries any more
-    if (n > 0) {
+    if (whole && n > 0) {
       if (ok) ok = mbar_wait_bounded_lanes(o_full, 0, abort_flag);
       tc_fence_after();
       const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
@@ -1235,7 +1286,7 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
       }
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        if (at_row < rows) *reinterpret_cast<uint4*>(dst) = o[d];
+        if (at_row < rows && whole && !idle) *reinterpret_cast<uint4*>(dst) = o[d];
         at_row += 2;
         dst += step;
         at_h += step_h;
@@ -1263,21 +1314,28 @@ static int make_cache_tmap(CUtensorMap* tm, const void* base, int64_t batch, int
   return make_tmap_3d(tm, base, kv_heads * kHeadDim, t_max, batch, kHeadDim, box);
 }
 
+template <bool RUNS>
 static int launch_prefill(const CUtensorMap& mk, const CUtensorMap& mv, const Fp8AttnArgs& a, void* stream) {
   static thread_local int done_dev = -1;
-  const int st = allow_smem(fp8_prefill_kernel, PfCfg::kAlone, &done_dev);
+  const int st = allow_smem(fp8_prefill_kernel<RUNS>, PfCfg::kAlone, &done_dev);
   if (st != PLQ_OK) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.batch) * a.kv_heads * a.row_tiles);
+  cfg.gridDim = dim3(static_cast<unsigned>(a.batch) * a.kv_heads * a.row_tiles, static_cast<unsigned>(a.runs ? a.runs : 1));
   cfg.blockDim = dim3(256, 1, 1);
-  cfg.dynamicSmemBytes = cfg.gridDim.x <= static_cast<unsigned>(sm_count()) ? PfCfg::kAlone : PfCfg::kSmemBytes;
+  cfg.dynamicSmemBytes = cfg.gridDim.x * cfg.gridDim.y <= static_cast<unsigned>(sm_count()) ? PfCfg::kAlone : PfCfg::kSmemBytes;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp8_prefill_kernel, mk, mv, a));
+  PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp8_prefill_kernel<RUNS>, mk, mv, a));
+  if (a.runs) {
+    cfg.gridDim = dim3(static_cast<unsigned>(a.batch * a.t * a.heads));
+    cfg.blockDim = dim3(128, 1, 1);
+    cfg.dynamicSmemBytes = 0;
+    PLQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp8_attention_join_kernel, a, PfCfg::kRows));
+  }
   return PLQ_OK;
 }
 
@@ -1295,18 +1353,22 @@ static AttnPlan attn_plan(int64_t batch, int64_t t, int64_t heads, int64_t kv_he
   int64_t runs = slots / units;
   if (runs > batch * tiles / 4) runs = batch * tiles / 4;
   p.runs = batch > kMaxFlat || batch * tiles > (1 << 30) || tiles <= 4 || runs < 2 ? 0 : static_cast<int>(runs);
-  if (rows <= 32) return p;
-  // More rows: the kernel with 128 of them per CTA, where it is the faster one.  Both take so many tenths of a microsecond for a
-  // tile: 14 (22 with a second CTA on the SM) for 128 rows, 26 for 32 of them, which the runs spread over the device.  One key
-  // head of 8 with 4 heads each behind 8000 positions: 9 tokens 93 and 24 us, 64 tokens 93 and 55 us, 128 tokens 94 and 103 us,
-  // 256 tokens 96 and 181 us; behind 1000: 9 tokens 16 and 16 us, 256 tokens 20 and 34 us.
+  if (rows <= 16) return p;
+  // More rows: the kernel with 128 of them per CTA, every sequence whole or in runs of its own, where it is the faster one.  Both
+  // take so many tenths of a microsecond for a tile: 14 (22 with a second CTA on the SM) for 128 rows, 26 for 32 of them; the join
+  // of the one's runs costs 5 us more and 0.3 for every 128 rows, that of the other's 10.  8 key heads with 4 heads each behind
+  // 8000 positions, 32 rows a CTA / 128 whole / 128 in runs: 9 tokens 21 / 88 / 16 us, 64 tokens 50 / 88 / 25, 256 tokens 170 / 90 /
+  // 65; four sequences of 128 tokens 370 / 90 / 116.
   const int64_t many = batch * kv_heads * ((rows + 127) / 128), few = units * batch;
-  const int64_t time_many = 50 + tiles * (2 * many <= slots ? 14 : 22 * ((many + slots - 1) / slots));
   const int64_t time_few = 150 + 26 * (p.runs ? (batch * tiles + p.runs - 1) / p.runs : tiles * ((few + slots - 1) / slots));
-  if (time_many <= time_few) {
-    p.rows = 128;
+  const int64_t time_whole = 50 + tiles * (2 * many <= slots ? 14 : 22 * ((many + slots - 1) / slots));
+  int64_t split = slots / many;
+  if (split > tiles / 4) split = tiles / 4;
+  const int64_t time_split = split < 2 ? time_whole + 1 : 100 + 3 * many + (tiles + split - 1) / split * (2 * many * split <= slots ? 14 : 22);
+  if (time_whole <= time_few || time_split <= time_few) {
+    p.rows = PfCfg::kRows;
     p.row_tiles = static_cast<int>((rows + 127) / 128);
-    p.runs = 0;
+    p.runs = time_whole <= time_split ? 0 : static_cast<int>(split);
   }
   return p;
 }
@@ -1400,7 +1462,8 @@ extern "C" int64_t plq_fp8_attention_workspace_bytes(int64_t batch, int64_t t, i
   using namespace plq;
   if (batch < 1 || t < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || ctx < 1) return 0;
   const AttnPlan p = attn_plan(batch, t, heads, kv_heads, ctx);
-  return kv_heads * p.row_tiles * static_cast<int64_t>(p.runs) * 2 * p.rows * static_cast<int64_t>((kHeadDim + 2) * sizeof(float));
+  const int64_t each = p.rows == PfCfg::kRows ? batch : 2;             // partial sums of a run and row: of every sequence, or of two
+  return kv_heads * p.row_tiles * static_cast<int64_t>(p.runs) * each * p.rows * static_cast<int64_t>((kHeadDim + 2) * sizeof(float));
 }
 
 extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const void* k_scales_f32, const void* v_codes, const void* v_scales_f32,
@@ -1449,7 +1512,7 @@ extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const 
   const int box = p.rows >= 128 ? kCacheBlock : 128;
   if ((st = make_cache_tmap(&mk, k_codes, batch, t_max, kv_heads, box)) != PLQ_OK) return st;
   if ((st = make_cache_tmap(&mv, v_codes, batch, t_max, kv_heads, box)) != PLQ_OK) return st;
-  if (p.rows >= 128) return launch_prefill(mk, mv, a, stream);
+  if (p.rows >= 128) return p.runs ? launch_prefill<true>(mk, mv, a, stream) : launch_prefill<false>(mk, mv, a, stream);
   if (p.rows == 8) return launch_attention<8>(mk, mv, a, stream);
   return p.rows == 16 ? launch_attention<16>(mk, mv, a, stream) : launch_attention<32>(mk, mv, a, stream);
 }

@@ -349,6 +349,27 @@ def test_several_row_tiles_behind_a_long_past(plq, b, t, heads, kv_heads, pos):
     plq.check_device_status()
 
 
+@pytest.mark.parametrize("t,heads,kv_heads,pos", [(128, 8, 2, [4000]), (24, 32, 4, [9000]), (100, 12, 2, [5000, 130, -1]), (17, 3, 1, [3000, 0, 2047, 511]),
+                                                  (65, 16, 1, [20000]), (300, 5, 5, [1, 7000])])
+def test_many_queries_in_runs(plq, t, heads, kv_heads, pos):
+    """Long pasts and few rows: every sequence cut along its positions; short ones are one run, absent ones none."""
+    b, room = len(pos), max(pos) + t + 70
+    cache = _filled(plq, b, room, kv_heads, [p + t if p >= 0 else 0 for p in pos], t + heads)
+    q = _rand_q((b, t, heads, 128), t).cuda()
+    at = torch.tensor(pos, device="cuda")
+    out = plq.ops.fp8_cache_attention(q, cache, at)
+    _check_attention(out, q, cache, pos)
+    assert torch.equal(plq.ops.fp8_cache_attention(q, cache, at, ctx=max(pos) + t), plq.ops.fp8_cache_attention(q, cache, at, ctx=max(pos) + t))
+    plq.check_device_status()
+    over = torch.tensor([room - t + 1] + pos[1:], device="cuda")
+    out = plq.ops.fp8_cache_attention(q, cache, over)
+    assert torch.all(out[0] == 0)
+    for i in range(1, b):
+        _check_attention(out[i: i + 1], q[i: i + 1], plq.kv_cache.Fp8Cache(*(x[i: i + 1] for x in (cache.k, cache.k_scale, cache.v, cache.v_scale))), pos[i: i + 1])
+    with pytest.raises(plq.PlqError):
+        plq.check_device_status()
+
+
 @pytest.mark.parametrize("lengths", [[0, 129, 500, -1, 63, 64], [1000, 2, 1, 190, -1, 0]])
 def test_many_queries_of_ragged_batches(plq, lengths):
     pos = [n - 1 if n == 0 else n for n in lengths]
