@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(256, 4) rope_kv_append_fp8_kernel(const Fp8App
 //          power-of-two scale per tile of queries)
 //   256 p  hi + lo, 256 p <= 256 within a tile of 128 tokens: off by at most 2^-9 of itself (a bf16 would be by 2^-8) or by
 //          half a step of 2^-9, which is 2^-18 of the tile's largest weight
-// With S^T = K Q^T the 128 tokens of a tile are the lanes of tensor memory and the query rows its columns (R = 8, 16 or 32 of
+// With S^T = K Q^T the 128 tokens of a tile are the lanes of tensor memory and the query rows its columns (R = 8 or 16 of
 // them: heads of a group x queries), so a thread owns one token, and the scale of its key is a factor of the whole warp;
 // O^T = V^T P^T has the 128 elements of the head as its lanes.  Each 64-token block of V gets an accumulator of its own, to
 // which the block's scale is applied in float32 on the way into the running sums in registers.
@@ -251,7 +251,7 @@ struct AtCfg {
   static constexpr int kN = 2 * R;                     // columns of either product: hi | lo
   static constexpr int kPBytes = kN * 128;
   static constexpr int kQBytes = kN * 128;
-  static constexpr int kKStages = 3, kVStages = R == 32 ? 2 : 3;
+  static constexpr int kKStages = 3, kVStages = 3;
   static constexpr int kTile = 128 * kHeadDim;         // 16 KiB
   static constexpr int kDCol0 = 2 * kN;                // two S accumulators, then one D per 64-token block
   static constexpr int kTmemCols = 8 * R;
@@ -326,11 +326,8 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
 
-  // ---- this CTA's work: rows [row0, row0 + nrows) of key head kh, tiles [run0, run1) of the row of tiles ----
-  const int unit = static_cast<int>(blockIdx.x), run = static_cast<int>(blockIdx.y);
-  const int rt = a.row_tiles - 1 - unit / a.kv_heads, kh = unit % a.kv_heads;       // the rows that see most first
-  const int row0 = rt * R, nrows = min(R, a.t * a.group - row0);
-  const int i_min = row0 / a.group, i_max = (row0 + nrows - 1) / a.group;
+  // ---- this CTA's work: all rows of key head kh, tiles [run0, run1) of the row of tiles ----
+  const int kh = static_cast<int>(blockIdx.x), run = static_cast<int>(blockIdx.y), nrows = a.t * a.group;
   int run0 = 0, run1 = 0;
   pdl_wait();
   pdl_launch_dependents();                             // behind the wait: what joins the sums reads the positions before its own
@@ -390,10 +387,10 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
       g.whole = g.tile0 == 0 && end == all;
       g.n = end - g.tile0;
     }
-    if (g.n > 0) g.n = max(0, min(g.n, static_cast<int>((g.pos + i_max) / 128) + 1 - g.tile0));      // what these rows see of it
+    if (g.n > 0) g.n = max(0, min(g.n, static_cast<int>((g.pos + a.t - 1) / 128) + 1 - g.tile0));      // what these rows see of it
     return true;
   };
-  if (unit == 0 && (run == 0 || !a.runs) && a.status != nullptr) {
+  if (kh == 0 && (run == 0 || !a.runs) && a.status != nullptr) {
     const int first = a.runs ? static_cast<int>(threadIdx.x) : run;
     for (int b = first; b < (a.runs ? a.batch : run + 1); b += 192) {
       const long long pos = a.pos_dev != nullptr ? a.pos_dev[b * a.pos_batch] : a.pos;
@@ -474,37 +471,33 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     const long long b = g.b, pos = g.pos;
     const int n = g.n, tile0 = g.tile0;
     // ---- the queries: tile-wide power-of-two scale, hi and lo codes ----
-    constexpr int kPer = R > 16 ? R / 16 : 1;         // 16-element chunks per thread
-    const bool has_q = R >= 16 || tid < 8 * R;
+    const bool has_q = tid < 8 * R;                   // 16 elements each
     const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu;      // a negative or no scale
     const __nv_bfloat16* q_base = a.q + ((b * a.t) * a.heads + static_cast<long long>(kh) * a.group) * kHeadDim;
-    uint4 qv[kPer][2];
+    uint4 qv[2];
     uint32_t top = 0;
+    const int r = tid >> 3;
+    qv[0] = qv[1] = make_uint4(0, 0, 0, 0);
+    if (r < nrows) {
+      const int i = r / a.group, h = r - i * a.group;
+      const uint4* src = reinterpret_cast<const uint4*>(q_base + (static_cast<long long>(i) * a.heads + h) * kHeadDim) + 2 * (tid & 7);
+      qv[0] = src[0];
+      qv[1] = src[1];
+    }
+    uint32_t* w = reinterpret_cast<uint32_t*>(qv);
 #pragma unroll
-    for (int c = 0; c < kPer; ++c) {
-      const int r = (tid >> 3) + 16 * c, row = row0 + r;
-      qv[c][0] = qv[c][1] = make_uint4(0, 0, 0, 0);
-      if (r < nrows) {
-        const int i = row / a.group, h = row - i * a.group;
-        const uint4* src = reinterpret_cast<const uint4*>(q_base + (static_cast<long long>(i) * a.heads + h) * kHeadDim) + 2 * (tid & 7);
-        qv[c][0] = src[0];
-        qv[c][1] = src[1];
-      }
-      uint32_t* w = reinterpret_cast<uint32_t*>(qv[c]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        w[e] = (w[e] & keep) ^ flip;
-        const uint32_t lo = (w[e] << 16) & 0x7FFF0000u, hi = w[e] & 0x7FFF0000u;
-        if (lo < 0x7F800000u) top = max(top, lo);
-        if (hi < 0x7F800000u) top = max(top, hi);
-      }
+    for (int e = 0; e < 8; ++e) {
+      w[e] = (w[e] & keep) ^ flip;
+      const uint32_t lo = (w[e] << 16) & 0x7FFF0000u, hi = w[e] & 0x7FFF0000u;
+      if (lo < 0x7F800000u) top = max(top, lo);
+      if (hi < 0x7F800000u) top = max(top, hi);
     }
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
     softmax_barrier();                                // the segment before has been read out
     if (lane == 0) reinterpret_cast<uint32_t*>(red)[sw] = top;
     if (tid < R) {
-      const int i = (row0 + tid) / a.group;
+      const int i = tid / a.group;
       lim_s[tid] = tid < nrows ? static_cast<int>(min(pos + i, 0x7FFFFFFFll)) : 0x7FFFFFFF;
     }
     softmax_barrier();
@@ -514,11 +507,9 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     // largest query in [128, 256): multiply by 2^e
     const int e = top == 0 ? 0 : min(max(134 - static_cast<int>(top >> 23), -120), 120);
     const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23), down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-#pragma unroll
-    for (int c = 0; c < kPer; ++c) {
-      const int r = (tid >> 3) + 16 * c, chunk = (tid & 7);
+    {
+      const int chunk = tid & 7;
       uint32_t hi[4], lo[4];
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(qv[c]);
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         uint32_t h2[2], l2[2];
@@ -549,7 +540,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
 #pragma unroll
     for (int r = 0; r < R; ++r) o[r] = l[r] = 0.0f;
     const long long head_scales = (b * a.kv_heads + kh) * a.scale_blocks;
-    const int lim_min = static_cast<int>(min(pos + i_min, 0x7FFFFFFFll));
+    const int lim_min = static_cast<int>(min(pos, 0x7FFFFFFFll));
     const long long written = pos + a.t;              // rows behind the last sequence position may hold anything
 
     // adds the product of the tile before: o = o * alpha + (D0 * vs0 + D1 * vs1) * beta / 256
@@ -740,10 +731,10 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
       my_max[lane] = total == 0.0f ? 0.0f : 1.0f / total;
     }
     __syncwarp();
-    const long long out_row = (b * a.t + i_min) * a.heads + static_cast<long long>(kh) * a.group;
+    const long long out_row = b * a.t * a.heads + static_cast<long long>(kh) * a.group;
     if (g.whole) {
-      int h = row0 - i_min * a.group;
-      __nv_bfloat16* dst = a.out + (out_row + h) * kHeadDim + tok;
+      int h = 0;
+      __nv_bfloat16* dst = a.out + out_row * kHeadDim + tok;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r < nrows) *dst = __float2bfloat16_rn(o[r] * my_max[r]);
@@ -751,7 +742,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
         dst += kHeadDim;
       }
     } else {
-      const long long slot = (static_cast<long long>(unit) * a.runs + run) * 2 + (first_s[b] + tile0 == run0 ? 0 : 1);
+      const long long slot = (static_cast<long long>(kh) * a.runs + run) * 2 + (first_s[b] + tile0 == run0 ? 0 : 1);
       float* dst = a.part + slot * R * kHeadDim + tok;
 #pragma unroll
       for (int r = 0; r < R; ++r)
@@ -1345,31 +1336,27 @@ struct AttnPlan { int rows, row_tiles, runs; };
 static AttnPlan attn_plan(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t ctx) {
   AttnPlan p;
   const int64_t rows = t * (heads / kv_heads), slots = 2 * static_cast<int64_t>(sm_count()), tiles = (ctx + 127) / 128;
-  p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-  p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
-  // Two CTAs fit an SM: as many runs as fill the device once, none shorter than four tiles of 128 positions (a CTA's set-up
-  // and its share of the join cost about what two tiles do).
-  const int64_t units = kv_heads * p.row_tiles;
-  int64_t runs = slots / units;
-  if (runs > batch * tiles / 4) runs = batch * tiles / 4;
-  p.runs = batch > kMaxFlat || batch * tiles > (1 << 30) || tiles <= 4 || runs < 2 ? 0 : static_cast<int>(runs);
-  if (rows <= 16) return p;
-  // More rows: the kernel with 128 of them per CTA, every sequence whole or in runs of its own, where it is the faster one.  Both
-  // take so many tenths of a microsecond for a tile: 14 (22 with a second CTA on the SM) for 128 rows, 26 for 32 of them; the join
-  // of the one's runs costs 5 us more and 0.3 for every 128 rows, that of the other's 10.  8 key heads with 4 heads each behind
-  // 8000 positions, 32 rows a CTA / 128 whole / 128 in runs: 9 tokens 21 / 88 / 16 us, 64 tokens 50 / 88 / 25, 256 tokens 170 / 90 /
-  // 65; four sequences of 128 tokens 370 / 90 / 116.
-  const int64_t many = batch * kv_heads * ((rows + 127) / 128), few = units * batch;
-  const int64_t time_few = 150 + 26 * (p.runs ? (batch * tiles + p.runs - 1) / p.runs : tiles * ((few + slots - 1) / slots));
-  const int64_t time_whole = 50 + tiles * (2 * many <= slots ? 14 : 22 * ((many + slots - 1) / slots));
+  if (rows <= 16) {
+    p.rows = rows <= 8 ? 8 : 16;
+    p.row_tiles = 1;
+    // Two CTAs fit an SM: as many runs as fill the device once, none shorter than four tiles of 128 positions (a CTA's set-up
+    // and its share of the join cost about what two tiles do).
+    int64_t runs = slots / kv_heads;
+    if (runs > batch * tiles / 4) runs = batch * tiles / 4;
+    p.runs = batch > kMaxFlat || batch * tiles > (1 << 30) || tiles <= 4 || runs < 2 ? 0 : static_cast<int>(runs);
+    return p;
+  }
+  // More rows: the kernel with 128 of them per CTA, every sequence whole or in runs of its own.  A tile takes a CTA 1.4 us, with a
+  // second one on the SM 2.2; runs cost 5 us and 0.3 for every 128 rows.  8 key heads with 4 heads each behind 8000 positions,
+  // whole / in runs: 9 tokens 88 / 16 us, 64 tokens 88 / 25, 256 tokens 90 / 65; four sequences of 128 tokens 90 / 116.
+  // (The other kernel with 32 rows takes 2.6 us a tile: 8 tokens of 16 sequences behind 4000 positions 60 us, here 48.)
+  const int64_t many = batch * kv_heads * ((rows + 127) / 128);
   int64_t split = slots / many;
   if (split > tiles / 4) split = tiles / 4;
-  const int64_t time_split = split < 2 ? time_whole + 1 : 100 + 3 * many + (tiles + split - 1) / split * (2 * many * split <= slots ? 14 : 22);
-  if (time_whole <= time_few || time_split <= time_few) {
-    p.rows = PfCfg::kRows;
-    p.row_tiles = static_cast<int>((rows + 127) / 128);
-    p.runs = time_whole <= time_split ? 0 : static_cast<int>(split);
-  }
+  const int64_t whole = 50 + tiles * (2 * many <= slots ? 14 : 22 * ((many + slots - 1) / slots));
+  p.rows = PfCfg::kRows;
+  p.row_tiles = static_cast<int>((rows + 127) / 128);
+  p.runs = split >= 2 && 100 + 3 * many + (tiles + split - 1) / split * (2 * many * split <= slots ? 14 : 22) < whole ? static_cast<int>(split) : 0;
   return p;
 }
 
@@ -1513,6 +1500,5 @@ extern "C" int plq_fp8_attention(const void* q_bf16, const void* k_codes, const 
   if ((st = make_cache_tmap(&mk, k_codes, batch, t_max, kv_heads, box)) != PLQ_OK) return st;
   if ((st = make_cache_tmap(&mv, v_codes, batch, t_max, kv_heads, box)) != PLQ_OK) return st;
   if (p.rows >= 128) return p.runs ? launch_prefill<true>(mk, mv, a, stream) : launch_prefill<false>(mk, mv, a, stream);
-  if (p.rows == 8) return launch_attention<8>(mk, mv, a, stream);
-  return p.rows == 16 ? launch_attention<16>(mk, mv, a, stream) : launch_attention<32>(mk, mv, a, stream);
+  return p.rows == 8 ? launch_attention<8>(mk, mv, a, stream) : launch_attention<16>(mk, mv, a, stream);
 }
