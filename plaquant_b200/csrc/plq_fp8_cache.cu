@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(256, 4) rope_kv_append_fp8_kernel(const Fp8App
 // sequence); a sequence that lies in several runs leaves partial sums, at most two per run (its first and its last segment),
 // which fp8_attention_join_kernel adds in a fixed order.
 // Bound by the cache's bytes for long ones: one sequence of 131072 positions (64 heads on 8) 52 us, 5.1 TB/s; 16 of 4096 (32 on 8)
-// 32 us, 4.2 TB/s, and 25 us of different lengths.  A tile is a chain of some 2000 cycles for a CTA (scores, maxima over the
+// 31 us, 4.3 TB/s, and 24 us of different lengths.  A tile is a chain of some 2000 cycles for a CTA (scores, maxima over the
 // lanes, weights, product), which two CTAs per SM turn into the memory's rate; about 2.5 us before the first tile and 4 us for
 // the join come on top, which is what a short cache consists of (1 x 4096: 9.4 us).  A join in the kernel itself by the
 // last CTA of a sequence took 64 and 36 us: its counters are six round trips to L2.
@@ -228,13 +228,14 @@ struct Fp8AttnArgs {
   const float* k_scale;        // [batch, kv_heads, scale_blocks]
   const float* v_scale;
   __nv_bfloat16* out;          // [batch, t, heads, 128]
-  float* part;                 // [units][runs][2][R][128] sums, then [units][runs][2][R][2] (maximum, weight)
+  float* part;                 // [units][runs][2][R][128] sums, then [units][runs][2][R][2] (maximum, weight); fp8_prefill_kernel:
+                               // [batch][units][runs][128][128], [batch][units][runs][128][2].  A unit is a row tile of a key head
   const long long* pos_dev;
   long long pos, t_max;
   int* status;
   float scale_log2;            // scale * log2(e)
   int batch, t, heads, kv_heads, group, pos_batch, scale_blocks, row_tiles;
-  int runs;                    // runs of the row of tiles, or 0: one CTA per sequence
+  int runs;                    // runs of the row of tiles (fp8_prefill_kernel: of each sequence), or 0: one CTA per sequence
 };
 
 // Tiles of 128 positions that sequence b has (0: it sits out, or does not fit).
