@@ -71,13 +71,17 @@ __device__ __forceinline__ void tc_mma_e4m3(uint32_t d_tmem, uint32_t a_lo, uint
                  "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// The same with A in tensor memory: row = lane, four consecutive elements of K per 32-bit column.
-__device__ __forceinline__ void tc_mma_e4m3_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 db, {%2, %3};\n\t"
-               "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], db, %4, p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc),
-               "r"(accumulate) : "memory");
-}
 constexpr uint32_t kIdescAE5m2 = 1u << 7;              // A as E5M2 instead of E4M3
+// The same with A in tensor memory (row = lane, four consecutive elements of K per 32-bit column), block-scaled (descriptor:
+// make_idesc): every row of A and of B has an E8M0 scale for the 32 elements of K, byte 0 of the
+// word that 512 bytes copied to these columns put there (row r: lane r % 32, column r / 32).
+__device__ __forceinline__ void tc_mma_mxf8_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t sfa_tmem,
+                                               uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %7, 0;\n\tmov.b64 db, {%2, %3};\n\t"
+               "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], [%1], db, %4, [%5], [%6], p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo),
+               "r"(b_hi), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate) : "memory");
+}
+constexpr uint32_t kIdescBMnMajor = 1u << 16;          // N contiguous instead of K
 
 // 16 consecutive 32-bit columns of a warp's 32 lanes
 __device__ __forceinline__ void tc_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {

@@ -774,7 +774,8 @@ struct PfCfg {
   static constexpr int kTile = 128 * kHeadDim;          // 16 KiB
   static constexpr int kBlock = kCacheBlock * kHeadDim; // 8 KiB: 64 positions of K or V
   static constexpr int kStages = 4;
-  static constexpr size_t kSmemBytes = 1024 + 2 * kTile + 2 * kStages * kBlock + 256;
+  static constexpr int kScaleBytes = 512;               // 128 rows, a word each
+  static constexpr size_t kSmemBytes = 1024 + 2 * kTile + 2 * kStages * kBlock + 3 * kScaleBytes + 256;
   // 128 registers a thread at launch (256 x 128); the warps with a row of scores per thread take what the others leave.
   static constexpr int kRegsMain = 56, kRegsRows = 200;
   static_assert(128 * kRegsMain + 128 * kRegsRows <= 256 * 128, "register split");
@@ -881,12 +882,17 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
 //          for what is at least 2^-10 of that, off by 2^-18 of it below
 //   S      of 64 positions, twice in tensor memory: the product of block j + 2 is issued behind the one that reads the weights
 //          of block j, so the scores of j + 1 lie ready when the weights of j are done
-//   p      hi + lo, E4M3 + E5M2, in tensor memory (A operand), in the place of the scores they come from: off by at most 2^-8
-//          of itself, or by 2^-14 below 2^-6 (the row's largest is 4 to 256): E4M3 leaves up to 2^-10 there, and E5M2 half of
-//          2^-3 of that
-//   O      stays in tensor memory.  The scale of a block of V is part of the weight's exponent: w = exp2(score + log2 vs - M + 2),
-//          with M within 2^6 of the row's largest such sum so far (only beyond that is O scaled, which is rare), and the sum of
-//          the weights takes w / vs.  So a block of large values that nobody looks at does not set the scale of the others.
+//   p      w = exp2(score + log2 vs - e + 8) with e the row's largest score + log2 vs in the block of 64, rounded up: the scale of
+//          V is part of the weight, and the block's largest is 128 to 256.  hi + lo, E4M3 + E5M2, in tensor memory (A operand),
+//          in the place of the scores they come from: off by at most 2^-8 + 2^-11 (f16 on the way) of itself, or by 2^-14
+//          below 2^-6: E4M3 leaves up to 2^-10 there, and E5M2 half of 2^-3 of that.  All steps of a block are 2^-15 of its
+//          largest.
+//   O      stays in tensor memory, in units of 2^R, R = e - 8 of the first block.  The tensor core applies 2^(e - 8 - R), an E8M0
+//          scale per row and 32 positions (kind::mxf8f6f4), so no block's weights share an exponent with another's: a long tail of
+//          small weights keeps its bits behind a position that outweighs each of them, and ordinary values behind a block of
+//          large ones.  (With one running exponent for the row, weights 12 nats below it were off by up to 24 %, beyond 13 nats
+//          by 69 % or gone; moving it down with the blocks cost a rescaling of O for 20 to 27 % of the time.)  R moves only when a
+//          block is 2^60 above it.  The sum of the weights takes w / vs.
 //   warp 0 producer, warp 1 MMA issuer, warps 4 - 7 the rows
 // 128 positions of two row tiles are 2048 cycles of the tensor core (four products of 128 x 128 x 128 each) and as many of
 // exponentials (16 a cycle).  They take 2.2 us (about 4000 cycles): without the weights' arithmetic 1.2 us, with exponentials
@@ -898,7 +904,9 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
 // (the next queries prepared meanwhile by two warps) was slower, 110 us: two warps take longer for that than the tiles before.
 // Few CTAs and a long past: each sequence is cut into runs, whose sums O and weight at their M go to the join (64 tokens of 32
 // heads on 8 behind 8000 positions 88 -> 25 us).
-constexpr float kHeadroom = 6.0f;                       // log2 of how far a weight may exceed that of M
+constexpr int kScaleBias = 127 - 8;                     // e - R = 8 is the scale one
+constexpr int kScaleTop = 127 + 60;                     // beyond it R moves: O stays below 2^60 * 2^8 * 448 * positions
+constexpr float kFarBelow = 92.0f;                      // blocks further below R than this share its scale, 2^-100
 
 // RUNS: every sequence in a.runs runs of its own, for the join; as a branch it would cost the other calls 4 %
 template <bool RUNS>
@@ -910,7 +918,9 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
   uint8_t* q_s = smem;                                  // [hi | lo][128 x 128 bytes]
   uint8_t* k_s = q_s + 2 * C::kTile;
   uint8_t* v_s = k_s + C::kStages * C::kBlock;
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(v_s + C::kStages * C::kBlock);
+  uint8_t* w_scale_s = v_s + C::kStages * C::kBlock;    // scales of the weights of two blocks
+  uint8_t* one_s = w_scale_s + 2 * C::kScaleBytes;      // ... of V: one
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(one_s + C::kScaleBytes);
   uint64_t* k_empty = k_full + C::kStages, *v_full = k_empty + C::kStages, *v_empty = v_full + C::kStages;
   uint64_t* q_full = v_empty + C::kStages, *s_full = q_full + 1, *p_full = s_full + 2, *o_done = p_full + 2, *o_full = o_done + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_full + 1);
@@ -931,6 +941,8 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
     tmem_alloc<1>(tmem_holder, 256);
     tmem_relinquish<1>();
   }
+  if (warp == 2) reinterpret_cast<uint4*>(one_s)[lane] = make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -979,7 +991,7 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
     }
   } else if (warp == 1) {
     if (elect_one() && n > 0) {
-      constexpr uint32_t idesc_s = make_idesc_e4m3(128, 64), idesc_o = make_idesc_e4m3(128, 128, false, true);
+      constexpr uint32_t idesc_s = make_idesc_e4m3(128, 64), idesc_o = make_idesc(0u /*E4M3*/, 128, 128, 1u /*E8M0*/) | kIdescBMnMajor;
       bool ok = true;
       auto scores = [&](int j) {
         const int st = j % C::kStages;
@@ -1002,10 +1014,12 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
         if (!ok) break;
         tc_fence_after();
         const uint32_t v_lo = desc_lo_sw128(v_base + st * C::kBlock), p = tmem_base + 64 * (j & 1), o = tmem_base + 128;
+        tc_cp_32x128b_warpx4<1>(p + 32, desc_lo_sf(smem_u32(w_scale_s + (j & 1) * C::kScaleBytes)), kDescHiSf);
+        tc_cp_32x128b_warpx4<1>(p + 36, desc_lo_sf(smem_u32(one_s)), kDescHiSf);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                   // 32 positions each: codes of hi, then of lo
-          tc_mma_e4m3_ts(o, p + 16 * h, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, j > 0 || h > 0);
-          tc_mma_e4m3_ts(o, p + 16 * h + 8, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o | kIdescAE5m2, 1u);
+          tc_mma_mxf8_ts(o, p + 16 * h, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, p + 32, p + 36, j > 0 || h > 0);
+          tc_mma_mxf8_ts(o, p + 16 * h + 8, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o | kIdescAE5m2, p + 32, p + 36, 1u);
         }
         tc_commit<1>(smem_u32(&v_empty[st]));
         tc_commit<1>(smem_u32(j + 1 == n ? o_full : o_done));
@@ -1112,7 +1126,8 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
     const float per_k = down * (a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2));
     const int lim = real ? written - a.t + i : written - 1;                             // last position the row sees
     const int lim_min = written - a.t + row0 / a.group;                       // ... of any row of the tile
-    float M = 0.0f, weight = 0.0f;
+    float R = 0.0f, weight = 0.0f;
+    const uint32_t scale_at = smem_u32(w_scale_s) + lane * 16 + quad * 4;
     bool ok = true;
     float next_k = 1.0f, next_v = 1.0f;
     auto fetch = [&](int j) {
@@ -1151,16 +1166,17 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
 #pragma unroll
       for (int d = 4; d < 32; ++d) m[d & 3] = fmaxf(m[d & 3], fmaxf(__uint_as_float(v[0][d]), __uint_as_float(v[1][d])));
       const float t_max = fmaf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), ck, lv);
+      float e = ceilf(t_max);
       if (j == 0) {
-        M = t_max > kNegInf ? t_max : 0.0f;
+        R = e > kNegInf ? e - 8.0f : 0.0f;
       } else {
-        const bool grow = t_max > M + kHeadroom;
-        if (__any_sync(0xFFFFFFFFu, grow)) {
+        const bool far = e - R > static_cast<float>(kScaleTop - kScaleBias);
+        if (__any_sync(0xFFFFFFFFu, far)) {
           ok = mbar_wait_bounded_lanes(o_done, (j - 1) & 1u, abort_flag);        // the product of the block before is in O
           if (!ok) break;
           tc_fence_after();
-          const float alpha = grow ? ex2_approx(M - t_max) : 1.0f;
-          if (grow) M = t_max;
+          const float alpha = far ? ex2_approx(R + 8.0f - e) : 1.0f;
+          if (far) R = e - 8.0f;
           weight *= alpha;
 #pragma unroll 1
           for (int c = 0; c < 8; ++c) {
@@ -1182,10 +1198,13 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
 #pragma unroll
           for (int c = 0; c < 4; ++c) dst[c] = make_uint4(0, 0, 0, 0);
         }
-        fence_proxy_async_smem();
       }
+      e = fmaxf(e, R - kFarBelow);                      // a number whatever the scores are
+      const uint32_t ws = static_cast<uint32_t>(max(1, min(__float2int_rn(e - R) + kScaleBias, kScaleTop)));
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(scale_at + (j & 1) * C::kScaleBytes), "r"(ws) : "memory");
+      fence_proxy_async_smem();
       // A block that the row sees and whose scale is NaN makes the row NaN, its masked positions included.
-      const float shift = lv + (8.0f - kHeadroom) - M;
+      const float shift = lv + 8.0f - e;
       const float2 ck2 = make_float2(ck, ck), shift2 = make_float2(shift, shift);
       float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -1207,7 +1226,7 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
         }
         tc_st_32x32b_x16(sp_at + 16 * c, p);            // columns of S that have been read
       }
-      weight = fmaf(sum.x + sum.y, inv_v, weight);
+      weight = fmaf(sum.x + sum.y, inv_v * __uint_as_float(ws << 23), weight);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -1238,8 +1257,8 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
                          "r"(v[d + 4]), "r"(v[d + 5]), "r"(v[d + 6]), "r"(v[d + 7]) : "memory");
         }
       }
-      if (real && !idle)                                // weights are in units of exp2(M + 2 - headroom), see above
-        *reinterpret_cast<float2*>(a.part + a.batch * units * a.runs * C::kRows * kHeadDim + 2 * slot) = make_float2(M - (8.0f - kHeadroom), weight);
+      if (real && !idle)                                // both in units of 2^R
+        *reinterpret_cast<float2*>(a.part + a.batch * units * a.runs * C::kRows * kHeadDim + 2 * slot) = make_float2(R, weight);
       tc_fence_before();
     }
     // ---- or the result: by way of the queries' memory, so that the stores are whole lines ----
