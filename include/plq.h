@@ -421,7 +421,8 @@ PLQ_API int plq_rope_kv_append_fp8(const void* qkv_bf16, int64_t ld, const void*
  * out = softmax(scale * q . k) v, head h reading key head h / (heads / kv_heads).  pos as above; a sequence with a negative
  * position sees nothing, one with pos + t > t_max is reported (PLQ_DEV_RANGE); their outputs are zeros.
  *   ctx            an upper bound of pos + t over the sequences (t_max where it is not known): how the work is split
- *   workspace      plq_fp8_attention_workspace_bytes(...) bytes (0 where the work is not cut along the positions), used by this call only
+ *   workspace      plq_fp8_attention_workspace_bytes(...) bytes (0 where the work is not cut along the positions), 16-byte aligned, used by
+ *                  this call only
  * Codes of visible positions have to be finite, as the append writes them; the others may hold anything.
  */
 PLQ_API int64_t plq_fp8_attention_workspace_bytes(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t ctx);

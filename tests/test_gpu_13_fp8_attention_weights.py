@@ -147,3 +147,28 @@ def test_blocks_of_zeros_leave_the_others(plq):
         cache.v.zero_()
         cache.v_scale.fill_(2.0 ** -100)
         assert torch.all(plq.ops.fp8_cache_attention(q, cache, n - t) == 0)
+
+
+@pytest.mark.parametrize("b,t,heads,kv_heads,n", [(1, 9, 8, 2, 9000), (1, 64, 32, 8, 8000), (3, 40, 10, 2, 5000), (2, 1, 16, 2, 5000), (1, 4, 16, 4, 3000)])
+def test_a_workspace_needs_no_more_than_sixteen_bytes_of_alignment(plq, b, t, heads, kv_heads, n):
+    """Workspaces at 0 and at 16 behind a multiple of 32: the same result, and nothing outside them is written."""
+    from plaquant_b200 import _lib
+    g = torch.Generator(device="cuda").manual_seed(n)
+    cache = _cache(plq, b, n, kv_heads, torch.randn(n, 128, generator=g, device="cuda"), torch.randn(n, 128, generator=g, device="cuda"),
+                   torch.ones(-(-n // BLOCK), device="cuda"), torch.ones(-(-n // BLOCK), device="cuda"))
+    q = torch.randn(b, t, heads, 128, generator=g, device="cuda").to(torch.bfloat16)
+    want = plq.ops.fp8_cache_attention(q, cache, n - t)
+    lib, status = _lib.lib(), plq.ops.status_word("cuda")
+    need = lib.plq_fp8_attention_workspace_bytes(b, t, heads, kv_heads, n)
+    assert need > 0
+    for shift in (0, 16):
+        room = torch.full((need + 128,), 0xA5, dtype=torch.uint8, device="cuda")
+        at = (room.data_ptr() + 63) // 32 * 32 + shift
+        out = torch.empty_like(q)
+        st = lib.plq_fp8_attention(q.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(), b, t, heads,
+                                   kv_heads, n, None, 0, n - t, n, 128 ** -0.5, out.data_ptr(), at, need, status.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert st == 0
+        torch.cuda.synchronize()
+        first = at - room.data_ptr()
+        assert torch.equal(out, want) and torch.all(room[:first] == 0xA5) and torch.all(room[first + need:] == 0xA5)
+    plq.check_device_status()
