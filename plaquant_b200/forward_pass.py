@@ -417,7 +417,7 @@ class ResQForwardB200:
         if pos0 == 0:
             self.kv[li] = kv_cache.Fp8Cache.empty(b, -(-need // 64) * 64 + 64, self.kv_heads, self.device)
         cache = self.kv[li]
-        if not isinstance(cache, kv_cache.Fp8Cache) or cache.room < pos0:
+        if not isinstance(cache, kv_cache.Fp8Cache) or not 0 <= pos0 <= (cache.room if cache.length is None else cache.length):
             raise RuntimeError(f"the cache of layer {li} does not hold the {pos0} positions in front of the new ones")
         if cache.room < need:
             cache = self.kv[li] = cache.grown(-(-(need + min(256, max(64, need // 8))) // 64) * 64)

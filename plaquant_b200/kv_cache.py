@@ -12,6 +12,7 @@ Hadamard (`rotate_heads`), which leaves q . k unchanged up to quantisation error
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional
 
 import torch
 
@@ -86,18 +87,23 @@ CACHE_BLOCK = 64        # positions that share a scale of an Fp8Cache
 class Fp8Cache:
     """Keys and values of one layer in E4M3, `room` positions for each sequence of a batch, heads of 128.  One scale per
     64 positions and head, a power of two: value = code * scale.  Positions nobody has written may hold anything.
-    ops.rope_kv_append_fp8 fills it in place, ops.fp8_cache_attention reads it; 1.03 bytes per 2 of a bf16 cache."""
+    ops.rope_kv_append_fp8 fills it in place, ops.fp8_cache_attention reads it; 1.03 bytes per 2 of a bf16 cache.
+
+    `length`: how many leading positions the host knows to be written.  An append at a host position within them moves it, one
+    at positions in device memory makes it None (as many as the caller knows of); what reads the cache by host positions, as the
+    decoder does, refuses to begin behind it."""
     k: torch.Tensor           # u8 [B, room, kv_heads, 128]
     k_scale: torch.Tensor     # float32 [B, kv_heads, ceil(room / 64)]
     v: torch.Tensor
     v_scale: torch.Tensor
+    length: Optional[int] = None
 
     @classmethod
     def empty(cls, batch: int, room: int, kv_heads: int, device) -> "Fp8Cache":
         def side():
             return (torch.empty(batch, room, kv_heads, HEAD_DIM, dtype=torch.uint8, device=device),
                     torch.empty(batch, kv_heads, -(-room // CACHE_BLOCK), dtype=torch.float32, device=device))
-        return cls(*side(), *side())
+        return cls(*side(), *side(), 0)
 
     @property
     def batch(self) -> int:
@@ -125,7 +131,7 @@ class Fp8Cache:
                 raise RuntimeError(f"cache.{name} is on {c.device}, the call on {device}")
 
     def clone(self) -> "Fp8Cache":
-        return Fp8Cache(self.k.clone(), self.k_scale.clone(), self.v.clone(), self.v_scale.clone())
+        return Fp8Cache(self.k.clone(), self.k_scale.clone(), self.v.clone(), self.v_scale.clone(), self.length)
 
     def grown(self, room: int) -> "Fp8Cache":
         """A cache with room for `room` positions (at least this one's) that holds what this one does."""
@@ -133,13 +139,21 @@ class Fp8Cache:
         new.copy_from(self, self.room)
         return new
 
+    def appended(self, pos, t: int) -> None:
+        """Notes that `t` positions from `pos` on (an int, or a tensor of positions) have been written."""
+        if isinstance(pos, torch.Tensor):
+            self.length = None
+        elif self.length is not None and 0 <= pos <= self.length:
+            self.length = max(self.length, pos + t)
+
     def copy_from(self, other: "Fp8Cache", t: int) -> None:
-        """Takes over the first `t` positions of another cache."""
+        """Takes over the first `t` positions of another cache; what this one held behind them is no longer part of it."""
         blocks = -(-t // CACHE_BLOCK)
         for dst, src in ((self.k, other.k), (self.v, other.v)):
             dst[:, :t].copy_(src[:, :t])
         for dst, src in ((self.k_scale, other.k_scale), (self.v_scale, other.v_scale)):
             dst[..., :blocks].copy_(src[..., :blocks])
+        self.length = None if other.length is None else min(t, other.length)
 
     def values(self, t: int):
         """bf16 keys and values [B, t, kv_heads, 128] of the first `t` positions."""

@@ -608,6 +608,7 @@ def rope_kv_append_fp8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
     q = None if word is None else _lib.torch_lib().rope_kv_append_fp8(qkv, cos, sin, heads, kv_heads, cache.k, cache.k_scale, cache.v,
                                                                       cache.v_scale, at, pos if at is None else 0, word)
     if q is not None:
+        cache.appended(pos, qkv.shape[1])
         return q
     _require_cuda(qkv, "qkv")
     b, t, n = qkv.shape
@@ -627,6 +628,7 @@ def rope_kv_append_fp8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, 
             _ptr(cache.k_scale), _ptr(cache.v), _ptr(cache.v_scale), cache.room, ptr, each, host, _ptr(status_word(qkv.device)),
             _stream(qkv.device))
     _lib.check(st)
+    cache.appended(pos, t)
     return q
 
 

@@ -1,0 +1,54 @@
+"""The decoder on the E4M3 cache and head: positions it does not hold, and what the options leave on the device."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def plq():
+    import plaquant_b200
+    return plaquant_b200
+
+
+def _config(**kw):
+    from plaquant_b200.forward_pass import LlamaConfig
+    return LlamaConfig(**{**dict(hidden_size=512, intermediate_size=1024, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=128, vocab_size=1003), **kw})
+
+
+def _ids(cfg, b, t, seed=1):
+    return torch.randint(0, cfg.vocab_size, (b, t), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def test_a_gap_behind_the_prompt_is_refused(plq):
+    from plaquant_b200.forward_pass import ResQForwardB200
+    cfg = _config()
+    m = ResQForwardB200(cfg, "cuda", seed=6, kv_quant="fp8")
+    ids = _ids(cfg, 2, 40)
+    m.forward(ids[:, :20])
+    assert [c.length for c in m.kv] == [20, 20] and m.kv[0].room > 30
+    for pos0 in (21, 30, -1):
+        with pytest.raises(RuntimeError):
+            m.forward(ids[:, 20:21], pos0=pos0)
+    kept = [c.clone() for c in m.kv]
+    a = m.forward(ids[:, 20:30], pos0=20)
+    assert m.kv[0].length == 30
+    m.kv = kept
+    assert torch.equal(m.forward(ids[:, 20:30], pos0=20), a)
+    again = m.forward(ids[:, 20:30], pos0=20)             # the same positions once more
+    assert again.isfinite().all() and m.kv[1].length == 30
+    plq.check_device_status()
+
+
+def test_the_append_keeps_the_length(plq):
+    from plaquant_b200 import kv_cache
+    cache = kv_cache.Fp8Cache.empty(1, 100, 1, "cuda")
+    qkv, one = torch.ones(1, 5, 3 * 128, dtype=torch.bfloat16, device="cuda"), torch.ones(5, 128, device="cuda")
+    plq.ops.rope_kv_append_fp8(qkv, one, one, 1, 1, cache, 0)
+    plq.ops.rope_kv_append_fp8(qkv, one, one, 1, 1, cache, 5)
+    assert cache.length == 10
+    with pytest.raises(plq.PlqError):
+        plq.ops.rope_kv_append_fp8(qkv, one, one, 1, 1, cache, 96)
+    assert cache.length == 10
+    plq.ops.rope_kv_append_fp8(qkv, one, one, 1, 1, cache, torch.tensor([10], device="cuda"))
+    assert cache.length is None
