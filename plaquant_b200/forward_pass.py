@@ -538,10 +538,7 @@ class ResQForwardB200:
         t = input_ids.shape[1]
         h, delta = self._run_layers(h, pos0, self._rope_rows(pos0, t), last_only=not all_positions)
         self.pos = pos0 + input_ids.shape[1]
-        if not all_positions and isinstance(delta, torch.Tensor):
-            h, delta = h[:, -1:], delta[:, -1:]
-        logits = self._head(h, delta)
-        return logits if all_positions else logits[:, -1]
+        return self._head(h, delta, last_only=not all_positions)
 
     def _prefill_scattered(self, input_ids: torch.Tensor, all_positions: bool) -> torch.Tensor:
         """Prefill with the residual stream sharded by rows (sequence-parallel between the linears).  Rank r keeps
@@ -577,12 +574,17 @@ class ResQForwardB200:
             return self._logits(full.view(b, t, -1))
         return self._logits(gather_last_positions(h, b, t, self.ctx.rank, self.ctx.size, self.ctx.group))
 
-    def _head(self, h: torch.Tensor, delta) -> torch.Tensor:
-        """Logits of the rows of a residual stream whose last MLP output has not been added to it yet."""
+    def _head(self, h: torch.Tensor, delta, last_only: bool = False) -> torch.Tensor:
+        """Logits [B, T, vocab] of a residual stream [B, T, hidden] whose last MLP output has not been added to it yet, or
+        those of the last position alone, [B, vocab]: norm and head then run on that many rows, wherever the output waits."""
+        if last_only and isinstance(delta, torch.Tensor):
+            h, delta = h[:, -1:], delta[:, -1:]
         if self.head8 is not None and isinstance(delta, torch.Tensor) and h.dtype == torch.bfloat16:
             _, p = ops.add_rmsnorm_fp8_pack(delta, h, self.final_norm, self.cfg.rms_eps)
-            return self.head8(p, out_dtype=torch.float32).view(*h.shape[:-1], -1)
-        return self._logits(self._finish(h, delta))
+            logits = self.head8(p, out_dtype=torch.float32).view(*h.shape[:-1], self.head8.out_features)
+            return logits[:, -1] if last_only else logits
+        h = self._finish(h, delta)
+        return self._logits(h[:, -1] if last_only else h)
 
     def _logits(self, h_last: torch.Tensor) -> torch.Tensor:
         """Final norm + LM head for rows [..., hidden]: in the model dtype (inference/forward_pass.py:178-181 in the reference)
@@ -656,7 +658,7 @@ class ResQForwardB200:
             h = F.embedding(tok, self.embed)
             cos_sin = self._rope_angles(st["pos"].to(torch.float32))
             h, delta = self._run_layers(h, 0, cos_sin, static=st)
-            tok.copy_(self._head(h, delta)[:, -1].argmax(-1, keepdim=True))
+            tok.copy_(self._head(h, delta, last_only=True).argmax(-1, keepdim=True))
             st["pos"].add_(1)
             step_idx.add_(1)
 
