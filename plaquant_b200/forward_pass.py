@@ -157,8 +157,7 @@ class ResQForwardB200:
         self._decode_states: Dict[tuple, _DecodeState] = {}
         # keys go into the cache as NVFP4 (Hadamard over the head dimension, per-head rows), queries get the same
         # rotation: the reference's QKRotationWrapper with k_had (promix/quantize/kv_quant.py:244-279)
-        if kv_quant not in (False, True, "fp8", "fake"):
-            raise ValueError(f"kv_quant is False, True, 'fp8' or 'fake', not {kv_quant!r}")
+        self._check_kv_quant(kv_quant)
         self.kv_quant = kv_quant                     # ... | "fake" (the packed rows' bf16 values)
         if kv_quant and c.head_dim != 128:
             raise ValueError("kv_quant needs head_dim = 128 (one Hadamard block per head)")
@@ -172,6 +171,13 @@ class ResQForwardB200:
         # packed rows in one kernel over peer memory instead of an NCCL all-reduce of bf16
         self.scatter = (tp.ScatterReduce(scatter_prefill_rows, c.hidden_size, self.k_hi_hidden, self.device, self.ctx.group)
                         if scatter_prefill_rows > 0 and self.ctx.size > 1 else None)
+
+    @staticmethod
+    def _check_kv_quant(kv_quant) -> None:
+        """Whatever is false is the bf16 cache and whatever else is true the packed rows; names of 8-bit forms that do not exist
+        are refused."""
+        if isinstance(kv_quant, str) and kv_quant.startswith("fp") and kv_quant != "fp8":
+            raise ValueError(f"kv_quant is False, True, 'fp8' or 'fake', not {kv_quant!r}")
 
     def __getstate__(self):
         return {**self.__dict__, "_kv_room": []}         # weak references: a copy's first append copies its cache
@@ -449,7 +455,7 @@ class ResQForwardB200:
         layer's attention nothing reads the other rows, and o_proj, norms and the MLP work row by row."""
         delta, c, chunk = None, self.cfg, {}
         b, t, _ = h.shape
-        native = (self.ctx.size == 1 and c.head_dim == 128 and self.kv_quant in (False, True) and 0 < b * t <= NATIVE_LAYER_ROWS
+        native = (self.ctx.size == 1 and c.head_dim == 128 and self.kv_quant not in ("fp8", "fake") and 0 < b * t <= NATIVE_LAYER_ROWS
                   and (t == 1 or pos0 == 0 or t * (pos0 + t) <= CHUNK_MASK_ELEMENTS)
                   and h.dtype == torch.bfloat16 and h.is_contiguous())
         if native:

@@ -94,3 +94,14 @@ def test_an_append_with_a_gap_leaves_the_length():
     cache.appended(0, 4)
     cache.appended(4, 10)
     assert cache.length == 14
+
+
+@pytest.mark.parametrize("value", [False, True, None, 0, 1, 2, "", "fp8", "fake", "nvfp4"])
+def test_forms_of_the_cache_that_were_accepted_before(value):
+    forward_pass.ResQForwardB200._check_kv_quant(value)
+
+
+@pytest.mark.parametrize("value", ["fp9", "fp4", "fp8_e5m2"])
+def test_forms_of_the_cache_that_do_not_exist(value):
+    with pytest.raises(ValueError):
+        forward_pass.ResQForwardB200._check_kv_quant(value)

@@ -52,3 +52,20 @@ def test_the_append_keeps_the_length(plq):
     assert cache.length == 10
     plq.ops.rope_kv_append_fp8(qkv, one, one, 1, 1, cache, torch.tensor([10], device="cuda"))
     assert cache.length is None
+
+
+@pytest.mark.parametrize("value,same_as", [(None, False), (0, False), (1, True), ("nvfp4", True)])
+def test_other_words_for_the_older_caches(plq, monkeypatch, value, same_as):
+    """None and other false values are the bf16 cache, other true ones the packed rows, on the same native call."""
+    from plaquant_b200 import _lib
+    from plaquant_b200.forward_pass import ResQForwardB200
+    cfg, calls = _config(), []
+    front = _lib.torch_lib()
+    layer = front.decoder_layer
+    monkeypatch.setattr(front, "decoder_layer", lambda *a: (calls.append(1), layer(*a))[1])
+    ids, got = _ids(cfg, 2, 30), []
+    for v in (value, same_as):
+        m = ResQForwardB200(cfg, "cuda", seed=6, kv_quant=v)
+        got.append((m.forward(ids[:, :29]), m.forward(ids[:, 29:], pos0=29), m.generate(ids, 5), m.kv_quant))
+        assert len(calls) % 2 == 0 and calls
+    assert all(torch.equal(x, y) for x, y in zip(got[0][:3], got[1][:3])) and got[0][3] is value
