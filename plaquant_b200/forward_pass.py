@@ -118,7 +118,7 @@ class ResQForwardB200:
 
         `kv_quant`: False (bf16 cache), True (packed NVFP4 rows), "fp8" (E4M3 with a scale per 64 positions and head, read
         by the package's own attention), "fake" (the NVFP4 rows' bf16 values).  `fp8_head`: the LM head in E4M3, the last
-        residual add and the final norm in its quantiser; logits are float32 sums."""
+        residual add and the final norm in its quantiser; logits are float32 sums, and `lm_head` is then in host memory."""
         self.cfg, self.device, self.ctx = cfg, torch.device(device), ctx or tp.TPContext()
         c, r, s = cfg, self.ctx.rank, self.ctx.size
         assert c.num_heads % s == 0 and c.num_kv_heads % s == 0 and c.intermediate_size % (s * 128) == 0
@@ -152,6 +152,7 @@ class ResQForwardB200:
                 self.lm_head = (torch.randn(c.vocab_size, c.hidden_size, generator=g, device=self.device) * 0.02).to(torch.bfloat16)
         if fp8_head:
             self.head8 = Fp8Linear.from_weight(self.lm_head)
+            self.lm_head = self.lm_head.cpu()            # for packed_state() alone: the device keeps the codes, half of its bytes
         self.kv: List[Tuple[torch.Tensor, torch.Tensor]] = []
         self.pos = 0
         self._decode_states: Dict[tuple, _DecodeState] = {}

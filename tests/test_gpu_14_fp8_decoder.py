@@ -69,3 +69,23 @@ def test_other_words_for_the_older_caches(plq, monkeypatch, value, same_as):
         got.append((m.forward(ids[:, :29]), m.forward(ids[:, 29:], pos0=29), m.generate(ids, 5), m.kv_quant))
         assert len(calls) % 2 == 0 and calls
     assert all(torch.equal(x, y) for x, y in zip(got[0][:3], got[1][:3])) and got[0][3] is value
+
+
+def test_the_quantised_head_takes_the_place_of_the_other(plq, tmp_path):
+    """Half of the bytes stay on the device; the container written from such a model holds the head as it was."""
+    from plaquant_b200 import weight_packer
+    from plaquant_b200.forward_pass import ResQForwardB200
+    cfg = _config(vocab_size=40000)
+    ids, sizes, models = _ids(cfg, 2, 20), [], []
+    for fp8_head in (False, True):
+        before = torch.cuda.memory_allocated()
+        models.append(ResQForwardB200(cfg, "cuda", seed=6, fp8_head=fp8_head))
+        sizes.append(torch.cuda.memory_allocated() - before)
+    plain, m = models
+    head = 40000 * 512
+    assert sizes[0] - sizes[1] >= head - head // 1024 - 4096 and m.lm_head.device.type == "cpu"
+    assert torch.equal(m.lm_head, plain.lm_head.cpu())
+    state = weight_packer.read_packed(weight_packer.save_packed(m, str(tmp_path / "m.pt")))
+    again = ResQForwardB200(cfg, "cuda", packed=state, fp8_head=True)
+    assert torch.equal(again.forward(ids), m.forward(ids)) and again.lm_head.device.type == "cpu"
+    assert torch.equal(ResQForwardB200(cfg, "cuda", packed=state).forward(ids), plain.forward(ids))
