@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(256, 4) rope_kv_append_fp8_kernel(const Fp8App
 // is the sum of two E4M3 numbers, which are two sets of columns of one product:
 //   q      hi + lo / 16 (4 + 4 significant bits: exact for bf16 within 2^-22 of the largest query of the tile; one
 //          power-of-two scale per tile of queries)
-//   256 p  hi + lo, 256 p <= 256 within a tile of 128 tokens: off by at most 2^-9 of itself (a bf16 would be by 2^-8) or by
-//          half a step of 2^-9, which is 2^-18 of the tile's largest weight
+//   256 p  hi + lo, 256 p <= 256 within a block of 64 tokens: off by at most 2^-9 + 2^-11 (f16 on the way) of itself or by half
+//          a step of 2^-9, which is 2^-18 of the block's largest weight, whatever the other block's weights and values are
 // With S^T = K Q^T the 128 tokens of a tile are the lanes of tensor memory and the query rows its columns (R = 8 or 16 of
 // them: heads of a group x queries), so a thread owns one token, and the scale of its key is a factor of the whole warp;
 // O^T = V^T P^T has the 128 elements of the head as its lanes.  Each 64-token block of V gets an accumulator of its own, to
@@ -256,7 +256,7 @@ struct AtCfg {
   static constexpr int kTile = 128 * kHeadDim;         // 16 KiB
   static constexpr int kDCol0 = 2 * kN;                // two S accumulators, then one D per 64-token block
   static constexpr int kTmemCols = 8 * R;
-  static constexpr int kStatFloats = 2 * 4 * R /* warp maxima */ + 4 * 2 * 2 * R /* per warp: factors */ + 4 * R /* per warp: maxima */ + 4 * R;
+  static constexpr int kStatFloats = 2 * 4 * R /* warp maxima */ + 4 * 2 * 3 * R /* per warp: factors */ + 4 * 2 * R /* per warp: its block's maxima and factors */ + 4 * R;
   static constexpr size_t kSmemBytes = 1024 + kQBytes + kPBytes + static_cast<size_t>(kKStages + kVStages) * kTile + kStatFloats * 4 + R * 4 + (2 * kMaxFlat + 6) * 4 + 256;
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
@@ -293,9 +293,9 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   uint8_t* k_s = p_s + C::kPBytes;
   uint8_t* v_s = k_s + C::kKStages * C::kTile;
   float* wmax = reinterpret_cast<float*>(v_s + C::kVStages * C::kTile);      // [2][4 warps][R]
-  float* fac = wmax + 2 * 4 * R;                                  // [4 warps][2][2: alpha, beta][R]
-  float* mloc = fac + 4 * 2 * 2 * R;                              // [4 warps][R]: the tile's maxima
-  float* red = mloc + 4 * R;                                      // [4 warps][R]
+  float* fac = wmax + 2 * 4 * R;                                  // [4 warps][2][3: alpha, factor of either block's product][R]
+  float* mloc = fac + 4 * 2 * 3 * R;                              // [4 warps][2: maxima of the warp's block, factor of its weights][R]
+  float* red = mloc + 4 * 2 * R;                                  // [4 warps][R]
   int* lim_s = reinterpret_cast<int*>(red + 4 * R);               // [R] last position a row sees, relative to the tile loop's base
   int* first_s = lim_s + R;                                       // [batch + 1] first tile of each sequence in the row of tiles
   int* pos_s = first_s + kMaxFlat + 1;                            // their positions
@@ -462,8 +462,9 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   } else {
     const int sw = warp - 2, quad = warp & 3, tok = quad * 32 + lane, tid = static_cast<int>(threadIdx.x) - 64;
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-    float* my_fac = fac + sw * 4 * R;
-    float* my_max = mloc + sw * R;
+    float* my_fac = fac + sw * 6 * R;
+    float* my_max = mloc + sw * 2 * R;
+    const bool second = quad >= 2;                    // the tile's second block of 64
 
     bool ok = true;
     uint32_t gs = 0;
@@ -544,20 +545,20 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     const int lim_min = static_cast<int>(min(pos, 0x7FFFFFFFll));
     const long long written = pos + a.t;              // rows behind the last sequence position may hold anything
 
-    // adds the product of the tile before: o = o * alpha + (D0 * vs0 + D1 * vs1) * beta / 256
+    // adds the product of the tile before: o = o * alpha + D0 * (vs0 * beta0 / 256) + D1 * (vs1 * beta1 / 256)
     auto promote = [&](int j, float vs0, float vs1) {
       ok = mbar_wait_bounded_lanes(d_full, (gs + j) & 1u, abort_flag);
       if (!ok) return;
       tc_fence_after();
-      const float* f = my_fac + (j & 1) * 2 * R;
+      const float* f = my_fac + (j & 1) * 3 * R;
       const bool finite = fabsf(vs0) < 3e38f && fabsf(vs1) < 3e38f;
-      auto add = [&](int r, float d0, float d1, float al, float be) {
+      auto add = [&](int r, float d0, float d1, float al, float f0, float f1) {
         if (!finite) {                                // a block of NaN: not for the rows that end before it
-          d0 = lim_s[r] >= (tile0 + j) * 128 ? d0 * vs0 : 0.0f;
-          d1 = lim_s[r] >= (tile0 + j) * 128 + kCacheBlock ? d1 * vs1 : 0.0f;
-          o[r] = fmaf(o[r], al, (d0 + d1) * be);
+          d0 = lim_s[r] >= (tile0 + j) * 128 ? d0 * f0 : 0.0f;
+          d1 = lim_s[r] >= (tile0 + j) * 128 + kCacheBlock ? d1 * f1 : 0.0f;
+          o[r] = fmaf(o[r], al, d0 + d1);
         } else {
-          o[r] = fmaf(o[r], al, fmaf(d0, vs0, d1 * vs1) * be);
+          o[r] = fmaf(o[r], al, fmaf(d0, f0, d1 * f1));
         }
       };
       if constexpr (R == 8) {
@@ -567,7 +568,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
         tc_wait_ld();
 #pragma unroll
         for (int r = 0; r < 8; ++r)
-          add(r, __uint_as_float(d0[r]) + __uint_as_float(d0[8 + r]), __uint_as_float(d1[r]) + __uint_as_float(d1[8 + r]), f[r], f[R + r]);
+          add(r, __uint_as_float(d0[r]) + __uint_as_float(d0[8 + r]), __uint_as_float(d1[r]) + __uint_as_float(d1[8 + r]), f[r], f[R + r], f[2 * R + r]);
       } else {
 #pragma unroll
         for (int c = 0; c < R / 8; ++c) {
@@ -579,8 +580,15 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
           tc_ld_32x32b_x8(at + C::kN + R, l1);
           tc_wait_ld();
 #pragma unroll
-          for (int x = 0; x < 8; ++x)
-            add(c * 8 + x, __uint_as_float(h0[x]) + __uint_as_float(l0[x]), __uint_as_float(h1[x]) + __uint_as_float(l1[x]), f[c * 8 + x], f[R + c * 8 + x]);
+          for (int x = 0; x < 8; x += 4) {
+            const float4 al = *reinterpret_cast<const float4*>(f + c * 8 + x), f0 = *reinterpret_cast<const float4*>(f + R + c * 8 + x),
+                         f1 = *reinterpret_cast<const float4*>(f + 2 * R + c * 8 + x);
+            const auto d = [&](const uint32_t (&h)[8], const uint32_t (&l)[8], int y) { return __uint_as_float(h[y]) + __uint_as_float(l[y]); };
+            add(c * 8 + x, d(h0, l0, x), d(h1, l1, x), al.x, f0.x, f1.x);
+            add(c * 8 + x + 1, d(h0, l0, x + 1), d(h1, l1, x + 1), al.y, f0.y, f1.y);
+            add(c * 8 + x + 2, d(h0, l0, x + 2), d(h1, l1, x + 2), al.z, f0.z, f1.z);
+            add(c * 8 + x + 3, d(h0, l0, x + 3), d(h1, l1, x + 3), al.w, f0.w, f1.w);
+          }
         }
       }
       tc_fence_before();
@@ -652,19 +660,24 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
       ok = softmax_barrier(ok);
       if (!ok) break;
       if (lane < R) {
-        const float m = fmaxf(fmaxf(wm[lane], wm[R + lane]), fmaxf(wm[2 * R + lane], wm[3 * R + lane]));
-        const float m_new = fmaxf(m_run, m);
-        my_fac[(j & 1) * 2 * R + lane] = m_run > kNegInf ? ex2_approx(m_run - m_new) : 0.0f;
-        my_fac[(j & 1) * 2 * R + R + lane] = m > kNegInf ? ex2_approx(m - m_new - 8.0f) : 0.0f;
+        // warps 2 and 3 of the four have the first 64 tokens
+        const float m0 = fmaxf(wm[2 * R + lane], wm[3 * R + lane]), m1 = fmaxf(wm[lane], wm[R + lane]), m = second ? m1 : m0;
+        const float m_new = fmaxf(m_run, fmaxf(m0, m1));
+        const float b0 = m0 > kNegInf ? ex2_approx(m0 - m_new - 8.0f) : 0.0f, b1 = m1 > kNegInf ? ex2_approx(m1 - m_new - 8.0f) : 0.0f;
+        float* f = my_fac + (j & 1) * 3 * R;
+        f[lane] = m_run > kNegInf ? ex2_approx(m_run - m_new) : 0.0f;
+        f[R + lane] = b0 * nv0;
+        f[2 * R + lane] = b1 * nv1;
         my_max[lane] = m > kNegInf ? 8.0f - m : 0.0f;
+        my_max[R + lane] = second ? b1 : b0;
         m_run = m_new;
       }
       __syncwarp();
-      const float* f = my_fac + (j & 1) * 2 * R;
+      const float* f = my_fac + (j & 1) * 3 * R;
       uint32_t hi[R / 4], lo[R / 4];
 #pragma unroll
       for (int r = 0; r < R; r += 4) {
-        const float4 mx = *reinterpret_cast<const float4*>(my_max + r), al = *reinterpret_cast<const float4*>(f + r), be = *reinterpret_cast<const float4*>(f + R + r);
+        const float4 mx = *reinterpret_cast<const float4*>(my_max + r), al = *reinterpret_cast<const float4*>(f + r), be = *reinterpret_cast<const float4*>(my_max + R + r);
         float p[4] = {ex2_approx(fmaf(s[r], ksc, mx.x)), ex2_approx(fmaf(s[r + 1], ksc, mx.y)), ex2_approx(fmaf(s[r + 2], ksc, mx.z)),
                       ex2_approx(fmaf(s[r + 3], ksc, mx.w))};      // 256 p
         if (masked) {                                  // whatever the scale of their block is

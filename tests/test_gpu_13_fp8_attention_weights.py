@@ -115,6 +115,26 @@ def test_a_channel_of_large_values_takes_nothing_from_the_others(plq, b, t, head
     plq.check_device_status()
 
 
+@pytest.mark.parametrize("rows", [(1, 1, 1), (2, 8, 1), (1, 16, 2)])
+def test_two_value_blocks_of_a_tile_keep_their_own_weights(plq, rows):
+    """The second half of a tile of 128 positions: weights of 2^-18.8 of the first half's, values 2^19 times as large."""
+    t, heads, kv_heads = rows
+    n = 128 + t
+    k, v = torch.zeros(n, 128, device="cuda"), torch.zeros(n, 128, device="cuda")
+    k[:64] = 1.0
+    v[:64, ::2], v[64:, 1::2] = 1.0, 1.0
+    v_scale = torch.tensor([1.0, 2.0 ** 19, 2.0 ** 19], device="cuda")[: -(-n // BLOCK)]
+    cache = _cache(plq, 1, n, kv_heads, k, v, torch.ones_like(v_scale), v_scale)
+    q = torch.full((1, t, heads, 128), 13.0 / 128 ** 0.5, device="cuda").to(torch.bfloat16)
+    out = plq.ops.fp8_cache_attention(q, cache, n - t)
+    _check(out, q, cache, n - t)
+    small = math.exp(-float(q[0, 0, 0, 0]) * 128 ** 0.5)
+    behind = 65.0 + torch.arange(t, device="cuda", dtype=torch.float64)[:, None]
+    want = behind * small / (64 + behind * small) * 2.0 ** 19
+    # a weight 2^-9 + 2^-11, steps 2^-12, the result 2^-8, the exponential of 13
+    assert float((out[0, ..., 1].double() / want - 1).abs().max()) <= 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -11 + 2.0 ** -12 + 2.0 ** -17
+
+
 @pytest.mark.parametrize("b,t,heads,kv_heads,n", [(1, 1, 8, 1, 3000), (2, 2, 8, 2, 900), (1, 8, 4, 1, 9000), (4, 70, 16, 4, 1500), (2, 300, 8, 2, 300)])
 @pytest.mark.parametrize("gain", [1.0, 4.0, 12.0])
 def test_scores_and_values_of_every_size(plq, b, t, heads, kv_heads, n, gain):
