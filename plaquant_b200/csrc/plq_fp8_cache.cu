@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(256, 4) rope_kv_append_fp8_kernel(const Fp8App
 // One pass over the cache with the 8-bit codes fed to the tensor core as they are (tcgen05 kind::f8f6f4): no thread
 // converts or scales a key or a value.  For that the other operand has to be 8-bit too, without losing its precision, and
 // is the sum of two E4M3 numbers, which are two sets of columns of one product:
-//   q      hi + lo / 16 (4 + 4 significant bits: exact for bf16 within 2^-22 of the largest query of the tile; one
-//          power-of-two scale per tile of queries)
+//   q      hi + lo / 16 at a power of two of the row's own that brings its largest element to [128, 256): exact for what is at
+//          least 2^-13 of that, off by 2^-21 of it below
 //   256 p  hi + lo, 256 p <= 256 within a block of 64 tokens: off by at most 2^-9 + 2^-11 (f16 on the way) of itself or by half
 //          a step of 2^-9, which is 2^-18 of the block's largest weight, whatever the other block's weights and values are
 // With S^T = K Q^T the 128 tokens of a tile are the lanes of tensor memory and the query rows its columns (R = 8 or 16 of
@@ -256,7 +256,7 @@ struct AtCfg {
   static constexpr int kTile = 128 * kHeadDim;         // 16 KiB
   static constexpr int kDCol0 = 2 * kN;                // two S accumulators, then one D per 64-token block
   static constexpr int kTmemCols = 8 * R;
-  static constexpr int kStatFloats = 2 * 4 * R /* warp maxima */ + 4 * 2 * 3 * R /* per warp: factors */ + 4 * 2 * R /* per warp: its block's maxima and factors */ + 4 * R;
+  static constexpr int kStatFloats = 2 * 4 * R /* warp maxima */ + 4 * 2 * 3 * R /* per warp: factors */ + 4 * 3 * R /* per warp: of its tokens */ + 4 * R + R;
   static constexpr size_t kSmemBytes = 1024 + kQBytes + kPBytes + static_cast<size_t>(kKStages + kVStages) * kTile + kStatFloats * 4 + R * 4 + (2 * kMaxFlat + 6) * 4 + 256;
   static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
@@ -294,9 +294,10 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
   uint8_t* v_s = k_s + C::kKStages * C::kTile;
   float* wmax = reinterpret_cast<float*>(v_s + C::kVStages * C::kTile);      // [2][4 warps][R]
   float* fac = wmax + 2 * 4 * R;                                  // [4 warps][2][3: alpha, factor of either block's product][R]
-  float* mloc = fac + 4 * 2 * 3 * R;                              // [4 warps][2: maxima of the warp's block, factor of its weights][R]
-  float* red = mloc + 4 * 2 * R;                                  // [4 warps][R]
-  int* lim_s = reinterpret_cast<int*>(red + 4 * R);               // [R] last position a row sees, relative to the tile loop's base
+  float* mloc = fac + 4 * 2 * 3 * R;                              // [4 warps][3: maxima of the block, factor of its weights, scale of its scores][R]
+  float* red = mloc + 4 * 3 * R;                                  // [4 warps][R]
+  float* down_s = red + 4 * R;                                    // [R] scale of a row's scores without that of the keys
+  int* lim_s = reinterpret_cast<int*>(down_s + R);               // [R] last position a row sees, relative to the tile loop's base
   int* first_s = lim_s + R;                                       // [batch + 1] first tile of each sequence in the row of tiles
   int* pos_s = first_s + kMaxFlat + 1;                            // their positions
   int* start_s = pos_s + kMaxFlat;                                // the run: first and last tile, sequence of the first
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     const int sw = warp - 2, quad = warp & 3, tok = quad * 32 + lane, tid = static_cast<int>(threadIdx.x) - 64;
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     float* my_fac = fac + sw * 6 * R;
-    float* my_max = mloc + sw * 2 * R;
+    float* my_max = mloc + sw * 3 * R;
     const bool second = quad >= 2;                    // the tile's second block of 64
 
     bool ok = true;
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     while (ok && next_segment(g)) {
     const long long b = g.b, pos = g.pos;
     const int n = g.n, tile0 = g.tile0;
-    // ---- the queries: tile-wide power-of-two scale, hi and lo codes ----
+    // ---- the queries: a row's scale, hi and lo codes ----
     const bool has_q = tid < 8 * R;                   // 16 elements each
     const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = a.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu;      // a negative or no scale
     const __nv_bfloat16* q_base = a.q + ((b * a.t) * a.heads + static_cast<long long>(kh) * a.group) * kHeadDim;
@@ -495,20 +496,16 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
       if (hi < 0x7F800000u) top = max(top, hi);
     }
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    for (int d = 4; d >= 1; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
     softmax_barrier();                                // the segment before has been read out
-    if (lane == 0) reinterpret_cast<uint32_t*>(red)[sw] = top;
     if (tid < R) {
       const int i = tid / a.group;
       lim_s[tid] = tid < nrows ? static_cast<int>(min(pos + i, 0x7FFFFFFFll)) : 0x7FFFFFFF;
     }
-    softmax_barrier();
-    top = max(max(reinterpret_cast<uint32_t*>(red)[0], reinterpret_cast<uint32_t*>(red)[1]),
-              max(reinterpret_cast<uint32_t*>(red)[2], reinterpret_cast<uint32_t*>(red)[3]));
-    softmax_barrier();
-    // largest query in [128, 256): multiply by 2^e
+    // largest element in [128, 256): multiply by 2^e
     const int e = top == 0 ? 0 : min(max(134 - static_cast<int>(top >> 23), -120), 120);
     const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23), down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    if (has_q && (tid & 7) == 0) down_s[r] = down * (a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2));
     {
       const int chunk = tid & 7;
       uint32_t hi[4], lo[4];
@@ -534,8 +531,9 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
       }
     }
     fence_proxy_async_smem();
-    __syncwarp();
+    softmax_barrier();
     if (lane == 0 && n > 0) mbar_arrive(q_full);
+    const float down_lane = lane < R ? down_s[lane] : 1.0f;
 
     // ---- the tiles ----
     float o[R], l[R], m_run = kNegInf;                // o: element `tok` of the head; m_run: row `lane`
@@ -599,7 +597,6 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     const int last_block = static_cast<int>((written - 1) / kCacheBlock);       // the last one that holds a position
     auto scale_of = [&](const float* side, int block) { return block <= last_block ? side[block] : 1.0f; };
     float next_k = 1.0f, next_v0 = 1.0f, next_v1 = 1.0f;
-    const float per_k = down * (a.scale_log2 == 0.0f ? 1.0f : fabsf(a.scale_log2));
     if (n > 0) {
       next_k = scale_of(k_scale, tile0 * 2 + (quad >> 1));
       next_v0 = scale_of(v_scale, tile0 * 2);
@@ -608,7 +605,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
     for (int j = 0; j < n; ++j) {                     // `ok` is looked at by all warps together, at the barrier
       const int tile = tile0 + j;
       const float nv0 = next_v0, nv1 = next_v1;
-      float ksc = next_k * per_k;                     // of the warp's tokens
+      float ksc = next_k * down_lane;                 // of the warp's tokens and row `lane`
       if (ksc < 1.2e-38f) ksc = 1.2e-38f;             // a score of zero, and minus infinity stays what it is
       if (j + 1 < n) {                                // a tile ahead: they come from L2
         next_k = scale_of(k_scale, tile * 2 + 2 + (quad >> 1));
@@ -670,6 +667,7 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
         f[2 * R + lane] = b1 * nv1;
         my_max[lane] = m > kNegInf ? 8.0f - m : 0.0f;
         my_max[R + lane] = second ? b1 : b0;
+        my_max[2 * R + lane] = ksc;
         m_run = m_new;
       }
       __syncwarp();
@@ -677,9 +675,10 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
       uint32_t hi[R / 4], lo[R / 4];
 #pragma unroll
       for (int r = 0; r < R; r += 4) {
-        const float4 mx = *reinterpret_cast<const float4*>(my_max + r), al = *reinterpret_cast<const float4*>(f + r), be = *reinterpret_cast<const float4*>(my_max + R + r);
-        float p[4] = {ex2_approx(fmaf(s[r], ksc, mx.x)), ex2_approx(fmaf(s[r + 1], ksc, mx.y)), ex2_approx(fmaf(s[r + 2], ksc, mx.z)),
-                      ex2_approx(fmaf(s[r + 3], ksc, mx.w))};      // 256 p
+        const float4 mx = *reinterpret_cast<const float4*>(my_max + r), al = *reinterpret_cast<const float4*>(f + r), be = *reinterpret_cast<const float4*>(my_max + R + r),
+                     ks = *reinterpret_cast<const float4*>(my_max + 2 * R + r);
+        float p[4] = {ex2_approx(fmaf(s[r], ks.x, mx.x)), ex2_approx(fmaf(s[r + 1], ks.y, mx.y)), ex2_approx(fmaf(s[r + 2], ks.z, mx.z)),
+                      ex2_approx(fmaf(s[r + 3], ks.w, mx.w))};      // 256 p
         if (masked) {                                  // whatever the scale of their block is
 #pragma unroll
           for (int x = 0; x < 4; ++x)

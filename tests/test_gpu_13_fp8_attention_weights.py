@@ -135,6 +135,26 @@ def test_two_value_blocks_of_a_tile_keep_their_own_weights(plq, rows):
     assert float((out[0, ..., 1].double() / want - 1).abs().max()) <= 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -11 + 2.0 ** -12 + 2.0 ** -17
 
 
+@pytest.mark.parametrize("t,heads,kv_heads", [(1, 4, 1), (2, 8, 1), (4, 8, 1), (40, 4, 1)])
+@pytest.mark.parametrize("power", [10, 20, 40])
+def test_a_small_query_beside_a_large_one(plq, t, heads, kv_heads, power):
+    """Heads of one group whose queries differ by powers of two: each has its own scale."""
+    n, g = 700, torch.Generator(device="cuda").manual_seed(power)
+    k = torch.randn(n, 128, generator=g, device="cuda")
+    v = torch.randn(n, 128, generator=g, device="cuda")
+    k[:, :64] *= 2.0 ** -6                             # what the large query looks at
+    k_scale = torch.full((11,), 2.0 ** (power - 6), device="cuda")
+    cache = _cache(plq, 1, n, kv_heads, k, v, k_scale, torch.ones(11, device="cuda"))
+    q = torch.randn(1, t, heads, 128, generator=g, device="cuda") * 2.0 ** (6 - power)
+    q[:, :, 0] = 0.0
+    q[:, :, 0, 3] = 2.0 ** 6
+    q[:, :, 1:, :64] = 0.0
+    q = q.to(torch.bfloat16)
+    cache.k.view(n, 128)[:, 3] = 0                     # nothing: its row is the plain mean
+    out = plq.ops.fp8_cache_attention(q, cache, n - t)
+    _check(out, q, cache, n - t)
+
+
 @pytest.mark.parametrize("b,t,heads,kv_heads,n", [(1, 1, 8, 1, 3000), (2, 2, 8, 2, 900), (1, 8, 4, 1, 9000), (4, 70, 16, 4, 1500), (2, 300, 8, 2, 300)])
 @pytest.mark.parametrize("gain", [1.0, 4.0, 12.0])
 def test_scores_and_values_of_every_size(plq, b, t, heads, kv_heads, n, gain):
