@@ -654,7 +654,7 @@ def fp8_cache_attention(q: torch.Tensor, cache, pos, scale: Optional[float] = No
         raise ValueError(f"{heads} query heads do not divide over {kv_heads} key heads")
     ptr, each, host = _positions(pos, b, q.device)
     if ptr is None and host >= 0:
-        ctx = min(host + t, cache.room)
+        ctx = max(1, min(host + t, cache.room))
     elif not ctx:
         ctx = cache.room
     L = _lib.lib()

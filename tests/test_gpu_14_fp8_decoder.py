@@ -89,3 +89,16 @@ def test_the_quantised_head_takes_the_place_of_the_other(plq, tmp_path):
     again = ResQForwardB200(cfg, "cuda", packed=state, fp8_head=True)
     assert torch.equal(again.forward(ids), m.forward(ids)) and again.lm_head.device.type == "cpu"
     assert torch.equal(ResQForwardB200(cfg, "cuda", packed=state).forward(ids), plain.forward(ids))
+
+
+def test_no_queries_in_front_of_nothing(plq):
+    """T = 0 at position 0, as at any other, and no sequences."""
+    from plaquant_b200 import kv_cache
+    for b in (0, 2):
+        cache = kv_cache.Fp8Cache.empty(b, 64, 2, "cuda")
+        for pos in (0, 3, torch.zeros(b, dtype=torch.int64, device="cuda")):
+            q = torch.empty(b, 0, 8, 128, dtype=torch.bfloat16, device="cuda")
+            assert plq.ops.fp8_cache_attention(q, cache, pos).shape == (b, 0, 8, 128)
+            none = torch.empty(0, 128, device="cuda")
+            assert plq.ops.rope_kv_append_fp8(torch.empty(b, 0, 12 * 128, dtype=torch.bfloat16, device="cuda"), none, none, 8, 2, cache, pos).shape == q.shape
+    plq.check_device_status()
