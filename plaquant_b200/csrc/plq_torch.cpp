@@ -167,6 +167,109 @@ struct Linear {
 
 Tensor heads_first(const Tensor& t) { return t.transpose(1, 2); }
 
+// The two halves of a decoder layer around its attention.  Workspace: the packed operand of the linear that runs, `packed`
+// bytes, then that linear's output.
+struct LayerSizes {
+  int64_t rows, hidden, ffn, packed, out0;
+  bool gated;                                          // the GEMM applies SiLU(gate) * up itself: one column per pair
+  LayerSizes(const Tensor& h, std::initializer_list<const Linear*> linears, int64_t ffn_)
+      : rows(h.size(0) * h.size(1)), hidden(h.size(2)), ffn(ffn_), packed(0), out0(up256(2 * rows * hidden)), gated(rows > 16) {
+    for (const Linear* l : linears) packed = std::max(packed, l->packed_bytes(rows));
+  }
+  int64_t back_bytes() const { return out0 + (gated ? 2 : 4) * rows * ffn; }
+};
+
+// h + delta -> RMSNorm(ln1) -> qkv at `out` [rows, qkv.n].  Returns the residual stream.
+Tensor front_half(const LayerSizes& z, const Linear& qkv, const Tensor& ln1, float eps, const Tensor& h, const std::optional<Tensor>& delta, void* ws,
+                  void* out, void* stream) {
+  Tensor h1 = h;
+  const PackedAt p(ws, z.rows, qkv.k_lo, qkv.k_hi);
+  if (delta) {
+    h1 = at::empty_like(h);
+    check(api.add_rmsnorm_pack(delta->const_data_ptr(), h.const_data_ptr(), h1.data_ptr(), ln1.const_data_ptr(), eps, z.rows, z.hidden,
+                               qkv.k_hi, 1, p.lo, p.lo_sf, p.hi, p.hi_sf, PLQ_SF_TILED, stream));
+  } else {
+    check(api.rmsnorm_pack(h.const_data_ptr(), ln1.const_data_ptr(), eps, z.rows, z.hidden, qkv.k_hi, 1, p.lo, p.lo_sf, p.hi, p.hi_sf,
+                           PLQ_SF_TILED, stream));
+  }
+  check(qkv.product(p, z.rows, out, qkv.n, stream));
+  return h1;
+}
+
+// attn -> o_proj -> residual h1, RMSNorm(ln2) -> gate_up -> SiLU * up -> down_proj, with z.back_bytes() of outputs at `act`.
+// Returns (residual stream, down_proj's output not added to it yet).
+std::tuple<Tensor, Tensor> back_half(const LayerSizes& z, const Linear& o, const Linear& gate_up, const Linear& down, const Tensor& ln2, float eps,
+                                     Tensor h1, Tensor attn, bool last_only, void* ws, uint8_t* act, void* stream) {
+  const int64_t b = h1.size(0), t = h1.size(1), hidden = z.hidden, ffn = z.ffn, like = z.rows;
+  if (last_only) {
+    attn = attn.slice(1, t - 1).contiguous();
+    h1 = h1.slice(1, t - 1).contiguous();
+  }
+  const int64_t out_rows = last_only ? b : z.rows;
+  Tensor h2 = at::empty_like(h1), delta2 = at::empty_like(h1);
+  uint8_t* gu = act + z.out0;
+  {
+    const PackedAt p(ws, out_rows, o.k_lo, o.k_hi);
+    check(api.pack(attn.const_data_ptr(), out_rows, o.k(), o.k_hi, 1, p.lo, p.lo_sf, p.hi, p.hi_sf, PLQ_SF_TILED, stream));
+    check(o.product(p, out_rows, act, hidden, stream, like));
+  }
+  {
+    const PackedAt p(ws, out_rows, gate_up.k_lo, gate_up.k_hi);
+    check(api.add_rmsnorm_pack(act, h1.const_data_ptr(), h2.data_ptr(), ln2.const_data_ptr(), eps, out_rows, hidden, gate_up.k_hi, 1, p.lo,
+                               p.lo_sf, p.hi, p.hi_sf, PLQ_SF_TILED, stream));
+    if (z.gated)
+      check(api.mixed_gemm_silu_mul(p.lo, p.lo_sf, p.hi, p.hi_sf, ptr(gate_up.lo), ptr(gate_up.lo_sf), ptr(gate_up.hi), ptr(gate_up.hi_sf),
+                                    out_rows, ffn, gate_up.k_lo, gate_up.k_hi, gu, ffn, gate_up.status.data_ptr<int32_t>(), stream));
+    else
+      check(gate_up.product(p, out_rows, gu, 2 * ffn, stream, like));
+  }
+  {
+    const PackedAt p(ws, out_rows, down.k_lo, down.k_hi);
+    if (z.gated)
+      check(api.pack(gu, out_rows, ffn, down.k_hi, 1, p.lo, p.lo_sf, p.hi, p.hi_sf, PLQ_SF_TILED, stream));
+    else
+      check(api.silu_mul_pack(gu, gu + 2 * ffn, 2 * ffn, out_rows, ffn, down.k_hi, 1, p.lo, p.lo_sf, p.hi, p.hi_sf, PLQ_SF_TILED, stream));
+    check(down.product(p, out_rows, delta2.data_ptr(), hidden, stream, like));
+  }
+  return {h2, delta2};
+}
+
+void check_stream(const Tensor& h, const std::optional<Tensor>& delta) {
+  TORCH_CHECK(h.dim() == 3 && h.is_contiguous() && h.scalar_type() == at::kBFloat16 && (!delta || (delta->is_contiguous() && delta->sizes() == h.sizes())),
+              "h and delta must be contiguous bfloat16 [B, T, hidden]");
+}
+
+// The halves as calls of their own, for an attention that is not one of decoder_layer's.
+// -> (residual stream, [B, T, qkv.n])
+std::tuple<Tensor, Tensor> layer_front(const Linear& qkv, const Tensor& ln1, double eps, const Tensor& h, const std::optional<Tensor>& delta) {
+  pybind11::gil_scoped_release nogil;
+  const c10::cuda::CUDAGuard guard(h.device());
+  check_stream(h, delta);
+  TORCH_CHECK(qkv.k() == h.size(2), "the layer's linears do not fit together");
+  const LayerSizes z(h, {&qkv}, 0);
+  const Tensor ws = at::empty({z.packed}, h.options().dtype(at::kByte));
+  Tensor out = at::empty({h.size(0), h.size(1), qkv.n}, h.options());
+  return {front_half(z, qkv, ln1, static_cast<float>(eps), h, delta, ws.data_ptr(), out.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()), out};
+}
+
+// attn: [B, T, o.k()].  -> (residual stream, down_proj's output not added to it yet)
+std::tuple<Tensor, Tensor> layer_back(const Linear& o, const Linear& gate_up, const Linear& down, const Tensor& ln2, double eps, const Tensor& h,
+                                      const Tensor& attn, bool last_only) {
+  pybind11::gil_scoped_release nogil;
+  const c10::cuda::CUDAGuard guard(h.device());
+  check_stream(h, std::nullopt);
+  const int64_t ffn = down.k();
+  TORCH_CHECK(o.n == h.size(2) && gate_up.k() == h.size(2) && gate_up.n == 2 * ffn && down.n == h.size(2) && ffn % 128 == 0,
+              "the layer's linears do not fit together");
+  TORCH_CHECK(attn.is_contiguous() && attn.scalar_type() == at::kBFloat16 && attn.dim() == 3 && attn.size(0) == h.size(0) && attn.size(1) == h.size(1) &&
+                  attn.size(2) == o.k() && attn.device() == h.device(),
+              "the attention's output must be contiguous bfloat16 [B, T, heads * head_dim]");
+  const LayerSizes z(h, {&o, &gate_up, &down}, ffn);
+  const Tensor ws = at::empty({z.packed + z.back_bytes()}, h.options().dtype(at::kByte));
+  uint8_t* at = static_cast<uint8_t*>(ws.data_ptr());
+  return back_half(z, o, gate_up, down, ln2, static_cast<float>(eps), h, attn, last_only, at, at + z.packed, c10::cuda::getCurrentCUDAStream().stream());
+}
+
 // One decoder layer on one GPU: h + delta -> RMSNorm(ln1) -> qkv -> RoPE, cache append -> attention -> o_proj -> residual,
 // RMSNorm(ln2) -> gate_up -> SiLU * up -> down_proj.  Returns (residual stream, down_proj's output not added to it yet).
 // k_view / v_view: the first `ctx` positions of caches allocated for `cap`; the new rows go to `pos` (or *pos_dev).
@@ -181,10 +284,9 @@ std::tuple<Tensor, Tensor> decoder_layer(const Linear& qkv, const Linear& o, con
                                          const std::optional<Tensor>& had, bool last_only) {
   pybind11::gil_scoped_release nogil;
   const c10::cuda::CUDAGuard guard(h.device());
+  check_stream(h, delta);
   const int64_t b = h.size(0), t = h.size(1), hidden = h.size(2), rows = b * t, ctx = k_view.size(1);
   const int64_t nq = (heads + 2 * kv_heads) * 128, ffn = down.k(), attn_width = heads * 128;
-  TORCH_CHECK(h.is_contiguous() && h.scalar_type() == at::kBFloat16 && (!delta || (delta->is_contiguous() && delta->sizes() == h.sizes())),
-              "h and delta must be contiguous bfloat16 [B, T, hidden]");
   TORCH_CHECK(qkv.n == nq && qkv.k() == hidden && o.k() == attn_width && o.n == hidden && gate_up.k() == hidden &&
                   gate_up.n == 2 * ffn && down.n == hidden && ffn % 128 == 0,
               "the layer's linears do not fit together");
@@ -197,32 +299,16 @@ std::tuple<Tensor, Tensor> decoder_layer(const Linear& qkv, const Linear& o, con
                     c->stride(1) == kv_heads * width && c->stride(2) == width && c->stride(3) == 1,
                 "the caches must be the leading positions of contiguous allocations");
   TORCH_CHECK(t == 1 || mask || t == ctx, "a chunk behind a prompt needs a mask");
-  int64_t packed_bytes = 0;
-  for (const Linear* l : {&qkv, &o, &gate_up, &down}) packed_bytes = std::max(packed_bytes, l->packed_bytes(rows));
   const auto opts = h.options();
-  // Workspace: the packed operand of the linear that runs, then its output; qkv's is dead before o's is written, and the
-  // attention's operands have storage of their own.
-  const bool gated = rows > 16;                        // the GEMM applies SiLU(gate) * up itself: one column per pair
-  const int64_t out0 = up256(2 * rows * hidden);
-  const Tensor ws = at::empty({packed_bytes + std::max(2 * rows * nq, out0 + (gated ? 2 : 4) * rows * ffn)}, opts.dtype(at::kByte));
-  uint8_t* act = static_cast<uint8_t*>(ws.data_ptr()) + packed_bytes;
+  // qkv's output is dead before o's is written, and the attention's operands have storage of their own.
+  const LayerSizes z(h, {&qkv, &o, &gate_up, &down}, ffn);
+  const Tensor ws = at::empty({z.packed + std::max(2 * rows * nq, z.back_bytes())}, opts.dtype(at::kByte));
+  uint8_t* act = static_cast<uint8_t*>(ws.data_ptr()) + z.packed;
   void* stream = c10::cuda::getCurrentCUDAStream().stream();
   int32_t* status = qkv.status.data_ptr<int32_t>();
   const float eps = static_cast<float>(eps_);
 
-  Tensor h1 = h;
-  {
-    const PackedAt p(ws.data_ptr(), rows, qkv.k_lo, qkv.k_hi);
-    if (delta) {
-      h1 = at::empty_like(h);
-      check(api.add_rmsnorm_pack(delta->const_data_ptr(), h.const_data_ptr(), h1.data_ptr(), ln1.const_data_ptr(), eps, rows, hidden,
-                                 qkv.k_hi, 1, p.lo, p.lo_sf, p.hi, p.hi_sf, PLQ_SF_TILED, stream));
-    } else {
-      check(api.rmsnorm_pack(h.const_data_ptr(), ln1.const_data_ptr(), eps, rows, hidden, qkv.k_hi, 1, p.lo, p.lo_sf, p.hi, p.hi_sf,
-                             PLQ_SF_TILED, stream));
-    }
-    check(qkv.product(p, rows, act, nq, stream));
-  }
+  const Tensor h1 = front_half(z, qkv, ln1, eps, h, delta, ws.data_ptr(), act, stream);
   Tensor q = at::empty({b, t, heads, 128}, packed ? opts.dtype(at::kFloat) : opts), kk = k_view, vv = v_view;
   const int64_t* at_pos = pos_dev ? pos_dev->const_data_ptr<int64_t>() : nullptr;
   if (packed) {
@@ -239,39 +325,7 @@ std::tuple<Tensor, Tensor> decoder_layer(const Linear& qkv, const Linear& o, con
   Tensor attn = heads_first(at::scaled_dot_product_attention(heads_first(q), heads_first(kk), heads_first(vv), mask, 0.0,
                                                                    !mask && t > 1, std::nullopt, true))
                           .contiguous();
-
-  const int64_t like = rows;
-  if (last_only) {
-    attn = attn.slice(1, t - 1).contiguous();
-    h1 = h1.slice(1, t - 1).contiguous();
-  }
-  const int64_t out_rows = last_only ? b : rows;
-  Tensor h2 = at::empty_like(h1), delta2 = at::empty_like(h1);
-  uint8_t* gu = act + out0;
-  {
-    const PackedAt p(ws.data_ptr(), out_rows, o.k_lo, o.k_hi);
-    check(api.pack(attn.const_data_ptr(), out_rows, attn_width, o.k_hi, 1, p.lo, p.lo_sf, p.hi, p.hi_sf, PLQ_SF_TILED, stream));
-    check(o.product(p, out_rows, act, hidden, stream, like));
-  }
-  {
-    const PackedAt p(ws.data_ptr(), out_rows, gate_up.k_lo, gate_up.k_hi);
-    check(api.add_rmsnorm_pack(act, h1.const_data_ptr(), h2.data_ptr(), ln2.const_data_ptr(), eps, out_rows, hidden, gate_up.k_hi, 1, p.lo,
-                               p.lo_sf, p.hi, p.hi_sf, PLQ_SF_TILED, stream));
-    if (gated)
-      check(api.mixed_gemm_silu_mul(p.lo, p.lo_sf, p.hi, p.hi_sf, ptr(gate_up.lo), ptr(gate_up.lo_sf), ptr(gate_up.hi), ptr(gate_up.hi_sf),
-                                    out_rows, ffn, gate_up.k_lo, gate_up.k_hi, gu, ffn, status, stream));
-    else
-      check(gate_up.product(p, out_rows, gu, 2 * ffn, stream, like));
-  }
-  {
-    const PackedAt p(ws.data_ptr(), out_rows, down.k_lo, down.k_hi);
-    if (gated)
-      check(api.pack(gu, out_rows, ffn, down.k_hi, 1, p.lo, p.lo_sf, p.hi, p.hi_sf, PLQ_SF_TILED, stream));
-    else
-      check(api.silu_mul_pack(gu, gu + 2 * ffn, 2 * ffn, out_rows, ffn, down.k_hi, 1, p.lo, p.lo_sf, p.hi, p.hi_sf, PLQ_SF_TILED, stream));
-    check(down.product(p, out_rows, delta2.data_ptr(), hidden, stream, like));
-  }
-  return {h2, delta2};
+  return back_half(z, o, gate_up, down, ln2, eps, h1, attn, last_only, ws.data_ptr(), act, stream);
 }
 
 // Does nothing else share the memory of a or of b?  (The base that a view keeps alive does not count.)
@@ -394,6 +448,8 @@ PYBIND11_MODULE(_plq_torch, m) {
   m.def("pack", &pack);
   m.def("alone", &alone);
   m.def("decoder_layer", &decoder_layer);
+  m.def("layer_front", &layer_front);
+  m.def("layer_back", &layer_back);
   m.def("fp8_pack", &fp8_pack);
   m.def("fp8_gemm", &fp8_gemm);
   m.def("rope_kv_append_fp8", &rope_kv_append_fp8);

@@ -456,10 +456,12 @@ class ResQForwardB200:
         layer's attention nothing reads the other rows, and o_proj, norms and the MLP work row by row."""
         delta, c, chunk = None, self.cfg, {}
         b, t, _ = h.shape
-        native = (self.ctx.size == 1 and c.head_dim == 128 and self.kv_quant not in ("fp8", "fake") and 0 < b * t <= NATIVE_LAYER_ROWS
-                  and (t == 1 or pos0 == 0 or t * (pos0 + t) <= CHUNK_MASK_ELEMENTS)
+        native = (self.ctx.size == 1 and c.head_dim == 128 and self.kv_quant != "fake" and 0 < b * t <= NATIVE_LAYER_ROWS
+                  and (t == 1 or pos0 == 0 or self.kv_quant == "fp8" or t * (pos0 + t) <= CHUNK_MASK_ELEMENTS)
                   and h.dtype == torch.bfloat16 and h.is_contiguous())
-        if native:
+        if native and self.kv_quant == "fp8":        # the halves around the package's own attention
+            front, back = _lib.torch_lib().layer_front, _lib.torch_lib().layer_back
+        elif native:
             call, (cos, sin) = _lib.torch_lib().decoder_layer, cos_sin
             had = kv_cache.head_rotation(h.device) if self.kv_quant else None
         for li, L in enumerate(self.layers):
@@ -467,6 +469,11 @@ class ResQForwardB200:
             tail = last_only and t > 1 and b * t > 16 and li + 1 == len(self.layers) and self.ctx.size == 1
             if not native or not self._plain_layer(L):
                 h, delta = self._forward_layer(li, h, delta, pos0, cos_sin, static=static, last_only=tail and self._plain_layer(L))
+                continue
+            if self.kv_quant == "fp8":
+                h, qkv = front(L.qkv.native(), L.ln1, c.rms_eps, h, delta)
+                attn = self._attention(li, qkv, pos0, cos_sin, static)
+                h, delta = back(L.o.native(), L.gate_up.native(), L.down.native(), L.ln2, c.rms_eps, h, attn, tail)
                 continue
             if static is None:
                 k, v, n, cap = self._cache_room(li, b, t, pos0)

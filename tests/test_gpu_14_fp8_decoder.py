@@ -102,3 +102,34 @@ def test_no_queries_in_front_of_nothing(plq):
             none = torch.empty(0, 128, device="cuda")
             assert plq.ops.rope_kv_append_fp8(torch.empty(b, 0, 12 * 128, dtype=torch.bfloat16, device="cuda"), none, none, 8, 2, cache, pos).shape == q.shape
     plq.check_device_status()
+
+
+@pytest.mark.parametrize("heads,kv_heads,fp8_head", [(4, 2, False), (4, 4, True), (18, 2, False)])
+def test_layer_calls_around_the_cache_equal_the_operator_path(plq, monkeypatch, heads, kv_heads, fp8_head):
+    """Prompts of up to 16 rows and more, a chunk, single steps, a captured decode; the caches as well."""
+    from plaquant_b200 import _lib, forward_pass
+    cfg = _config(hidden_size=heads * 128, num_heads=heads, num_kv_heads=kv_heads)
+    ids = _ids(cfg, 3, 40, seed=7)
+    m = forward_pass.ResQForwardB200(cfg, "cuda", seed=3, kv_quant="fp8", fp8_head=fp8_head)
+    front, calls = _lib.torch_lib(), []
+    back = front.layer_back
+    monkeypatch.setattr(front, "layer_back", lambda *a: (calls.append(1), back(*a))[1])
+
+    def everything():
+        out = [m.forward(ids[:, :21]), m.forward(ids[:, 21:24], pos0=21)]
+        out += [m.forward(ids[:, i:i + 1], pos0=i) for i in range(24, 28)]
+        out += [x for c in m.kv for x in (c.k[:, :28].clone(), c.k_scale[..., 0].clone(), c.v[:, :28].clone(), c.v_scale[..., 0].clone())]
+        m._decode_states.clear()
+        return out + [m.generate(ids[:, :9], 5), m.forward(ids[:, :9], all_positions=True), m.forward(ids[:, :1]), m.forward(ids[:1, :5])]
+    got = everything()
+    n = len(calls)
+    assert n >= 2 * 12
+    monkeypatch.setattr(forward_pass, "NATIVE_LAYER_ROWS", 0)
+    want = everything()
+    assert len(calls) == n and all(torch.equal(a, b) for a, b in zip(got, want)) and len(got) == len(want)
+    with pytest.raises(RuntimeError):
+        back(m.layers[0].o.native(), m.layers[0].gate_up.native(), m.layers[0].down.native(), m.layers[0].ln2, 1e-6,
+             torch.zeros(1, 2, heads * 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 3, heads * 128, dtype=torch.bfloat16, device="cuda"), False)
+    with pytest.raises(RuntimeError):
+        front.layer_front(m.layers[0].qkv.native(), m.layers[0].ln1, 1e-6, torch.zeros(1, 2, 128, dtype=torch.bfloat16, device="cuda"), None)
+    plq.check_device_status()
