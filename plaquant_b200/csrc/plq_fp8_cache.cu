@@ -249,6 +249,7 @@ __device__ __forceinline__ int run_length(int total, int runs) { return max(1, (
 
 template <int R>
 struct AtCfg {
+  static_assert(R == 8 || R == 16, "rows of a key head: queries x heads of a group");
   static constexpr int kN = 2 * R;                     // columns of either product: hi | lo
   static constexpr int kPBytes = kN * 128;
   static constexpr int kQBytes = kN * 128;
@@ -389,7 +390,6 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
       g.whole = g.tile0 == 0 && end == all;
       g.n = end - g.tile0;
     }
-    if (g.n > 0) g.n = max(0, min(g.n, static_cast<int>((g.pos + a.t - 1) / 128) + 1 - g.tile0));      // what these rows see of it
     return true;
   };
   if (kh == 0 && (run == 0 || !a.runs) && a.status != nullptr) {
@@ -625,15 +625,12 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
 #pragma unroll
           for (int r = 0; r < 8; ++r) s[r] = fmaf(__uint_as_float(v[8 + r]), 0.0625f, __uint_as_float(v[r]));
         } else {
+          uint32_t v[16], y[16];
+          tc_ld_32x32b_x16(at, v);
+          tc_ld_32x32b_x16(at + 16, y);
+          tc_wait_ld();
 #pragma unroll
-          for (int c = 0; c < R / 16; ++c) {
-            uint32_t v[16], y[16];
-            tc_ld_32x32b_x16(at + c * 16, v);
-            tc_ld_32x32b_x16(at + R + c * 16, y);
-            tc_wait_ld();
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[c * 16 + r] = fmaf(__uint_as_float(y[r]), 0.0625f, __uint_as_float(v[r]));
-          }
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(__uint_as_float(y[r]), 0.0625f, __uint_as_float(v[r]));
         }
         tc_fence_before();
         __syncwarp();
@@ -701,11 +698,8 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
       if constexpr (R == 8) {
         *reinterpret_cast<uint4*>(p_s + tok * 16) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
       } else {
-#pragma unroll
-        for (int c = 0; c < R / 16; ++c) {
-          *reinterpret_cast<uint4*>(p_s + c * 2048 + tok * 16) = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
-          *reinterpret_cast<uint4*>(p_s + (R / 16 + c) * 2048 + tok * 16) = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
-        }
+        *reinterpret_cast<uint4*>(p_s + tok * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(p_s + 2048 + tok * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
       if (static_cast<long long>(tile) * 128 + 128 > written) {  // rows that nobody has written: 0 x NaN would be NaN
         const uint32_t vs = x % C::kVStages;
@@ -891,7 +885,7 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
 // so that a row's maximum and weight need no exchange.  A CTA has 128 rows and two CTAs share an SM: while one of them begins
 // or ends, or turns scores into weights, the tensor core works for the other.
 //   q      hi + lo, both E4M3 at the scale of the row (a power of two that brings its largest element to [128, 256)): exact
-//          for what is at least 2^-10 of that, off by 2^-18 of it below
+//          for what is at least 2^-9 of that, off by 2^-17 of 128 below
 //   S      of 64 positions, twice in tensor memory: the product of block j + 2 is issued behind the one that reads the weights
 //          of block j, so the scores of j + 1 lie ready when the weights of j are done
 //   p      w = exp2(score + log2 vs - e + 8) with e the row's largest score + log2 vs in the block of 64, rounded up: the scale of
@@ -1405,7 +1399,7 @@ static int launch_attention(const CUtensorMap& mk, const CUtensorMap& mv, const 
   const int st = allow_smem(fp8_attention_kernel<R>, C::kSmemBytes, &done_dev);
   if (st != PLQ_OK) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.kv_heads * a.row_tiles), static_cast<unsigned>(a.runs ? a.runs : a.batch));
+  cfg.gridDim = dim3(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(a.runs ? a.runs : a.batch));
   cfg.blockDim = dim3(192, 1, 1);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = static_cast<cudaStream_t>(stream);
