@@ -6,8 +6,8 @@
 //   weights codes [n, k], scales [ceil(n / 128), ceil(k / 128)], a over 128 x 128 elements
 //
 // The last block of a row may be shorter (k is a multiple of 16).  A block with a value that is not finite has the scale
-// NaN and codes of zero: its values are NaN, and no code ever is.  The floor keeps 448 / a finite; a block below it keeps
-// steps of 2^-109, far below anything a bf16 product can show.
+// NaN and codes of zero: its values are NaN, and no code ever is.  The floor keeps 448 / a finite; a block below it has
+// the scale 2^-109 and steps of 2^-118, far below anything a bf16 product can show.
 //
 // Bound by memory: 7 bytes per element with a residual (two bf16 in, one bf16 and one code out), 3 without.  8192 x 8192 with
 // residual and norm: 71.5 us replayed from a graph (6.6 TB/s), 333 x 4112 2.5 us, one row of 4096 2.1 us (a launch and the

@@ -87,7 +87,7 @@ CACHE_BLOCK = 64        # positions that share a scale of an Fp8Cache
 class Fp8Cache:
     """Keys and values of one layer in E4M3, `room` positions for each sequence of a batch, heads of 128.  One scale per
     64 positions and head, a power of two: value = code * scale.  Positions nobody has written may hold anything.
-    ops.rope_kv_append_fp8 fills it in place, ops.fp8_cache_attention reads it; 1.03 bytes per 2 of a bf16 cache.
+    ops.rope_kv_append_fp8 fills it in place, ops.fp8_cache_attention reads it; 1.0005 bytes per element, a bf16 cache has 2.
 
     `length`: how many leading positions the host knows to be written.  An append at a host position within them moves it, one
     at positions in device memory makes it None (as many as the caller knows of); what reads the cache by host positions, as the
