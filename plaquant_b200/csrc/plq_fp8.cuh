@@ -38,18 +38,6 @@ __device__ __forceinline__ uint32_t e4m3_split(float a, float b) {
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(lo) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
   return hi | static_cast<uint32_t>(lo) << 16;
 }
-// The same with the rest as E5M2 codes, whose smallest step is 2^-16.
-__device__ __forceinline__ uint32_t e4m3_e5m2_split(float a, float b) {
-  uint32_t x, back;
-  uint16_t hi, lo;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(x) : "f"(b), "f"(a));
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(hi) : "r"(x));
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(hi));
-  const __half2 rest = __hsub2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&back));
-  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(lo) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
-  return hi | static_cast<uint32_t>(lo) << 16;
-}
-
 // Instruction descriptor of kind::f8f6f4 with E4M3 operands and a float32 accumulator:
 //   [4,6) accumulator 1 = float32  [7,10), [10,13) operand formats 0 = E4M3  [15], [16] A, B with M / N contiguous instead of K
 //   [17,23) N / 8  [24,29) M / 16
@@ -71,7 +59,6 @@ __device__ __forceinline__ void tc_mma_e4m3(uint32_t d_tmem, uint32_t a_lo, uint
                  "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-constexpr uint32_t kIdescAE5m2 = 1u << 7;              // A as E5M2 instead of E4M3
 // The same with A in tensor memory (row = lane, four consecutive elements of K per 32-bit column), block-scaled (descriptor:
 // make_idesc): every row of A and of B has an E8M0 scale for the 32 elements of K, byte 0 of the
 // word that 512 bytes copied to these columns put there (row r: lane r % 32, column r / 32).

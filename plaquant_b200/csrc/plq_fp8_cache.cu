@@ -889,10 +889,9 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
 //   S      of 64 positions, twice in tensor memory: the product of block j + 2 is issued behind the one that reads the weights
 //          of block j, so the scores of j + 1 lie ready when the weights of j are done
 //   p      w = exp2(score + log2 vs - e + 8) with e the row's largest score + log2 vs in the block of 64, rounded up: the scale of
-//          V is part of the weight, and the block's largest is 128 to 256.  hi + lo, E4M3 + E5M2, in tensor memory (A operand),
-//          in the place of the scores they come from: off by at most 2^-8 + 2^-11 (f16 on the way) of itself, or by 2^-14
-//          below 2^-6: E4M3 leaves up to 2^-10 there, and E5M2 half of 2^-3 of that.  All steps of a block are 2^-15 of its
-//          largest.
+//          V is part of the weight, and the block's largest is 128 to 256.  hi + lo, both E4M3, in tensor memory (A operand), in
+//          the place of the scores they come from: off by at most 2^-9 + 2^-11 (f16 on the way) of itself or by half a step of
+//          2^-9, which is 2^-17 of the block's largest weight
 //   O      stays in tensor memory, in units of 2^R, R = e - 8 of the first block.  The tensor core applies 2^(e - 8 - R), an E8M0
 //          scale per row and 32 positions (kind::mxf8f6f4), so no block's weights share an exponent with another's: a long tail of
 //          small weights keeps its bits behind a position that outweighs each of them, and ordinary values behind a block of
@@ -1025,7 +1024,7 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                   // 32 positions each: codes of hi, then of lo
           tc_mma_mxf8_ts(o, p + 16 * h, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, p + 32, p + 36, j > 0 || h > 0);
-          tc_mma_mxf8_ts(o, p + 16 * h + 8, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o | kIdescAE5m2, p + 32, p + 36, 1u);
+          tc_mma_mxf8_ts(o, p + 16 * h + 8, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, p + 32, p + 36, 1u);
         }
         tc_commit<1>(smem_u32(&v_empty[st]));
         tc_commit<1>(smem_u32(j + 1 == n ? o_full : o_done));
@@ -1226,7 +1225,7 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
             w[y + 1] = ex2_approx(z.y);
             sum = __fadd2_rn(sum, make_float2(w[y], w[y + 1]));
           }
-          const uint32_t c0 = e4m3_e5m2_split(w[0], w[1]), c1 = e4m3_e5m2_split(w[2], w[3]);
+          const uint32_t c0 = e4m3_split(w[0], w[1]), c1 = e4m3_split(w[2], w[3]);
           p[d / 4] = __byte_perm(c0, c1, 0x5410);
           p[8 + d / 4] = __byte_perm(c0, c1, 0x7632);
         }

@@ -640,8 +640,8 @@ def fp8_cache_attention(q: torch.Tensor, cache, pos, scale: Optional[float] = No
     split.  Returns bf16 [B, T, heads, 128].
 
     Scores, maxima and sums are float32.  Queries and softmax weights are two 8-bit codes each: a weight is off by 2^-9 + 2^-11 of
-    itself, or by 2^-18 of the largest of its 64 positions, with up to 16 rows (T * heads / key heads), by 2^-8 + 2^-11 or 2^-21
-    with more; a query's elements below 2^-13 (2^-9 with more rows) of its largest are off by 2^-21 (2^-17) of that."""
+    itself, or by 2^-17 of the largest of its 64 positions (2^-18 with up to 16 rows, T * heads / key heads); a query's elements
+    below 2^-9 of its largest are off by 2^-17 of that (up to 16 rows: 2^-13 and 2^-21)."""
     scale = 128 ** -0.5 if scale is None else scale
     word, at = _status_words.get(q.get_device()), pos if isinstance(pos, torch.Tensor) else None
     out = None if word is None else _lib.torch_lib().fp8_attention(q, cache.k, cache.k_scale, cache.v, cache.v_scale, at, pos if at is None else 0,

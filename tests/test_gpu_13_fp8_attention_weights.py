@@ -27,11 +27,10 @@ def _cache(plq, batch, n, kv_heads, k, v, k_scale, v_scale):
 
 
 # Rounding of a weight, and what all fixed steps of a block of 64 positions add up to, of the block's own largest weight:
-#   up to 16 rows per key head ("few"): f16 (2^-11), then E4M3 + E4M3: half of 2^-3, of that rest half of 2^-3, 2^-9 in all; the
-#     block's largest is 2^8, below 2^-6 the step is 2^-9: 64 halves of it are 2^-4 = 2^-12 of 2^8
-#   more ("many"): f16, E4M3 + E5M2: half of 2^-3, of that rest half of 2^-2, 2^-8 in all; the block's largest is above 2^7,
-#     below 2^-6 a weight is off by 2^-14 at most: 64 of these are 2^-8 = 2^-15 of 2^7
-ROUND = {"few": (2.0 ** -9 + 2.0 ** -11, 2.0 ** -12), "many": (2.0 ** -8 + 2.0 ** -11, 2.0 ** -15)}
+#   f16 (2^-11), then E4M3 + E4M3: half of 2^-3, of that rest half of 2^-3, 2^-9 in all
+#   no step is below 2^-9: 64 halves of it are 2^-4, and the block's largest is 2^8 ("few": up to 16 rows per key head), or above 2^7
+#   ("many"): 2^-12 or 2^-11 of it
+ROUND = {"few": (2.0 ** -9 + 2.0 ** -11, 2.0 ** -12), "many": (2.0 ** -9 + 2.0 ** -11, 2.0 ** -11)}
 
 
 def _check(out, q, cache, pos, scale=128 ** -0.5):
@@ -70,7 +69,7 @@ SHAPES = [(1, 1, 1, 1), (1, 4, 4, 1), (1, 8, 4, 1), (12, 200, 8, 1), (3, 9, 8, 2
 @pytest.mark.parametrize("nats", [6.0, 12.0, 13.0, 14.0, 18.0])
 def test_a_long_flat_tail_behind_a_first_token(plq, b, t, heads, kv_heads, nats):
     """One position far above a tail of equal scores and equal values: the tail's part of the sum is the result.  Its weights may be
-    off by 2^-8 + 2^-11 each, all in the same direction; the 63 that share a block with the first may be lost beside it."""
+    off by 2^-9 + 2^-11 each, all in the same direction; the 63 that share a block with the first may be lost beside it."""
     n = 131072 if b == 1 else 16384
     k, v = torch.zeros(n, 128, device="cuda"), torch.ones(n, 128, device="cuda")
     k[0], v[0] = 1.0, 0.0
@@ -81,8 +80,8 @@ def test_a_long_flat_tail_behind_a_first_token(plq, b, t, heads, kv_heads, nats)
     above = math.exp(float(q[0, 0, 0, 0]) * 128 ** 0.5)
     tail = torch.arange(n - t, n, device="cuda", dtype=torch.float64)[None, :, None, None]       # positions behind the first that a query sees
     want = 0.5 * tail / (tail + above)
-    # a weight 2^-8 + 2^-11, the steps of a block 2^-12, the result's rounding 2^-8, the exponential of 18
-    assert float(((out.double() - want) / want).abs().max()) <= 2.0 ** -7 + 2.0 ** -11 + 2.0 ** -12 + 2.0 ** -16 + 63 / (n - t)
+    # a weight 2^-9 + 2^-11, the steps of a block 2^-11, the result's rounding 2^-8, the exponential of 18
+    assert float(((out.double() - want) / want).abs().max()) <= 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -10 + 2.0 ** -16 + 63 / (n - t)
     plq.check_device_status()
 
 
@@ -111,7 +110,7 @@ def test_a_channel_of_large_values_takes_nothing_from_the_others(plq, b, t, head
     w = torch.softmax(score.masked_fill(~seen, -math.inf), -1)
     want = (w * (v[:, 0] != 0)).sum(-1)
     err = (out[0][..., [0, 4, 6, 127]] / want[..., None] - 1).abs().max()
-    assert float(err) <= 2.0 ** -7 + 2.0 ** -11 + 2.0 ** -12 + 2.0 ** -19 * (1 + float(score.abs().max()))
+    assert float(err) <= 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -10 + 2.0 ** -19 * (1 + float(score.abs().max()))
     plq.check_device_status()
 
 
