@@ -60,8 +60,8 @@ __device__ __forceinline__ void tc_mma_e4m3(uint32_t d_tmem, uint32_t a_lo, uint
 }
 
 // The same with A in tensor memory (row = lane, four consecutive elements of K per 32-bit column), block-scaled (descriptor:
-// make_idesc): every row of A and of B has an E8M0 scale for the 32 elements of K, byte 0 of the
-// word that 512 bytes copied to these columns put there (row r: lane r % 32, column r / 32).
+// make_idesc): every row of A and of B has an E8M0 scale for the 32 elements of K, a byte of the word that 512 bytes copied
+// to these columns put there (row r: lane r % 32, column r / 32); which one, the descriptor and bits 30 and 31 of the address say.
 __device__ __forceinline__ void tc_mma_mxf8_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t sfa_tmem,
                                                uint32_t sfb_tmem, uint32_t accumulate) {
   asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %7, 0;\n\tmov.b64 db, {%2, %3};\n\t"

@@ -781,7 +781,7 @@ struct PfCfg {
   static constexpr int kBlock = kCacheBlock * kHeadDim; // 8 KiB: 64 positions of K or V
   static constexpr int kStages = 4;
   static constexpr int kScaleBytes = 512;               // 128 rows, a word each
-  static constexpr size_t kSmemBytes = 1024 + 2 * kTile + 2 * kStages * kBlock + 3 * kScaleBytes + 256;
+  static constexpr size_t kSmemBytes = 1024 + 2 * kTile + 2 * kStages * kBlock + 2 * kScaleBytes + 256;
   // 128 registers a thread at launch (256 x 128); the warps with a row of scores per thread take what the others leave.
   static constexpr int kRegsMain = 56, kRegsRows = 200;
   static_assert(128 * kRegsMain + 128 * kRegsRows <= 256 * 128, "register split");
@@ -923,9 +923,8 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
   uint8_t* q_s = smem;                                  // [hi | lo][128 x 128 bytes]
   uint8_t* k_s = q_s + 2 * C::kTile;
   uint8_t* v_s = k_s + C::kStages * C::kBlock;
-  uint8_t* w_scale_s = v_s + C::kStages * C::kBlock;    // scales of the weights of two blocks
-  uint8_t* one_s = w_scale_s + 2 * C::kScaleBytes;      // ... of V: one
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(one_s + C::kScaleBytes);
+  uint8_t* w_scale_s = v_s + C::kStages * C::kBlock;    // two blocks' words: byte 0 scale of the row's weights, byte 1 that of V (one)
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(w_scale_s + 2 * C::kScaleBytes);
   uint64_t* k_empty = k_full + C::kStages, *v_full = k_empty + C::kStages, *v_empty = v_full + C::kStages;
   uint64_t* q_full = v_empty + C::kStages, *s_full = q_full + 1, *p_full = s_full + 2, *o_done = p_full + 2, *o_full = o_done + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(o_full + 1);
@@ -946,8 +945,6 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
     tmem_alloc<1>(tmem_holder, 256);
     tmem_relinquish<1>();
   }
-  if (warp == 2) reinterpret_cast<uint4*>(one_s)[lane] = make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -996,7 +993,7 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
     }
   } else if (warp == 1) {
     if (elect_one() && n > 0) {
-      constexpr uint32_t idesc_s = make_idesc_e4m3(128, 64), idesc_o = make_idesc(0u /*E4M3*/, 128, 128, 1u /*E8M0*/) | kIdescBMnMajor;
+      constexpr uint32_t idesc_s = make_idesc_e4m3(128, 64), idesc_o = make_idesc(0u /*E4M3*/, 128, 128, 1u /*E8M0*/) | kIdescBMnMajor | (1u << 4 /*B: byte 1*/);
       bool ok = true;
       auto scores = [&](int j) {
         const int st = j % C::kStages;
@@ -1020,11 +1017,11 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
         tc_fence_after();
         const uint32_t v_lo = desc_lo_sw128(v_base + st * C::kBlock), p = tmem_base + 64 * (j & 1), o = tmem_base + 128;
         tc_cp_32x128b_warpx4<1>(p + 32, desc_lo_sf(smem_u32(w_scale_s + (j & 1) * C::kScaleBytes)), kDescHiSf);
-        tc_cp_32x128b_warpx4<1>(p + 36, desc_lo_sf(smem_u32(one_s)), kDescHiSf);
+        const uint32_t sfa = p + 32, sfb = sfa + (1u << 30);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                   // 32 positions each: codes of hi, then of lo
-          tc_mma_mxf8_ts(o, p + 16 * h, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, p + 32, p + 36, j > 0 || h > 0);
-          tc_mma_mxf8_ts(o, p + 16 * h + 8, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, p + 32, p + 36, 1u);
+          tc_mma_mxf8_ts(o, p + 16 * h, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, sfa, sfb, j > 0 || h > 0);
+          tc_mma_mxf8_ts(o, p + 16 * h + 8, v_lo + h * (4096 >> 4), kDescHiSw128, idesc_o, sfa, sfb, 1u);
         }
         tc_commit<1>(smem_u32(&v_empty[st]));
         tc_commit<1>(smem_u32(j + 1 == n ? o_full : o_done));
@@ -1206,7 +1203,7 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
       }
       e = fmaxf(e, R - kFarBelow);                      // a number whatever the scores are
       const uint32_t ws = static_cast<uint32_t>(max(1, min(__float2int_rn(e - R) + kScaleBias, kScaleTop)));
-      asm volatile("st.shared.b32 [%0], %1;" ::"r"(scale_at + (j & 1) * C::kScaleBytes), "r"(ws) : "memory");
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(scale_at + (j & 1) * C::kScaleBytes), "r"(ws | 0x7F00u) : "memory");
       fence_proxy_async_smem();
       // A block that the row sees and whose scale is NaN makes the row NaN, its masked positions included.
       const float shift = lv + 8.0f - e;
