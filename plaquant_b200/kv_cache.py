@@ -119,7 +119,7 @@ class Fp8Cache:
 
     def check(self, batch: int, kv_heads: int, device) -> None:
         """Raises unless this is a well-formed cache of `batch` sequences on `device`."""
-        if self.k.dim() != 4 or self.room < 1:
+        if self.k.dim() != 4 or self.room < 1 or kv_heads < 1:
             raise TypeError(f"cache.k must be uint8 [B, room, kv_heads, {HEAD_DIM}], it is {list(self.k.shape)}")
         room = self.room
         for name, c, s in (("k", self.k, self.k_scale), ("v", self.v, self.v_scale)):

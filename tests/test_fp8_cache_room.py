@@ -105,3 +105,8 @@ def test_forms_of_the_cache_that_were_accepted_before(value):
 def test_forms_of_the_cache_that_do_not_exist(value):
     with pytest.raises(ValueError):
         forward_pass.ResQForwardB200._check_kv_quant(value)
+
+
+def test_a_cache_without_heads_is_refused():
+    with pytest.raises(TypeError):
+        kv_cache.Fp8Cache.empty(1, 64, 0, "cpu").check(1, 0, torch.device("cpu"))
