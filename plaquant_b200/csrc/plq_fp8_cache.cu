@@ -216,10 +216,10 @@ __global__ void __launch_bounds__(256, 4) rope_kv_append_fp8_kernel(const Fp8App
 // different lengths load it evenly and no length has to be known on the host.  A run is one or several segments (tiles of one
 // sequence); a sequence that lies in several runs leaves partial sums, at most two per run (its first and its last segment),
 // which fp8_attention_join_kernel adds in a fixed order.
-// Bound by the cache's bytes for long ones: one sequence of 131072 positions (64 heads on 8) 52 us, 5.1 TB/s; 16 of 4096 (32 on 8)
-// 31 us, 4.3 TB/s, and 24 us of different lengths.  A tile is a chain of some 2000 cycles for a CTA (scores, maxima over the
+// Bound by the cache's bytes for long ones: one sequence of 131072 positions (64 heads on 8) 51 us, 5.2 TB/s; 16 of 4096 (32 on 8)
+// 31 us, 4.3 TB/s, and 25 us of different lengths.  A tile is a chain of some 2000 cycles for a CTA (scores, maxima over the
 // lanes, weights, product), which two CTAs per SM turn into the memory's rate; about 2.5 us before the first tile and 4 us for
-// the join come on top, which is what a short cache consists of (1 x 4096: 9.4 us).  A join in the kernel itself by the
+// the join come on top, which is what a short cache consists of (1 x 4096: 9.3 us).  A join in the kernel itself by the
 // last CTA of a sequence took 64 and 36 us: its counters are six round trips to L2.
 constexpr int kMaxFlat = 256;                          // sequences whose tiles are cut as one row
 
@@ -895,20 +895,20 @@ __global__ void __launch_bounds__(128) fp8_attention_join_kernel(const Fp8AttnAr
 //   O      stays in tensor memory, in units of 2^R, R = e - 8 of the first block.  The tensor core applies 2^(e - 8 - R), an E8M0
 //          scale per row and 32 positions (kind::mxf8f6f4), so no block's weights share an exponent with another's: a long tail of
 //          small weights keeps its bits behind a position that outweighs each of them, and ordinary values behind a block of
-//          large ones.  (With one running exponent for the row, weights 12 nats below it were off by up to 24 %, beyond 13 nats
-//          by 69 % or gone; moving it down with the blocks cost a rescaling of O for 20 to 27 % of the time.)  R moves only when a
-//          block is 2^60 above it.  The sum of the weights takes w / vs.
+//          large ones.  R moves only when a block is 2^60 above it.  The sum of the weights takes w / vs.  (With one running
+//          exponent for the row two prompts of 2048 take 82 us instead of 84, 104 instead of 87 where scores spread four times
+//          as wide and O is scaled often, but weights 12 nats below the row's largest are off by 24 % and those beyond 13 gone.)
 //   warp 0 producer, warp 1 MMA issuer, warps 4 - 7 the rows
 // 128 positions of two row tiles are 2048 cycles of the tensor core (four products of 128 x 128 x 128 each) and as many of
 // exponentials (16 a cycle).  They take 2.2 us (about 4000 cycles): without the weights' arithmetic 1.2 us, with exponentials
 // alone 1.9 us.  Bound by the instructions that turn scores into weights (some 11 an element, of which 3 the two codes), not by
 // their latency: twice the warps with half of the blocks each took 5 % longer, codes by integer arithmetic 3 to 5 % longer.
-// 8192 tokens of 32 heads on 8: 474 us (1.16 PFLOP/s); two prompts of 2048: 80 us.  Of these a CTA's beginning and end take
+// 8192 tokens of 32 heads on 8: 490 us (1.12 PFLOP/s); two prompts of 2048: 84 us.  Of these a CTA's beginning and end take
 // 6 us each; they were 12 with the loops over queries and output unrolled, since code that runs once costs its fetch, and with
 // both row tiles in one CTA nothing hid them: 102 us.  A CTA that took further work over from CTAs that had not started yet
 // (the next queries prepared meanwhile by two warps) was slower, 110 us: two warps take longer for that than the tiles before.
-// Few CTAs and a long past: each sequence is cut into runs, whose sums O and weight at their M go to the join (64 tokens of 32
-// heads on 8 behind 8000 positions 88 -> 25 us).
+// Few CTAs and a long past: each sequence is cut into runs, whose sums O and weight in units of their 2^R go to the join (64
+// tokens of 32 heads on 8 behind 8000 positions 88 -> 26 us).
 constexpr int kScaleBias = 127 - 8;                     // e - R = 8 is the scale one
 constexpr int kScaleTop = 127 + 60;                     // beyond it R moves: O stays below 2^60 * 2^8 * 448 * positions
 constexpr float kFarBelow = 92.0f;                      // blocks further below R than this share its scale, 2^-100
@@ -1202,7 +1202,8 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
         }
       }
       e = fmaxf(e, R - kFarBelow);                      // a number whatever the scores are
-      const uint32_t ws = static_cast<uint32_t>(max(1, min(__float2int_rn(e - R) + kScaleBias, kScaleTop)));
+      // e - R is a whole number from -92 to 68: the low byte of the sum's bits is the scale, without a conversion
+      const uint32_t ws = __float_as_uint((e - R) + (12582912.0f + kScaleBias)) & 0xFFu;
       asm volatile("st.shared.b32 [%0], %1;" ::"r"(scale_at + (j & 1) * C::kScaleBytes), "r"(ws | 0x7F00u) : "memory");
       fence_proxy_async_smem();
       // A block that the row sees and whose scale is NaN makes the row NaN, its masked positions included.
@@ -1376,8 +1377,8 @@ static AttnPlan attn_plan(int64_t batch, int64_t t, int64_t heads, int64_t kv_he
   }
   // More rows: the kernel with 128 of them per CTA, every sequence whole or in runs of its own.  A tile takes a CTA 1.4 us, with a
   // second one on the SM 2.2; runs cost 5 us and 0.3 for every 128 rows.  8 key heads with 4 heads each behind 8000 positions,
-  // whole / in runs: 9 tokens 88 / 16 us, 64 tokens 88 / 25, 256 tokens 90 / 65; four sequences of 128 tokens 90 / 116.
-  // (The other kernel with 32 rows takes 2.6 us a tile: 8 tokens of 16 sequences behind 4000 positions 60 us, here 48.)
+  // whole / in runs: 9 tokens 88 / 16 us, 64 tokens 88 / 26, 256 tokens 90 / 66; four sequences of 128 tokens 93 / 116.
+  // (The other kernel with 32 rows takes 2.6 us a tile: 8 tokens of 16 sequences behind 4000 positions 60 us, here 50.)
   const int64_t many = batch * kv_heads * ((rows + 127) / 128);
   int64_t split = slots / many;
   if (split > tiles / 4) split = tiles / 4;
