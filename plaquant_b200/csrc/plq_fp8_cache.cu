@@ -282,6 +282,10 @@ __device__ __forceinline__ bool softmax_barrier(bool ok = true) {
 }
 
 constexpr float kNegInf = -__builtin_huge_valf();
+// Behind scores (base 2) far beyond 2^21 the 8 of 8 - m has no bits left and the weights would be anything.  Inside a block such
+// scores are scaled down to 2^21, so that differences of 2^-21 of their size are one; between blocks they count as they are.
+constexpr float kVast = 2097152.0f;
+__device__ __forceinline__ float vast_factor(float m) { return fminf(1.0f, kVast * rcp_approx(fabsf(m))); }
 
 template <int R>
 __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -662,9 +666,10 @@ __global__ void __launch_bounds__(192, 2) fp8_attention_kernel(const __grid_cons
         f[lane] = m_run > kNegInf ? ex2_approx(m_run - m_new) : 0.0f;
         f[R + lane] = b0 * nv0;
         f[2 * R + lane] = b1 * nv1;
-        my_max[lane] = m > kNegInf ? 8.0f - m : 0.0f;
+        const float v = vast_factor(m);
+        my_max[lane] = m > kNegInf ? fmaf(-m, v, 8.0f) : 0.0f;
         my_max[R + lane] = second ? b1 : b0;
-        my_max[2 * R + lane] = ksc;
+        my_max[2 * R + lane] = ksc * v;
         m_run = m_new;
       }
       __syncwarp();
@@ -1139,7 +1144,7 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
     for (int j = 0; ok && j < n; ++j) {
       const int t0 = (j0 + j) * kCacheBlock;
       const bool sees = lim >= t0;
-      float ck = sees ? next_k * per_k : 1.0f;
+      float ck = sees ? next_k * per_k : 0.0f;
       if (ck < 1.2e-38f) ck = 1.2e-38f;                 // a score of zero, and minus infinity stays what it is
       float vs = sees ? next_v : 1.0f;
       if (vs < 1e-36f) vs = 1e-36f;
@@ -1167,7 +1172,9 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
       for (int d = 0; d < 4; ++d) m[d] = fmaxf(__uint_as_float(v[0][d]), __uint_as_float(v[1][d]));
 #pragma unroll
       for (int d = 4; d < 32; ++d) m[d & 3] = fmaxf(m[d & 3], fmaxf(__uint_as_float(v[0][d]), __uint_as_float(v[1][d])));
-      const float t_max = fmaf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), ck, lv);
+      const float s_max = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), t_max = fmaf(s_max, ck, lv);
+      ck *= vast_factor(t_max);
+      if (ck < 1.2e-38f) ck = 1.2e-38f;
       float e = ceilf(t_max);
       if (j == 0) {
         R = e > kNegInf ? e - 8.0f : 0.0f;
@@ -1207,7 +1214,7 @@ __global__ void __launch_bounds__(256, 2) fp8_prefill_kernel(const __grid_consta
       asm volatile("st.shared.b32 [%0], %1;" ::"r"(scale_at + (j & 1) * C::kScaleBytes), "r"(ws | 0x7F00u) : "memory");
       fence_proxy_async_smem();
       // A block that the row sees and whose scale is NaN makes the row NaN, its masked positions included.
-      const float shift = lv + 8.0f - e;
+      const float shift = fmaf(-fmaxf(s_max, -3e38f), ck, (t_max - e) + 8.0f);
       const float2 ck2 = make_float2(ck, ck), shift2 = make_float2(shift, shift);
       float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll

@@ -211,3 +211,27 @@ def test_a_workspace_needs_no_more_than_sixteen_bytes_of_alignment(plq, b, t, he
         first = at - room.data_ptr()
         assert torch.equal(out, want) and torch.all(room[:first] == 0xA5) and torch.all(room[first + need:] == 0xA5)
     plq.check_device_status()
+
+
+@pytest.mark.parametrize("t,heads,kv_heads,n", [(1, 4, 1, 300), (1, 8, 2, 5000), (4, 4, 1, 700), (40, 4, 2, 300), (40, 8, 2, 5000), (300, 2, 2, 300)])
+@pytest.mark.parametrize("scale", [1e3, 1e6, 1e8, -1e8, 1e12, 1e25])
+def test_scores_beyond_what_float32_counts(plq, t, heads, kv_heads, n, scale):
+    """Scores so large that their differences are millions: the largest one's value is the result, wherever it is well apart (a
+    score is off by 2^-21 of its size, and differences count in units of that: 2^-14 of it are 128)."""
+    g = torch.Generator(device="cuda").manual_seed(n + t)
+    k, v = (torch.randn(n, 128, generator=g, device="cuda") for _ in range(2))
+    cache = _cache(plq, 2, n, kv_heads, k, v, torch.full((-(-n // BLOCK),), 0.5, device="cuda"), torch.ones(-(-n // BLOCK), device="cuda"))
+    q = torch.randn(2, t, heads, 128, generator=g, device="cuda").to(torch.bfloat16)
+    kk, vv = (x.view(torch.float8_e4m3fn).double() for x in (cache.k[0, :, 0], cache.v[0, :, 0]))
+    score = (q.double() @ kk.t()) * 0.5 * scale
+    score = score.masked_fill(torch.arange(n, device="cuda") > n - t + torch.arange(t, device="cuda")[:, None, None], -math.inf)
+    best, at = score.topk(2, -1)
+    size = score.masked_fill(score == -math.inf, 0.0).abs().amax(-1)
+    clear = (best[..., 0] - best[..., 1] > 2.0 ** -14 * size + 30.0) & (at[..., 0] >= 0)
+    assert clear.double().mean() > 0.9
+    out = plq.ops.fp8_cache_attention(q, cache, n - t, scale=scale).double()
+    want = vv[at[..., 0]]
+    # the weight 2^-9 + 2^-11, the result 2^-8; what is left of the others e^-30 each
+    err = (out - want).abs() - want.abs() * (2.0 ** -8 + 2.0 ** -9 + 2.0 ** -11) - 1e-8
+    assert out.isfinite().all() and float(err[clear].max()) <= 0
+    plq.check_device_status()
