@@ -422,7 +422,7 @@ class ResQForwardB200:
         """The E4M3 cache of layer `li` with room for positions up to pos0 + t; a longer one takes over what it held."""
         need = pos0 + t
         if pos0 == 0:
-            self.kv[li] = kv_cache.Fp8Cache.empty(b, -(-need // 64) * 64 + 64, self.kv_heads, self.device)
+            self.kv[li] = kv_cache.Fp8Cache.empty(b, -(-need // 64) * 64 + 64, self.kv_heads, self.device, length=0)
         cache = self.kv[li]
         if not isinstance(cache, kv_cache.Fp8Cache) or not 0 <= pos0 <= (cache.room if cache.length is None else cache.length):
             raise RuntimeError(f"the cache of layer {li} does not hold the {pos0} positions in front of the new ones")

@@ -89,9 +89,9 @@ class Fp8Cache:
     64 positions and head, a power of two: value = code * scale.  Positions nobody has written may hold anything.
     ops.rope_kv_append_fp8 fills it in place, ops.fp8_cache_attention reads it; 1.0005 bytes per element, a bf16 cache has 2.
 
-    `length`: how many leading positions the host knows to be written.  An append at a host position within them moves it, one
-    at positions in device memory makes it None (as many as the caller knows of); what reads the cache by host positions, as the
-    decoder does, refuses to begin behind it."""
+    `length`: how many leading positions are written, where the host keeps count (the decoder does for its caches), else None.
+    An append at a host position within them moves it, one at positions in device memory makes it None.  The decoder refuses to
+    begin behind it; without one the room is the limit, and what lies there is the caller's to answer for."""
     k: torch.Tensor           # u8 [B, room, kv_heads, 128]
     k_scale: torch.Tensor     # float32 [B, kv_heads, ceil(room / 64)]
     v: torch.Tensor
@@ -99,11 +99,12 @@ class Fp8Cache:
     length: Optional[int] = None
 
     @classmethod
-    def empty(cls, batch: int, room: int, kv_heads: int, device) -> "Fp8Cache":
+    def empty(cls, batch: int, room: int, kv_heads: int, device, length: Optional[int] = None) -> "Fp8Cache":
+        """Nothing written yet: `length` is 0 for a cache whose positions are to be counted."""
         def side():
             return (torch.empty(batch, room, kv_heads, HEAD_DIM, dtype=torch.uint8, device=device),
                     torch.empty(batch, kv_heads, -(-room // CACHE_BLOCK), dtype=torch.float32, device=device))
-        return cls(*side(), *side(), 0)
+        return cls(*side(), *side(), length)
 
     @property
     def batch(self) -> int:

@@ -58,7 +58,7 @@ def test_a_cache_put_back_keeps_its_length(model):
     assert _step(model, 1, 70).length == 71
     grown = kept.grown(1000)
     assert grown.length == 71 and grown.room == 1000
-    other = kv_cache.Fp8Cache.empty(2, 200, 2, "cpu")
+    other = kv_cache.Fp8Cache.empty(2, 200, 2, "cpu", length=0)
     assert other.length == 0
     other.copy_from(kept, 33)
     assert other.length == 33
@@ -67,15 +67,18 @@ def test_a_cache_put_back_keeps_its_length(model):
 
 
 def test_a_cache_of_the_callers_own_is_the_callers_to_answer_for(model):
-    """Filled at positions in device memory, or made from tensors: the host does not know its length, the room is the limit."""
-    cache = kv_cache.Fp8Cache.empty(2, 100, 2, "cpu")
+    """Filled at positions in device memory, by copies or made from tensors: the host does not count, the room is the limit."""
+    own = kv_cache.Fp8Cache.empty(2, 100, 2, "cpu")
+    own.appended(0, 10)
+    assert own.length is None
+    cache = kv_cache.Fp8Cache.empty(2, 100, 2, "cpu", length=0)
     cache.appended(torch.tensor([5, 9]), 1)
     assert cache.length is None
     cache.appended(3, 1)
     assert cache.length is None
     made = kv_cache.Fp8Cache(cache.k, cache.k_scale, cache.v, cache.v_scale)
     assert made.length is None and made.clone().length is None
-    for c in (cache, made):
+    for c in (own, cache, made):
         model.kv[0] = c
         assert model._fp8_room(0, 2, 1, 99) is c
         with pytest.raises(RuntimeError):
@@ -86,7 +89,7 @@ def test_a_cache_of_the_callers_own_is_the_callers_to_answer_for(model):
 
 
 def test_an_append_with_a_gap_leaves_the_length():
-    cache = kv_cache.Fp8Cache.empty(1, 100, 1, "cpu")
+    cache = kv_cache.Fp8Cache.empty(1, 100, 1, "cpu", length=0)
     cache.appended(4, 10)
     assert cache.length == 0
     cache.appended(-1, 10)

@@ -42,7 +42,7 @@ def test_a_gap_behind_the_prompt_is_refused(plq):
 
 def test_the_append_keeps_the_length(plq):
     from plaquant_b200 import kv_cache
-    cache = kv_cache.Fp8Cache.empty(1, 100, 1, "cuda")
+    cache = kv_cache.Fp8Cache.empty(1, 100, 1, "cuda", length=0)
     qkv, one = torch.ones(1, 5, 3 * 128, dtype=torch.bfloat16, device="cuda"), torch.ones(5, 128, device="cuda")
     plq.ops.rope_kv_append_fp8(qkv, one, one, 1, 1, cache, 0)
     plq.ops.rope_kv_append_fp8(qkv, one, one, 1, 1, cache, 5)
